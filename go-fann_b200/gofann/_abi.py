@@ -20,12 +20,13 @@ OK = 0
 ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_CAPACITY, ERR_TIMEOUT = -1, -2, -3, -4, -5
 EARLY_STOP_FIXED, EARLY_STOP_OFF, EARLY_STOP_ADAPTIVE = 0, 1, 2
 SCORER_PQ, SCORER_RABITQ = 0, 1
-DTYPE_U8, DTYPE_F32, DTYPE_F16 = 0, 1, 2
+DTYPE_U8, DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2, 3  # BF16: the cache operators only
 PQ_LUT_GLOBAL, PQ_LUT_SHARED, PQ_DIRECT, PQ_U8 = 0, 1, 2, 3
 TABLE_MODES = (PQ_LUT_GLOBAL, PQ_LUT_SHARED)  # modes that read a per-query table batch
 GEMM_TF32, GEMM_TF32X3 = 0, 1
 MAX_DEGREE, MAX_QUEUE, MAX_TOPK, MAX_RESULT_WIDTH, MAX_SHORTLIST = 64, 512, 10, 512, 400
 PQ_CENTROIDS, HASH_CAPACITY = 256, 4096
+KV_PAGE, KV_GROUP, KV_MAX_SELECT = 64, 64, 1024
 U32MAX = 0xFFFFFFFF
 FLT_MAX = float(np.finfo(np.float32).max)
 
@@ -117,6 +118,34 @@ class BatchParams(C.Structure):
 class SearchOut(C.Structure):
     _fields_ = [("ids", P), ("dists", P), ("steps", P), ("counters", P), ("status", P), ("trace", P),
                 ("trace_width", U32), ("reserved", U32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("pages", P), ("bounds", P), ("bound_scale", P), ("n_pages", U32), ("n_kv_heads", U32),
+                ("head_dim", U32), ("reserved", U32)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("page_table", P), ("seq_len", P), ("row_offset", P), ("status", P), ("n_seqs", U32),
+                ("max_pages", U32), ("n_rows", U32), ("max_rows", U32)]
+
+
+class KvAppendParams(C.Structure):
+    _fields_ = [("q", P), ("k", P), ("v", P), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("v_stride", C.c_uint64), ("cos", P), ("sin", P), ("positions", P), ("q_out", P), ("k_out", P),
+                ("v_out", P), ("dtype", I32), ("n_heads", U32), ("n_positions", U32), ("rotary_dim", U32),
+                ("interleaved", I32), ("reserved", U32)]
+
+
+class KvSelectParams(C.Structure):
+    _fields_ = [("q", P), ("q_stride", C.c_uint64), ("ids", P), ("scores", P), ("dtype", I32), ("n_heads", U32),
+                ("n_select", U32), ("n_first", U32), ("n_recent", U32), ("reserved", U32)]
+
+
+class KvAttentionParams(C.Structure):
+    _fields_ = [("q", P), ("q_stride", C.c_uint64), ("selected", P), ("key_bits", P), ("out", P), ("lse", P),
+                ("scale", C.c_float), ("dtype", I32), ("n_heads", U32), ("n_select", U32), ("key_words", U32),
+                ("causal", I32), ("window", U32), ("reserved", U32)]
 
 
 def ptr(x) -> int | None:
@@ -282,6 +311,10 @@ def lib() -> C.CDLL:
                                 C.POINTER(SearchParams), C.POINTER(SearchOut), sp, C.c_size_t, sp],
         "gofann_exact_posting_scan": [sp, C.c_int, U32, U32, sp, C.POINTER(Attrs), C.POINTER(Routes), sp, sp, sp,
                                       I32, sp, sp, sp],
+        "gofann_kv_append": [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAppendParams), sp],
+        "gofann_kv_select": [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvSelectParams), sp, C.c_size_t, sp],
+        "gofann_kv_attention": [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAttentionParams), sp, C.c_size_t,
+                                sp],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -301,6 +334,13 @@ def lib() -> C.CDLL:
     L.gofann_row_record_stride.argtypes = [U32]
     L.gofann_row_record_stride.restype = C.c_size_t
     L.gofann_search_batch_scratch_bytes.restype = C.c_size_t
+    L.gofann_kv_chunk_bytes.argtypes = [U32]
+    L.gofann_kv_chunk_bytes.restype = C.c_size_t
+    L.gofann_kv_select_scratch_bytes.argtypes = [C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvSelectParams)]
+    L.gofann_kv_select_scratch_bytes.restype = C.c_size_t
+    L.gofann_kv_attention_scratch_bytes.argtypes = [C.POINTER(KvCache), C.POINTER(KvBatch),
+                                                    C.POINTER(KvAttentionParams)]
+    L.gofann_kv_attention_scratch_bytes.restype = C.c_size_t
     _LIB = L
     return L
 
@@ -327,7 +367,9 @@ EXPORTED = ("gofann_abi_version", "gofann_last_error", "gofann_device_sm_count",
             "gofann_search_batch", "gofann_rerank", "gofann_route_merge", "gofann_shard_merge",
             "gofann_row_record_stride", "gofann_build_row_records", "gofann_offset_ids",
             "gofann_exact_search_scratch_bytes", "gofann_exact_search", "gofann_exact_posting_scan",
-            "gofann_string_peq", "gofann_plan_categorical")
+            "gofann_string_peq", "gofann_plan_categorical", "gofann_kv_chunk_bytes", "gofann_kv_append",
+            "gofann_kv_select_scratch_bytes", "gofann_kv_select", "gofann_kv_attention_scratch_bytes",
+            "gofann_kv_attention")
 
 
 def header_symbols(header: str | os.PathLike | None = None) -> list[str]:

@@ -1,0 +1,286 @@
+"""A language model's key/value cache in 4 bits, searched like an index.
+
+The cache operators of the C ABI (gofann_kv_append, gofann_kv_select,
+gofann_kv_attention) on torch-managed device memory: new rows are rotated and
+written in 4 bits, an int8 bound picks the blocks that a query reads, and
+attention reads all blocks or the picked ones.
+
+    cache = KVCache.empty(n_pages, n_kv_heads, head_dim)
+    cos, sin = rope_tables(max_positions, rotary_dim)
+    batch = KVBatch(page_table, seq_len, row_offset, n_rows, max_rows)
+    q, _, _ = cache.append(batch, q, k, v, cos=cos, sin=sin, rotary_dim=rotary_dim)
+    ids, _ = cache.select(batch, q, n_select=64, first=1, recent=2)
+    out, lse = cache.attend(batch, q, selected=ids)
+
+Calls run on the current stream of the cache's device (or on `stream`).
+Scratch belongs to the batch object, so calls of one batch object are ordered
+on one stream.  There is no CPU or torch fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _abi as A
+
+PAGE, GROUP = A.KV_PAGE, A.KV_GROUP
+DTYPES = {torch.bfloat16: A.DTYPE_BF16, torch.float16: A.DTYPE_F16}
+
+
+def chunk_bytes(head_dim: int) -> int:
+    """Bytes of one (page, key/value head)."""
+    n = int(A.lib().gofann_kv_chunk_bytes(head_dim))
+    if n == 0:
+        raise ValueError(f"head_dim {head_dim} is not supported (64 or 128)")
+    return n
+
+
+def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, scaling: str = "none",
+                factor: float = 1.0, original: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                magnitude: float | None = None, device="cuda"):
+    """cos and sin tables [n_positions][rotary_dim / 2] (f32, computed in f64).
+
+    scaling "none"; "linear": positions divided by `factor`; "ntk": the base
+    raised to base * factor^(r / (r - 2)), which leaves the fastest pair alone
+    and slows the slowest by `factor`; "parts": pairs that turn more than
+    `beta_fast` times over the `original` context keep their frequency, those
+    below `beta_slow` turns are divided by `factor`, with a linear ramp in the
+    pair index between.  `magnitude` multiplies both tables (default 1, for
+    "parts" 0.1 ln(factor) + 1)."""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even")
+    if scaling not in ("none", "linear", "ntk", "parts"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if not factor >= 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(rotary_dim, 1))
+    if scaling == "linear":
+        freq = freq / factor
+    if scaling == "parts":
+        if original <= 0:
+            raise ValueError('"parts" needs the original context length')
+
+        def pair(turns: float) -> float:  # the pair that turns this often over the original context
+            return rotary_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))
+
+        lo = max(math.floor(pair(beta_fast)), 0)
+        hi = min(math.ceil(pair(beta_slow)), max(rotary_dim // 2 - 1, 0))
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - ramp) + freq / factor * ramp
+        if magnitude is None:
+            magnitude = 0.1 * math.log(factor) + 1.0
+    m = 1.0 if magnitude is None else magnitude
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+    return (angle.cos() * m).float(), (angle.sin() * m).float()
+
+
+def _rows(x: torch.Tensor, heads: int, dim: int, dtype, name: str) -> tuple[int, int]:
+    """Address and row stride of [rows][heads][dim] with contiguous heads."""
+    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim:
+        raise ValueError(f"{name} must be [rows][{heads}][{dim}], got {tuple(x.shape)}")
+    if x.dtype != dtype:
+        raise TypeError(f"{name} is {x.dtype}, not {dtype}")
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
+        raise ValueError(f"{name}: the heads of a row must be contiguous")
+    stride = x.stride(0) if x.shape[0] > 1 else heads * dim
+    return x.data_ptr(), stride
+
+
+def _out(x: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, name: str) -> torch.Tensor:
+    if x is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if tuple(x.shape) != shape or x.dtype != dtype or not x.is_contiguous() or x.device != like.device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {like.device}")
+    return x
+
+
+class KVBatch:
+    """The sequences of a call and their query rows (gofann_kv_batch).
+
+    page_table int32 [n_seqs][max_pages], seq_len int32 [n_seqs] (tokens in
+    the cache, this call's rows among them), row_offset int32 [n_seqs + 1].
+    The tensors stay on the device and may be updated in place between calls;
+    n_rows = row_offset[-1] and max_rows, the longest sequence's rows, are the
+    host's."""
+
+    def __init__(self, page_table: torch.Tensor, seq_len: torch.Tensor, row_offset: torch.Tensor, n_rows: int,
+                 max_rows: int, status: torch.Tensor | None = None):
+        for name, t in (("page_table", page_table), ("seq_len", seq_len), ("row_offset", row_offset)):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 tensor")
+            if t.device != page_table.device:
+                raise ValueError(f"{name} is on {t.device}, page_table on {page_table.device}")
+        n_seqs = int(seq_len.shape[0])
+        if page_table.dim() != 2 or page_table.shape[0] != n_seqs or tuple(row_offset.shape) != (n_seqs + 1,):
+            raise ValueError("page_table [n_seqs][max_pages], seq_len [n_seqs] and row_offset [n_seqs + 1] disagree")
+        if n_rows < 0 or not 0 <= max_rows <= n_rows:
+            raise ValueError(f"n_rows {n_rows} and max_rows {max_rows}")
+        self.page_table, self.seq_len, self.row_offset = page_table, seq_len, row_offset
+        self.n_rows, self.max_rows = int(n_rows), int(max_rows)
+        self.status = status if status is not None else torch.zeros(1, dtype=torch.int32, device=page_table.device)
+        self.struct = A.KvBatch(page_table=page_table.data_ptr(), seq_len=seq_len.data_ptr(),
+                                row_offset=row_offset.data_ptr(), status=self.status.data_ptr(), n_seqs=n_seqs,
+                                max_pages=int(page_table.shape[1]), n_rows=self.n_rows, max_rows=self.max_rows)
+        self._ref = C.byref(self.struct)
+        self._scratch = None
+
+    def scratch(self, n_bytes: int) -> int:
+        """Address of at least n_bytes of device scratch (kept, grown on demand)."""
+        if self._scratch is None or self._scratch.numel() < n_bytes:
+            self._scratch = torch.empty(max(n_bytes, 256), dtype=torch.uint8, device=self.page_table.device)
+        return self._scratch.data_ptr()
+
+    def check(self) -> None:
+        """Raises where a call found a page, position, length or row out of range (synchronises)."""
+        if int(self.status.item()) != A.OK:
+            status = int(self.status.item())
+            self.status.zero_()
+            raise A.GofannError(status, "kv cache call (device)")
+
+
+class KVCache:
+    """Pages of a 4-bit key/value cache and the int8 bounds of their blocks."""
+
+    def __init__(self, head_dim: int, pages: torch.Tensor | None = None, bounds: torch.Tensor | None = None,
+                 bound_scale: torch.Tensor | None = None):
+        size = chunk_bytes(head_dim)
+        first = pages if pages is not None else bounds
+        if first is None:
+            raise ValueError("a cache needs pages or bounds")
+        n_pages, n_kv = int(first.shape[0]), int(first.shape[1])
+        if pages is not None and (tuple(pages.shape) != (n_pages, n_kv, size) or pages.dtype != torch.uint8 or
+                                  not pages.is_contiguous()):
+            raise ValueError(f"pages must be contiguous uint8 [n_pages][n_kv_heads][{size}]")
+        if (bounds is None) != (bound_scale is None):
+            raise ValueError("bounds and bound_scale go together")
+        if bounds is not None and (tuple(bounds.shape) != (n_pages, n_kv, 2, head_dim) or bounds.dtype != torch.int8 or
+                                   tuple(bound_scale.shape) != (n_pages, n_kv) or bound_scale.dtype != torch.float32 or
+                                   not bounds.is_contiguous() or not bound_scale.is_contiguous()):
+            raise ValueError(f"bounds must be contiguous int8 [n_pages][n_kv_heads][2][{head_dim}] and bound_scale "
+                             "float32 [n_pages][n_kv_heads]")
+        self.head_dim, self.n_kv_heads, self.n_pages = head_dim, n_kv, n_pages
+        self.pages, self.bounds, self.bound_scale = pages, bounds, bound_scale
+        self.device = first.device
+        self._lib = A.lib()
+        self.struct = A.KvCache(pages=A.ptr(pages), bounds=A.ptr(bounds), bound_scale=A.ptr(bound_scale),
+                                n_pages=n_pages, n_kv_heads=n_kv, head_dim=head_dim)
+        self._ref = C.byref(self.struct)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv_heads: int, head_dim: int, device="cuda") -> "KVCache":
+        """An empty cache (pages hold nothing until rows are appended)."""
+        return cls(head_dim,
+                   pages=torch.zeros((n_pages, n_kv_heads, chunk_bytes(head_dim)), dtype=torch.uint8, device=device),
+                   bounds=torch.zeros((n_pages, n_kv_heads, 2, head_dim), dtype=torch.int8, device=device),
+                   bound_scale=torch.zeros((n_pages, n_kv_heads), dtype=torch.float32, device=device))
+
+    def _stream(self, stream) -> int:
+        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+
+    def _heads(self, q: torch.Tensor) -> int:
+        if q.dim() != 3 or q.shape[1] % self.n_kv_heads:
+            raise ValueError(f"queries must be [rows][heads][{self.head_dim}] with heads a multiple of {self.n_kv_heads}")
+        if q.dtype not in DTYPES:
+            raise TypeError(f"queries are {q.dtype}, not bfloat16 or float16")
+        return int(q.shape[1])
+
+    def append(self, batch: KVBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos=None, sin=None,
+               rotary_dim: int = 0, interleaved: bool = False, positions=None, q_out=None, k_out=None, v_out=None,
+               held: bool = False, stream=None):
+        """Rotates q and k, writes k and v to the pages, renews the touched bounds.
+
+        Returns the rotated queries and, where k_out / v_out are given or
+        `held` is set, the keys and values as the cache holds them (else None)."""
+        d, n_kv, n = self.head_dim, self.n_kv_heads, batch.n_rows
+        dtype = k.dtype
+        if dtype not in DTYPES:
+            raise TypeError(f"keys are {dtype}, not bfloat16 or float16")
+        p = A.KvAppendParams()
+        p.k, p.k_stride = _rows(k, n_kv, d, dtype, "k")
+        p.v, p.v_stride = _rows(v, n_kv, d, dtype, "v")
+        heads = n_kv
+        if q is not None:
+            heads = self._heads(q)
+            p.q, p.q_stride = _rows(q, heads, d, dtype, "q")
+            q_out = _out(q_out, (n, heads, d), dtype, k, "q_out")
+            p.q_out = q_out.data_ptr()
+        if any(x is not None and x.shape[0] != n for x in (q, k, v)):
+            raise ValueError(f"q, k and v must have the batch's {n} rows")
+        if held or k_out is not None:
+            k_out = _out(k_out, (n, n_kv, d), dtype, k, "k_out")
+            p.k_out = k_out.data_ptr()
+        if held or v_out is not None:
+            v_out = _out(v_out, (n, n_kv, d), dtype, k, "v_out")
+            p.v_out = v_out.data_ptr()
+        if rotary_dim:
+            for t in (cos, sin):
+                if t is None or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
+                        t.shape[1] != rotary_dim // 2 or t.shape != cos.shape:
+                    raise ValueError(f"cos and sin must be contiguous float32 [positions][{rotary_dim // 2}]")
+            p.cos, p.sin, p.n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        if positions is not None:
+            if positions.dtype != torch.int32 or tuple(positions.shape) != (n,) or not positions.is_contiguous():
+                raise ValueError("positions must be contiguous int32 [n_rows]")
+            p.positions = positions.data_ptr()
+        p.dtype, p.n_heads = DTYPES[dtype], heads
+        p.rotary_dim, p.interleaved = rotary_dim, int(interleaved)
+        A.check(self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), self._stream(stream)), "gofann_kv_append")
+        return q_out if q is not None else None, k_out, v_out
+
+    def select(self, batch: KVBatch, q: torch.Tensor, n_select: int, first: int = 1, recent: int = 1, ids=None,
+               scores=None, stream=None):
+        """Blocks that each row and key/value head reads: ids int32 and scores
+        f32 [n_rows][n_kv_heads][n_select], ascending blocks, -1 / -inf fill."""
+        heads, n = self._heads(q), batch.n_rows
+        p = A.KvSelectParams()
+        p.q, p.q_stride = _rows(q, heads, self.head_dim, q.dtype, "q")
+        if q.shape[0] != n:
+            raise ValueError(f"q must have the batch's {n} rows")
+        shape = (n, self.n_kv_heads, n_select)
+        ids = _out(ids, shape, torch.int32, q, "ids")
+        scores = _out(scores, shape, torch.float32, q, "scores")
+        p.ids, p.scores = ids.data_ptr(), scores.data_ptr()
+        p.dtype, p.n_heads, p.n_select, p.n_first, p.n_recent = DTYPES[q.dtype], heads, n_select, first, recent
+        ref = C.byref(p)
+        need = self._lib.gofann_kv_select_scratch_bytes(self._ref, batch._ref, ref)
+        A.check(self._lib.gofann_kv_select(self._ref, batch._ref, ref, batch.scratch(need), need, self._stream(stream)),
+                "gofann_kv_select")
+        return ids, scores
+
+    def attend(self, batch: KVBatch, q: torch.Tensor, scale: float | None = None, causal: bool = True, window: int = 0,
+               selected=None, key_bits=None, out=None, lse=None, stream=None):
+        """softmax(scale q.K^T) V over the cache: out like q, lse f32 [n_rows][heads].
+
+        selected int32 [n_rows][n_kv_heads][width]: the blocks that each row
+        reads (select's ids); key_bits int32 [n_seqs][words]: a bit per token,
+        0 hides it (filtered out or evicted).  scale defaults to
+        head_dim^-0.5."""
+        heads, n, d = self._heads(q), batch.n_rows, self.head_dim
+        p = A.KvAttentionParams()
+        p.q, p.q_stride = _rows(q, heads, d, q.dtype, "q")
+        if q.shape[0] != n:
+            raise ValueError(f"q must have the batch's {n} rows")
+        out = _out(out, (n, heads, d), q.dtype, q, "out")
+        lse = _out(lse, (n, heads), torch.float32, q, "lse")
+        p.out, p.lse = out.data_ptr(), lse.data_ptr()
+        if selected is not None:
+            if selected.dtype != torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
+                    tuple(selected.shape[:2]) != (n, self.n_kv_heads):
+                raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width]")
+            p.selected, p.n_select = selected.data_ptr(), selected.shape[2]
+        if key_bits is not None:
+            if key_bits.dtype != torch.int32 or key_bits.dim() != 2 or not key_bits.is_contiguous() or \
+                    key_bits.shape[0] != batch.struct.n_seqs:
+                raise ValueError("key_bits must be contiguous int32 [n_seqs][words]")
+            p.key_bits, p.key_words = key_bits.data_ptr(), key_bits.shape[1]
+        p.scale = d ** -0.5 if scale is None else scale
+        p.dtype, p.n_heads, p.causal, p.window = DTYPES[q.dtype], heads, int(causal), window
+        ref = C.byref(p)
+        need = self._lib.gofann_kv_attention_scratch_bytes(self._ref, batch._ref, ref)
+        A.check(self._lib.gofann_kv_attention(self._ref, batch._ref, ref, batch.scratch(need), need,
+                                              self._stream(stream)), "gofann_kv_attention")
+        return out, lse

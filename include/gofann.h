@@ -44,6 +44,8 @@
  *   gofann_plan_categorical   greedy_min_posting routing + route_predicate::compile (host)
  *                                                     src/data/dataloader.cpp:7833, 10972;
  *                                                     src/planning/route_predicate_plan.h:175-315
+ *   gofann_kv_*               (no reference counterpart: the same cheap-score, shortlist and exact
+ *                             stages over a language model's key/value cache)
  */
 #ifndef GOFANN_H
 #define GOFANN_H
@@ -83,7 +85,8 @@ typedef enum gofann_status {
 
 enum { GOFANN_EARLY_STOP_FIXED = 0, GOFANN_EARLY_STOP_OFF = 1, GOFANN_EARLY_STOP_ADAPTIVE = 2 };
 enum { GOFANN_SCORER_PQ = 0, GOFANN_SCORER_RABITQ = 1 };
-enum { GOFANN_DTYPE_U8 = 0, GOFANN_DTYPE_F32 = 1, GOFANN_DTYPE_F16 = 2 };
+/* GOFANN_DTYPE_BF16 is a type of the cache operators (gofann_kv_*) only. */
+enum { GOFANN_DTYPE_U8 = 0, GOFANN_DTYPE_F32 = 1, GOFANN_DTYPE_F16 = 2, GOFANN_DTYPE_BF16 = 3 };
 /* PQ scoring inside the traversal: read a prebuilt LUT from global memory,
  * stage it in shared memory per route, or evaluate each table entry from the
  * query and the codebook where it is used (no per-query table at all).
@@ -647,6 +650,160 @@ GOFANN_API int gofann_build_row_records(const gofann_graph* graph, const gofann_
 
 /* Adds base to every id that is not UINT32_MAX (local -> global shard ids). */
 GOFANN_API int gofann_offset_ids(uint32_t* ids, size_t n, uint32_t base, void* stream);
+
+/* ------------------------------------------------ 4-bit key/value cache */
+/* A language model's key/value cache as a vector store that every new token
+ * searches: gofann_kv_append writes it, gofann_kv_select picks the blocks a
+ * query reads by a cheap integer score, gofann_kv_attention reads all of it
+ * or the selected blocks.  Serving operators: no gradients.
+ *
+ * A page holds GOFANN_KV_PAGE tokens of one sequence and is the block that
+ * gofann_kv_select scores.  Per token and key/value head, each group of
+ * GOFANN_KV_GROUP dimensions is held as 4-bit codes c with an f16 scale s and
+ * minimum m; a code stands for c * s + m (f32, product rounded first).  The
+ * chunk of one (page, head), gofann_kv_chunk_bytes(head_dim) bytes, holds, in
+ * this order and row-major, with G = head_dim / 64 and digits in brackets
+ * running over their sizes:
+ *   key codes     [kt 4][grp G][g1 4][g0 2][t 4][j 4][e 2][r 2] bytes: the
+ *                 low (n = 0) and high (n = 1) nibble is token 16 g1 + 4 kt +
+ *                 2 r + g0, dimension 64 grp + 16 t + 4 j + 2 n + e
+ *   key params    [g1 4][g0 2][kt 4][r 2][grp G] f16 pairs (s, m) of the
+ *                 token above
+ *   value codes   [dt head_dim/16][g 8][t 4][kt 4][e 2][r 2] bytes: nibble n
+ *                 is dimension 16 dt + 8 r + g, token 16 t + 4 kt + 2 n + e
+ *   value params  as the key params
+ * Both orders are what one lane feeds to a 16 x 8 x 16 matrix instruction:
+ * 16 consecutive bytes per lane, no shuffle between load and use. */
+#define GOFANN_KV_PAGE 64u
+#define GOFANN_KV_GROUP 64u
+#define GOFANN_KV_MAX_SELECT 1024u
+/* Keys and values are clamped to this magnitude (NaN becomes 0), so that
+ * every scale, minimum and code value is a finite f16. */
+#define GOFANN_KV_CLAMP 57344.0f
+
+typedef struct gofann_kv_cache {
+    uint8_t* pages;      /* device [n_pages][n_kv_heads][gofann_kv_chunk_bytes], 16-byte aligned */
+    int8_t* bounds;      /* device [n_pages][n_kv_heads][2][head_dim], 16-byte aligned: the largest, then
+                            the smallest key value of each dimension over the page's tokens, in units of
+                            bound_scale (rounded outwards) */
+    float* bound_scale;  /* device [n_pages][n_kv_heads] = max |key value| / 127 */
+    uint32_t n_pages;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;   /* 64 or 128 */
+    uint32_t reserved;
+} gofann_kv_cache;
+
+/* Sequences of one call and their query rows.  Row i of sequence s (rows
+ * row_offset[s] .. row_offset[s+1] - 1 of the call) is the token at position
+ * seq_len[s] - rows + i: a sequence's rows are its newest tokens.  seq_len
+ * counts the tokens in the cache with this call's rows among them. */
+typedef struct gofann_kv_batch {
+    const int32_t* page_table;   /* device [n_seqs][max_pages]: pages of a sequence in token order */
+    const uint32_t* seq_len;     /* device [n_seqs], at most max_pages * GOFANN_KV_PAGE */
+    const uint32_t* row_offset;  /* device [n_seqs + 1], ascending from 0 to n_rows */
+    int32_t* status;             /* device [1] error word or NULL: set to GOFANN_ERR_INVALID where a page,
+                                    position, length or row is out of range; that item is skipped */
+    uint32_t n_seqs;
+    uint32_t max_pages;
+    uint32_t n_rows;
+    uint32_t max_rows;           /* largest number of rows of a sequence; chooses kernels, not results */
+} gofann_kv_batch;
+
+/* Rows of q, k and v are [heads][head_dim] contiguous, consecutive rows
+ * *_stride elements apart (one fused projection can hold all three). */
+typedef struct gofann_kv_append_params {
+    const void* q;               /* device, n_heads heads per row; NULL = keys and values only */
+    const void* k;               /* device, n_kv_heads heads per row */
+    const void* v;
+    uint64_t q_stride, k_stride, v_stride;
+    const float* cos;            /* device [n_positions][rotary_dim / 2], as are sin's */
+    const float* sin;
+    const int32_t* positions;    /* device [n_rows] rotary positions, or NULL = the token's position */
+    void* q_out;                 /* device [n_rows][n_heads][head_dim] rotated queries (NULL iff q is) */
+    void* k_out;                 /* device [n_rows][n_kv_heads][head_dim] key values as the cache holds
+                                    them, or NULL */
+    void* v_out;
+    int32_t dtype;               /* GOFANN_DTYPE_BF16 or GOFANN_DTYPE_F16: q, k, v and the outputs */
+    uint32_t n_heads;            /* a multiple of n_kv_heads */
+    uint32_t n_positions;
+    uint32_t rotary_dim;         /* even, 0 (no rotation) .. head_dim; dimensions beyond it are copied */
+    int32_t interleaved;         /* pairs (2i, 2i+1) instead of (i, i + rotary_dim / 2) */
+    uint32_t reserved;
+} gofann_kv_append_params;
+
+typedef struct gofann_kv_select_params {
+    const void* q;               /* device rotated queries, rows q_stride elements apart */
+    uint64_t q_stride;
+    int32_t* ids;                /* device [n_rows][n_kv_heads][n_select] block numbers, ascending, -1 fill */
+    float* scores;               /* device, as ids: their scores (-inf fill), or NULL */
+    int32_t dtype;
+    uint32_t n_heads;
+    uint32_t n_select;           /* 1 .. GOFANN_KV_MAX_SELECT */
+    uint32_t n_first;            /* blocks always kept: the sequence's first n_first and, ending with the */
+    uint32_t n_recent;           /* row's own block, the n_recent newest; n_first + n_recent <= n_select */
+    uint32_t reserved;
+} gofann_kv_select_params;
+
+typedef struct gofann_kv_attention_params {
+    const void* q;               /* device rotated queries, rows q_stride elements apart */
+    uint64_t q_stride;
+    const int32_t* selected;     /* device [n_rows][n_kv_heads][n_select] distinct block numbers (others than
+                                    those of the sequence's pages are skipped), or NULL = every block */
+    const uint32_t* key_bits;    /* device [n_seqs][key_words]: bit i % 32 of word i / 32 shows token i
+                                    (the layout of gofann_predicate_pass_masks; tokens beyond the words are
+                                    hidden), or NULL = every token */
+    void* out;                   /* device [n_rows][n_heads][head_dim]; a row that sees no key gives 0 */
+    float* lse;                  /* device [n_rows][n_heads] natural log of the sum of exponentials (-inf for
+                                    a row that sees no key), or NULL */
+    float scale;                 /* of q.k, finite */
+    int32_t dtype;               /* q and out */
+    uint32_t n_heads;
+    uint32_t n_select;           /* width of selected */
+    uint32_t key_words;
+    int32_t causal;              /* 1 = a row sees the tokens up to its own, 0 = all of its sequence */
+    uint32_t window;             /* a row at position p sees tokens above p - window only; 0 = no window */
+    uint32_t reserved;
+} gofann_kv_attention_params;
+
+/* Bytes of one (page, head) chunk; 0 for a head_dim that is not supported. */
+GOFANN_API size_t gofann_kv_chunk_bytes(uint32_t head_dim);
+
+/* Rotates the rows of q and k by their positions (x_a cos - x_b sin, x_b cos +
+ * x_a sin, each product rounded, f32), writes the keys and values of the rows
+ * to their sequences' pages in 4 bits (group minimum m = f16(min), scale s =
+ * f16((max - min) / 15), code = clamp(rint((x - m) / s), 0, 15), or 0 where s
+ * is 0) and renews the bounds of the touched pages from all tokens that they
+ * hold.  Tokens of the touched pages other than the rows keep their codes.
+ * One launch, no scratch; q_out may be q where q's rows are contiguous. */
+GOFANN_API int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                                const gofann_kv_append_params* params, void* stream);
+
+/* The n_select blocks of each row and key/value head with the largest score,
+ * among the blocks from the sequence's first to the row's own.  The score is
+ * an upper bound of q.k over the block's keys in 8 bits: per query head q8 =
+ * rint(q / qs), qs = max |q| / 127 (both 0 where q is zero or not finite), u =
+ * sum over d of q8 * (q8 > 0 ? largest : smallest) as an integer, score = max
+ * over the query heads of the key/value head of (u * qs), times bound_scale.
+ * Integers and rounded products only: the same ids on every run.  Ties go to
+ * the lowest block.  scratch: gofann_kv_select_scratch_bytes, 256-byte
+ * aligned. */
+GOFANN_API size_t gofann_kv_select_scratch_bytes(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                                                 const gofann_kv_select_params* params);
+GOFANN_API int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                                const gofann_kv_select_params* params, void* scratch, size_t scratch_bytes,
+                                void* stream);
+
+/* out = softmax(scale * q.K^T) V over the cached tokens that each row sees:
+ * those of the selected blocks (or of all blocks), up to the row's own token
+ * (causal), inside the window and shown by key_bits.  Query head h reads
+ * key/value head h / (n_heads / n_kv_heads).  Logits, maxima, sums and the
+ * output are accumulated in f32.  scratch: gofann_kv_attention_scratch_bytes,
+ * 256-byte aligned. */
+GOFANN_API size_t gofann_kv_attention_scratch_bytes(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                                                    const gofann_kv_attention_params* params);
+GOFANN_API int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                                   const gofann_kv_attention_params* params, void* scratch, size_t scratch_bytes,
+                                   void* stream);
 
 #ifdef __cplusplus
 }
