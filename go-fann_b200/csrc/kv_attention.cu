@@ -12,7 +12,7 @@
 // Tokens are the rows (M = 16) and query heads the columns (N = 8) of both
 // products: S^T = K Q^T, then O^T = V^T P^T; the transposition of P between
 // the two layouts is one movmatrix per 8 x 8 tile.
-#include "kv_common.cuh"
+#include "kv_async.cuh"
 
 namespace gofann {
 namespace {
@@ -35,6 +35,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+// 2^x by the special function unit (2 ulp; results below 2^-126 are 0).
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // The A operand of 16 rows x 16 steps from one word of eight codes.
 __device__ __forceinline__ void code_operand(uint32_t w, uint32_t (&a)[4])
 {
@@ -52,14 +59,29 @@ __device__ __forceinline__ float high_half(uint32_t w)
 {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
 }
+// N (1, 2 or 4) words from an address that is a multiple of 4 N.
+template <int N>
+__device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[N])
+{
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
 __device__ __forceinline__ uint32_t pack_f16(float a, float b)
 {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A block's work: the query columns of one tile (rows of a sequence x query
-// heads of one key/value head) and the cache blocks that any of them sees.
+// The query columns that a block works on at a time: rows of a sequence x
+// query heads of one key/value head, and the cache blocks that any of them
+// sees.
 struct Tile {
     uint32_t seq;
     int first_row, n_rows, len;  // of the sequence
@@ -68,39 +90,98 @@ struct Tile {
     int block_lo, block_hi;      // cache blocks (dense) or slots of the list (selected)
 };
 
-template <bool kSelected>
-__device__ __forceinline__ bool find_tile(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group,
-                                          int width, uint32_t flat, Tile& tile)
+// Cache blocks that the columns [col0, col0 + cols) of a sequence see.
+__device__ __forceinline__ void dense_blocks(const gofann_kv_attention_params& p, int group, int len, int n_rows,
+                                             int col0, int cols, int& lo, int& hi)
 {
-    const int per_row = (group + width - 1) / width;
-    uint32_t at;
-    const auto tiles = [&](uint32_t s) {
-        int first, n;
-        kv_rows(b, s, first, n);
-        return static_cast<uint32_t>(kSelected ? n * per_row : (n * group + width - 1) / width);
-    };
-    if (!kv_find(b.n_seqs, flat, tiles, tile.seq, at)) return false;
-    kv_rows(b, tile.seq, tile.first_row, tile.n_rows);
-    tile.len = kv_len(b, tile.seq);
+    const int pos0 = len - n_rows + col0 / group, pos1 = len - n_rows + (col0 + cols - 1) / group;
+    const int end = p.causal ? pos1 + 1 : len;
+    hi = end > 0 && pos1 >= 0 ? (end + kKvPage - 1) / kKvPage : 0;
+    const long long low = p.window ? static_cast<long long>(pos0) - p.window + 1 : 0;
+    lo = low > 0 ? static_cast<int>(low / kKvPage) : 0;
+    if (lo > hi) lo = hi;
+}
+
+// A sequence's share of the work in units of one cache block for one tile and
+// key/value head: every tile counts `span` blocks from `lo` on (what all of
+// the sequence's rows see), at least one, so that each tile has an owner.
+struct SeqWork {
+    int tiles, lo, span;
+};
+template <bool kSelected>
+__device__ __forceinline__ SeqWork seq_work(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group,
+                                            int width, uint32_t s)
+{
+    int first, n, lo = 0, hi = static_cast<int>(p.n_select);
+    kv_rows(b, s, first, n);
+    SeqWork w{0, 0, 1};
+    if (n == 0) return w;
     if (kSelected) {
-        tile.row = static_cast<int>(at) / per_row;
-        tile.col0 = static_cast<int>(at) % per_row * width;
+        w.tiles = n * ((group + width - 1) / width);
+    } else {
+        w.tiles = (n * group + width - 1) / width;
+        dense_blocks(p, group, kv_len(b, s), n, 0, n * group, lo, hi);
+    }
+    w.lo = lo;
+    w.span = hi > lo ? hi - lo : 1;
+    return w;
+}
+
+// Blocks [b0, b1) of one tile and head, and its place among all units.
+struct Segment {
+    Tile tile;
+    uint32_t head;
+    int b0, b1;
+    uint64_t item_begin, item_end, end;  // units of the whole (tile, head), and where this part ends
+};
+
+template <bool kSelected>
+__device__ __forceinline__ void make_tile(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group,
+                                          int width, uint32_t seq, int at, Tile& tile)
+{
+    tile.seq = seq;
+    kv_rows(b, seq, tile.first_row, tile.n_rows);
+    tile.len = kv_len(b, seq);
+    if (kSelected) {
+        const int per_row = (group + width - 1) / width;
+        tile.row = at / per_row;
+        tile.col0 = at % per_row * width;
         tile.cols = group - tile.col0 < width ? group - tile.col0 : width;
         tile.block_lo = 0;
         tile.block_hi = static_cast<int>(p.n_select);
     } else {
         const int total = tile.n_rows * group;
         tile.row = 0;
-        tile.col0 = static_cast<int>(at) * width;
+        tile.col0 = at * width;
         tile.cols = total - tile.col0 < width ? total - tile.col0 : width;
-        const int pos0 = tile.len - tile.n_rows + tile.col0 / group;
-        const int pos1 = tile.len - tile.n_rows + (tile.col0 + tile.cols - 1) / group;
-        const int end = p.causal ? pos1 + 1 : tile.len;
-        tile.block_hi = end > 0 ? (end + kKvPage - 1) / kKvPage : 0;
-        const long long low = p.window ? static_cast<long long>(pos0) - p.window + 1 : 0;
-        tile.block_lo = low > 0 ? static_cast<int>(low / kKvPage) : 0;
-        if (pos1 < 0) tile.block_hi = 0;
+        dense_blocks(p, group, tile.len, tile.n_rows, tile.col0, tile.cols, tile.block_lo, tile.block_hi);
     }
+}
+
+// The segment of units [flat, limit) that starts at `flat`; false at the end.
+template <bool kSelected>
+__device__ __forceinline__ bool segment_at(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+                                           int group, int width, uint64_t flat, uint64_t limit, Segment& sg)
+{
+    if (flat >= limit) return false;
+    uint32_t seq;
+    uint64_t at;
+    const auto units = [&](uint32_t s) {
+        const SeqWork w = seq_work<kSelected>(b, p, group, width, s);
+        return static_cast<uint64_t>(w.tiles) * n_kv * w.span;
+    };
+    if (!kv_find<uint64_t>(b.n_seqs, flat, units, seq, at)) return false;
+    const SeqWork w = seq_work<kSelected>(b, p, group, width, seq);
+    const uint64_t item = at / w.span;
+    const int off = static_cast<int>(at % w.span);
+    sg.head = static_cast<uint32_t>(item % n_kv);
+    make_tile<kSelected>(b, p, group, width, seq, static_cast<int>(item / n_kv), sg.tile);
+    sg.item_begin = flat - off;
+    sg.item_end = sg.item_begin + w.span;
+    sg.end = sg.item_end < limit ? sg.item_end : limit;
+    const int b0 = w.lo + off, b1 = w.lo + static_cast<int>(sg.end - sg.item_begin);
+    sg.b0 = b0 > sg.tile.block_lo ? b0 : sg.tile.block_lo;
+    sg.b1 = b1 < sg.tile.block_hi ? b1 : sg.tile.block_hi;
     return true;
 }
 
@@ -157,23 +238,14 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
     float s[4][NT][4];
 
     // ---- scores of 64 tokens x 8 NT columns
-    uint32_t kp[8][G];
-    {
-        const uint4* src = reinterpret_cast<const uint4*>(chunk + Chunk::kKeyParams + g * 32 * G);
-#pragma unroll
-        for (int i = 0; i < 2 * G; ++i) {
-            const uint4 w = src[i];
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) kp[(4 * i + k) / G][(4 * i + k) % G] = v[k];
-        }
-    }
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[kt][n][i] = 0.0f;
+        uint32_t kp[2 * G];  // tokens first + 4 kt, + 2
+        load_words<2 * G>(chunk + Chunk::kKeyParams + (g * 4 + kt) * 8 * G, kp);
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
             const uint4 w4 = reinterpret_cast<const uint4*>(chunk)[(kt * G + grp) * 32 + lane];
@@ -192,7 +264,7 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float ks = low_half(kp[2 * kt + r][grp]), km = high_half(kp[2 * kt + r][grp]);
+                const float ks = low_half(kp[r * G + grp]), km = high_half(kp[r * G + grp]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -216,23 +288,16 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
             }
     }
 
-    // ---- value params; a hidden token's may be anything, so they count as 0
-    uint32_t vp[8][G];
+    // ---- the largest value scale; a hidden token's params may be anything,
+    // so they count as 0 here and below
     uint32_t top = 0;
-    {
-        const uint4* src = reinterpret_cast<const uint4*>(chunk + Chunk::kValueParams + g * 32 * G);
 #pragma unroll
-        for (int i = 0; i < 2 * G; ++i) {
-            const uint4 w = src[i];
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < 8; ++i) {
+        uint32_t w[G];
+        load_words<G>(chunk + Chunk::kValueParams + (g * 8 + i) * 4 * G, w);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int at = (4 * i + k) / G;
-                const uint32_t x = !masked || ((shown >> (first + 2 * at)) & 1) ? v[k] : 0u;
-                vp[at][(4 * i + k) % G] = x;
-                top = max(top, x & 0x7c00u);
-            }
-        }
+        for (int grp = 0; grp < G; ++grp)
+            if (!masked || ((shown >> (first + 2 * i)) & 1)) top = max(top, w[grp] & 0x7c00u);
     }
     // The weights p * scale become f16 operands.  They are taken relative to
     // the largest scale exponent so far (2^26-e below), so that f16 holds
@@ -251,7 +316,7 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
             const float use = mx == kNegInf ? 0.0f : mx;
-            const float f = exp2f(st.m[n][c] - use);
+            const float f = exp2_fast(st.m[n][c] - use);
             st.m[n][c] = mx;
             st.l[n][c] *= f;
 #pragma unroll
@@ -261,7 +326,7 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float x = exp2f(s[kt][n][2 * r + c] - use);
+                    const float x = exp2_fast(s[kt][n][2 * r + c] - use);
                     s[kt][n][2 * r + c] = x;
                     st.l[n][c] += x;
                 }
@@ -282,7 +347,8 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const uint32_t w = vp[2 * kt + r][grp];
+                uint32_t w = reinterpret_cast<const uint32_t*>(chunk + Chunk::kValueParams)[(g * 8 + 2 * kt + r) * G + grp];
+                if (masked && !((shown >> (first + 4 * kt + 2 * r)) & 1)) w = 0;
                 const float scale = low_half(w), vs = scale * (r ? up * 0.0625f : up);
                 const float vm = fmaf(8.0f, scale, high_half(w));
 #pragma unroll
@@ -410,143 +476,339 @@ __device__ __forceinline__ void load_query(const gofann_kv_batch& batch, const g
     }
 }
 
+// Shared memory of a block: a ring of kStages chunks per warp, the warps'
+// partial results of a segment, the ring's barriers.
+template <int D, int NT>
+struct AttendShared {
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kStages = D == 64 ? 4 : 2;
+    static constexpr size_t kRing = static_cast<size_t>(kAttendWarps) * kStages * KvChunk<D>::kBytes;
+    static constexpr size_t kMerge = sizeof(float) * kAttendWarps * kCols * (D + 4 + 2);
+    static constexpr size_t kBytes = kRing + kMerge + sizeof(uint64_t) * kAttendWarps * kStages;
+};
+
+// Units of one block: a share of the total, at least one per warp.
+__device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks)
+{
+    const uint64_t c = (total + blocks - 1) / blocks;
+    return c > kAttendWarps ? c : kAttendWarps;
+}
+
+// A partial result in scratch: [cols] max, [cols] sum, [cols][D] values; two
+// per block (its first segment, and its last if that is another).
+template <int D, int NT>
+constexpr size_t kPartFloats = 8 * NT * (D + 2);
+
+template <int D>
+__device__ __forceinline__ void store_row(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head, int group,
+                                          bool selected, int c, int d, float m, float l, const float (&o)[4])
+{
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int col = tile.col0 + c;
+    const uint64_t row = tile.first_row + (selected ? tile.row : col / group);
+    const uint64_t at = row * p.n_heads + head * group + (selected ? col : col % group);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d) =
+        l > 0.0f ? make_uint2(kv_pack2(o[0] * inv, o[1] * inv, p.dtype), kv_pack2(o[2] * inv, o[3] * inv, p.dtype))
+                 : make_uint2(0u, 0u);
+    if (d == 0 && p.lse) p.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
+}
+
+// The chunks that a warp reads, in order: its share (every kAttendWarps-th
+// block) of each segment of the thread block.  Page numbers are looked up 32
+// blocks at a time, one per lane.
+template <int D, bool kSelected>
+struct Reader {
+    Segment sg;
+    int next;       // this warp's next block (or slot) of the segment
+    int batch_at;   // `next` of lane 0's entry
+    int block, page;  // this lane's entry: cache block and page, -1 = nothing to read
+    bool more;
+
+    __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofann_kv_batch& b,
+                                            const gofann_kv_attention_params& p)
+    {
+        const int lane = threadIdx.x & 31;
+        const int i = next + lane * kAttendWarps;
+        batch_at = next;
+        block = page = -1;
+        if (i < sg.b1) {
+            const int seq_blocks = (sg.tile.len + kKvPage - 1) / kKvPage;
+            block = i;
+            if (kSelected)
+                block = __ldg(p.selected +
+                              (static_cast<size_t>(sg.tile.first_row + sg.tile.row) * cache.n_kv_heads + sg.head) * p.n_select + i);
+            if (block >= 0 && block < seq_blocks) {
+                page = __ldg(b.page_table + static_cast<size_t>(sg.tile.seq) * b.max_pages + block);
+                if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
+                    page = -1;
+                    kv_invalid(b);
+                }
+            }
+        }
+    }
+};
+
 template <int D, int NT, bool kSelected>
-__global__ void __launch_bounds__(kAttendThreads) kv_attend_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
-                                                                   gofann_kv_attention_params p, bool wide)
+__global__ void __launch_bounds__(kAttendThreads, 1) kv_attend_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
+                                                                      gofann_kv_attention_params p, bool wide,
+                                                                      float* __restrict__ parts)
 {
     using Chunk = KvChunk<D>;
-    constexpr int G = Chunk::kGroups, kCols = 8 * NT;
-    extern __shared__ __align__(16) float smem[];
-    float* merge_o = smem;                                      // [warps][cols][D + 4]
-    float* merge_m = merge_o + kAttendWarps * kCols * (D + 4);  // [warps][cols]
+    using Shared = AttendShared<D, NT>;
+    constexpr int G = Chunk::kGroups, kCols = 8 * NT, kStages = Shared::kStages;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* merge_o = reinterpret_cast<float*>(smem + Shared::kRing);  // [warps][cols][D + 4]
+    float* merge_m = merge_o + kAttendWarps * kCols * (D + 4);        // [warps][cols]
     float* merge_l = merge_m + kAttendWarps * kCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t head = blockIdx.y;
+    const unsigned char* ring = smem + static_cast<size_t>(warp) * kStages * Chunk::kBytes;
+    const uint32_t bars = shared_addr(smem + Shared::kRing + Shared::kMerge) + warp * kStages * 8;
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
-    Tile tile;
-    if (!find_tile<kSelected>(batch, p, group, kCols, blockIdx.x, tile)) return;
 
-    Query<D, NT> q;
-    load_query<D, NT>(batch, p, tile, head, group, kSelected, wide, q);
-    int limit = 0x7fffffff, low = -1;  // keys in (low, limit] are seen by every column
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            limit = min(limit, q.limit[n][e]);
-            low = max(low, q.low[n][e]);
-        }
-    limit = __reduce_min_sync(kFull, limit);
-    low = __reduce_max_sync(kFull, low);
-    limit = min(limit, tile.len - 1);
+    if (lane < kStages) barrier_init(bars + 8 * lane, 1);
+    barrier_fence();
+    launch_next();
+    __syncwarp();
+    const auto units = [&](uint32_t s) {
+        const SeqWork w = seq_work<kSelected>(batch, p, group, kCols, s);
+        return static_cast<uint64_t>(w.tiles) * cache.n_kv_heads * w.span;
+    };
+    const uint64_t total = kv_total<uint64_t>(batch.n_seqs, units);
+    const uint64_t share = units_per_block(total, gridDim.x);
+    const uint64_t u0 = share * blockIdx.x, u1 = u0 + share < total ? u0 + share : total;
+    if (u0 >= u1) return;
 
-    State<D, NT> st;
-    clear(st);
-    const int32_t* table = batch.page_table + static_cast<size_t>(tile.seq) * batch.max_pages;
-    const int32_t* list = kSelected ? p.selected + (static_cast<size_t>(tile.first_row + tile.row) * cache.n_kv_heads + head) *
-                                                       p.n_select
-                                    : nullptr;
-    const int seq_blocks = (tile.len + kKvPage - 1) / kKvPage;
-    for (int i = tile.block_lo + warp; i < tile.block_hi; i += kAttendWarps) {
-        const int block = kSelected ? __ldg(list + i) : i;
-        if (block < 0 || block >= seq_blocks) continue;
-        const int page = __ldg(table + block);
-        if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
-            if (lane == 0) kv_invalid(batch);
-            continue;
+    // ---- the loads run ahead of the work by up to kStages chunks
+    Reader<D, kSelected> rd;
+    rd.more = segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, u0, u1, rd.sg);
+    rd.next = rd.sg.b0 + warp;
+    rd.look_up(cache, batch, p);
+    uint32_t issued = 0, taken = 0;  // chunks of this warp
+    const auto advance = [&]() {     // issues the next chunk's load, skipping entries with nothing to read
+        while (rd.more) {
+            if (rd.next >= rd.sg.b1) {
+                rd.more = segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, rd.sg.end, u1, rd.sg);
+                if (!rd.more) return;
+                rd.next = rd.sg.b0 + warp;
+                rd.look_up(cache, batch, p);
+                continue;
+            }
+            int l = (rd.next - rd.batch_at) / kAttendWarps;
+            if (l >= 32) {
+                rd.look_up(cache, batch, p);
+                l = 0;
+            }
+            const int page = __shfl_sync(kFull, rd.page, l);
+            rd.next += kAttendWarps;
+            if (page < 0) continue;
+            if (lane == 0) {
+                const uint32_t st = issued % kStages;
+                barrier_expect(bars + 8 * st, Chunk::kBytes);
+                bulk_load(shared_addr(ring + st * Chunk::kBytes),
+                          cache.pages + (static_cast<size_t>(page) * cache.n_kv_heads + rd.sg.head) * Chunk::kBytes,
+                          Chunk::kBytes, bars + 8 * st);
+            }
+            ++issued;
+            return;
         }
-        const int key0 = block * kKvPage;
-        uint64_t shown = ~0ull;
-        if (p.key_bits) {
-            const uint32_t* bits = p.key_bits + static_cast<size_t>(tile.seq) * p.key_words;
-            const uint32_t w = 2u * block;
-            const uint32_t b0 = w < p.key_words ? __ldg(bits + w) : 0u, b1 = w + 1 < p.key_words ? __ldg(bits + w + 1) : 0u;
-            shown = b0 | (static_cast<uint64_t>(b1) << 32);
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) advance();
+
+    // ---- segment by segment
+    bool alive = true;  // false once a wait has run out
+    uint64_t flat = u0;
+    Reader<D, kSelected> use;
+    while (segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, flat, u1, use.sg)) {
+        const Segment& sg = use.sg;
+        const Tile& tile = sg.tile;
+        Query<D, NT> q;
+        load_query<D, NT>(batch, p, tile, sg.head, group, kSelected, wide, q);
+        int limit = 0x7fffffff, low = -1;  // keys in (low, limit] are seen by every column
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                limit = min(limit, q.limit[n][e]);
+                low = max(low, q.low[n][e]);
+            }
+        limit = __reduce_min_sync(kFull, limit);
+        low = __reduce_max_sync(kFull, low);
+        State<D, NT> st;
+        clear(st);
+        use.next = sg.b0 + warp;
+        while (use.next < sg.b1) {
+            use.look_up(cache, batch, p);
+            const uint32_t* bits = p.key_bits ? p.key_bits + static_cast<size_t>(tile.seq) * p.key_words : nullptr;
+#pragma unroll 1
+            for (int l = 0; l < 32 && use.next < sg.b1; ++l, use.next += kAttendWarps) {
+                if (__shfl_sync(kFull, use.page, l) < 0) continue;
+                const int block = __shfl_sync(kFull, use.block, l), key0 = block * kKvPage;
+                uint64_t shown = ~0ull;
+                if (bits) {
+                    const uint32_t w = 2u * block;
+                    shown = (w < p.key_words ? __ldg(bits + w) : 0u) |
+                            (static_cast<uint64_t>(w + 1 < p.key_words ? __ldg(bits + w + 1) : 0u) << 32);
+                }
+                if (tile.len - key0 < kKvPage) shown &= (1ull << (tile.len - key0)) - 1;
+                const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
+                const uint32_t stage = taken % kStages;
+                alive = alive && barrier_wait(bars + 8 * stage, (taken / kStages) & 1);
+                if (!alive) continue;
+                attend_page<D, NT>(ring + stage * Chunk::kBytes, q, st, key0, masked, shown);
+                ++taken;
+                __syncwarp();
+                advance();
+            }
         }
-        if (tile.len - key0 < kKvPage) shown &= (1ull << (tile.len - key0)) - 1;
-        const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
-        const unsigned char* chunk =
-            cache.pages + (static_cast<size_t>(page) * cache.n_kv_heads + head) * Chunk::kBytes;
-        attend_page<D, NT>(chunk, q, st, key0, masked, shown);
+
+        // ---- this warp's partial result, in units of its own maximum
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = n * 8 + 2 * t + c;
+                float l = st.l[n][c];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFull, l, off);
+                if (g == 0) {
+                    merge_m[warp * kCols + col] = st.m[n][c];
+                    merge_l[warp * kCols + col] = l;
+                }
+                const float unit = exp2f(static_cast<float>(st.e - 2));  // 2^24 of the codes, 2^(e - 26) of the weights
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp) {
+                    float z = st.z[n][c][grp];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) z += __shfl_xor_sync(kFull, z, off);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            merge_o[(warp * kCols + col) * (D + 4) + (grp * 4 + i) * 16 + 8 * r + g] =
+                                fmaf(st.o[grp * 4 + i][n][2 * r + c], unit, z);
+                }
+            }
+        __syncthreads();
+
+        // ---- join the warps: the output where the block has the whole item,
+        // else a partial result for the joining kernel
+        const bool whole = flat == sg.item_begin && sg.end == sg.item_end;
+        float* part = parts + (2ull * blockIdx.x + (flat == u0 ? 0 : 1)) * kPartFloats<D, NT>;
+        for (int i = threadIdx.x; i < tile.cols * (D / 4); i += kAttendThreads) {
+            const int c = i / (D / 4), d = i % (D / 4) * 4;
+            float m = kNegInf;
+#pragma unroll
+            for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, merge_m[w * kCols + c]);
+            float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float base = m == kNegInf ? 0.0f : m;
+#pragma unroll
+            for (int w = 0; w < kAttendWarps; ++w) {
+                const float f = exp2_fast(merge_m[w * kCols + c] - base);
+                const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * kCols + c) * (D + 4) + d]);
+                l = fmaf(merge_l[w * kCols + c], f, l);
+                o[0] = fmaf(v.x, f, o[0]);
+                o[1] = fmaf(v.y, f, o[1]);
+                o[2] = fmaf(v.z, f, o[2]);
+                o[3] = fmaf(v.w, f, o[3]);
+            }
+            if (whole) {
+                store_row<D>(p, tile, sg.head, group, kSelected, c, d, m, l, o);
+            } else {
+                if (d == 0) {
+                    part[c] = m;
+                    part[kCols + c] = l;
+                }
+                *reinterpret_cast<float4*>(part + 2 * kCols + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        __syncthreads();
+        flat = sg.end;
     }
+    // loads in flight may not outlive the block's shared memory
+    for (; taken < issued; ++taken) alive = barrier_wait(bars + 8 * (taken % kStages), (taken / kStages) & 1) && alive;
+    if (!alive && lane == 0) kv_timeout(batch);
+}
 
-    // ---- this warp's partial result, in units of its own maximum
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int col = n * 8 + 2 * t + c;
-            float l = st.l[n][c];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFull, l, off);
-            if (g == 0) {
-                merge_m[warp * kCols + col] = st.m[n][c];
-                merge_l[warp * kCols + col] = l;
-            }
-            const float unit = exp2f(static_cast<float>(st.e - 2));  // 2^24 of the codes, 2^(e - 26) of the weights
-#pragma unroll
-            for (int grp = 0; grp < G; ++grp) {
-                float z = st.z[n][c][grp];
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) z += __shfl_xor_sync(kFull, z, off);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        merge_o[(warp * kCols + col) * (D + 4) + (grp * 4 + i) * 16 + 8 * r + g] =
-                            fmaf(st.o[grp * 4 + i][n][2 * r + c], unit, z);
-            }
-        }
-    __syncthreads();
-
-    // ---- join the warps
-    for (int i = threadIdx.x; i < tile.cols * (D / 4); i += kAttendThreads) {
+// Items that several blocks share: their partial results in block order, so
+// that the sum does not depend on which block was done first.
+template <int D, int NT, bool kSelected>
+__global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
+                                                      gofann_kv_attention_params p, uint32_t blocks,
+                                                      const float* __restrict__ parts)
+{
+    constexpr int kCols = 8 * NT;
+    const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
+    const auto units = [&](uint32_t s) {
+        const SeqWork w = seq_work<kSelected>(batch, p, group, kCols, s);
+        return static_cast<uint64_t>(w.tiles) * cache.n_kv_heads * w.span;
+    };
+    const uint64_t share = units_per_block(kv_total<uint64_t>(batch.n_seqs, units), blocks);
+    // the blocks' ends inside items: block i joins the item that end i falls into, if it is the item's first
+    const uint64_t cut = share * (blockIdx.x + 1);
+    Segment sg;
+    if (!segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, cut, ~0ull, sg)) return;
+    if (sg.item_begin >= cut || sg.item_begin < share * blockIdx.x) return;
+    wait_previous();
+    const uint64_t first = blockIdx.x, last = (sg.item_end - 1) / share;
+    for (int i = threadIdx.x; i < sg.tile.cols * (D / 4); i += 128) {
         const int c = i / (D / 4), d = i % (D / 4) * 4;
-        float m = kNegInf;
-#pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, merge_m[w * kCols + c]);
-        float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float use = m == kNegInf ? 0.0f : m;
-#pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) {
-            const float f = exp2f(merge_m[w * kCols + c] - use);
-            const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * kCols + c) * (D + 4) + d]);
-            l = fmaf(merge_l[w * kCols + c], f, l);
-            o[0] = fmaf(v.x, f, o[0]);
-            o[1] = fmaf(v.y, f, o[1]);
-            o[2] = fmaf(v.z, f, o[2]);
-            o[3] = fmaf(v.w, f, o[3]);
+        float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint64_t b = first; b <= last; ++b) {
+            const bool start = share * b >= sg.item_begin;  // the item is the block's first segment
+            const float* part = parts + (2 * b + (start ? 0 : 1)) * kPartFloats<D, NT>;
+            const float pm = __ldcg(part + c), pl = __ldcg(part + kCols + c);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * kCols + c * D + d));
+            const float top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
+            const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
+            l = l * f + pl * h;
+            o[0] = o[0] * f + v.x * h;
+            o[1] = o[1] * f + v.y * h;
+            o[2] = o[2] * f + v.z * h;
+            o[3] = o[3] * f + v.w * h;
+            m = top;
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        const int col = tile.col0 + c;
-        const uint64_t row = tile.first_row + (kSelected ? tile.row : col / group);
-        const uint64_t at = row * p.n_heads + head * group + (kSelected ? col : col % group);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d) =
-            l > 0.0f ? make_uint2(kv_pack2(o[0] * inv, o[1] * inv, p.dtype), kv_pack2(o[2] * inv, o[3] * inv, p.dtype))
-                     : make_uint2(0u, 0u);
-        if (d == 0 && p.lse) p.lse[at] = l > 0.0f ? (use + log2f(l)) * kLn2 : kNegInf;
+        store_row<D>(p, sg.tile, sg.head, group, kSelected, c, d, m, l, o);
     }
+}
+
+// Thread blocks of the attention kernel: one per SM (the ring takes most of
+// its shared memory), no more than there can be units.
+uint32_t attend_blocks(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
+{
+    const uint64_t span = p.selected ? p.n_select : batch.max_pages;
+    const uint64_t units = static_cast<uint64_t>(batch.n_rows) * p.n_heads * (span ? span : 1);
+    const uint64_t most = (units + kAttendWarps - 1) / kAttendWarps;
+    const int sms = sm_count();
+    const uint64_t want = sms > 0 ? sms : 1;
+    return static_cast<uint32_t>(most < want ? most : want);
 }
 
 template <int D, int NT, bool kSelected>
 int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                  cudaStream_t s)
+                  float* parts, cudaStream_t s)
 {
-    const uint64_t group = p.n_heads / cache.n_kv_heads, width = 8 * NT;
-    // a sequence of n rows has at most n group / width + 1 tiles, and at most one per column
-    const uint64_t cols = static_cast<uint64_t>(batch.n_rows) * group;
-    uint64_t tiles = kSelected ? batch.n_rows * ((group + width - 1) / width) : cols / width + batch.n_seqs;
-    if (tiles > cols) tiles = cols;
-    if (tiles > 0x7fffffffull)
-        return fail(GOFANN_ERR_UNSUPPORTED, "kv_attention: %llu tiles (at most 2^31 - 1)", static_cast<unsigned long long>(tiles));
-    const size_t smem = sizeof(float) * kAttendWarps * width * (D + 4 + 2);
+    const size_t smem = AttendShared<D, NT>::kBytes;
     auto* kernel = kv_attend_kernel<D, NT, kSelected>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return cuda_status(e, "kv_attention: shared memory attribute");
     const uintptr_t q = reinterpret_cast<uintptr_t>(p.q);
     const bool wide = (q & 7) == 0 && (p.q_stride & 3) == 0;
-    kernel<<<dim3(static_cast<uint32_t>(tiles), cache.n_kv_heads), kAttendThreads, smem, s>>>(cache, batch, p, wide);
+    const uint32_t blocks = attend_blocks(cache, batch, p);
+    kernel<<<blocks, kAttendThreads, smem, s>>>(cache, batch, p, wide, parts);
     GOFANN_CHECK_LAUNCH("kv_attend_kernel");
+    if (blocks == 1) return GOFANN_OK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks - 1);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kv_join_kernel<D, NT, kSelected>, cache, batch, p, blocks, static_cast<const float*>(parts));
+    if (e != cudaSuccess) return cuda_status(e, "kv_join_kernel");
     return GOFANN_OK;
 }
 
@@ -561,7 +823,9 @@ size_t gofann_kv_attention_scratch_bytes(const gofann_kv_cache* cache, const gof
                                          const gofann_kv_attention_params* params)
 {
     if (!cache || !batch || !params) return 0;
-    return 256;
+    const size_t part = sizeof(float) * (cache->head_dim <= 64 ? kPartFloats<64, 2> : kPartFloats<128, 2>);
+    const int sms = sm_count();
+    return 2 * part * static_cast<size_t>(sms > 0 ? sms : 1);
 }
 
 int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
@@ -590,8 +854,10 @@ int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* bat
     const uint32_t group = p.n_heads / cache->n_kv_heads;
     const uint64_t cols = p.selected ? group : static_cast<uint64_t>(batch->max_rows) * group;
     cudaStream_t s = as_stream(stream);
-#define GOFANN_KV_LAUNCH(D, NT) \
-    return p.selected ? launch_attend<D, NT, true>(*cache, *batch, p, s) : launch_attend<D, NT, false>(*cache, *batch, p, s)
+    float* parts = static_cast<float*>(scratch);
+#define GOFANN_KV_LAUNCH(D, NT)                                                   \
+    return p.selected ? launch_attend<D, NT, true>(*cache, *batch, p, parts, s) \
+                      : launch_attend<D, NT, false>(*cache, *batch, p, parts, s)
     if (d == 64) {
         if (cols <= 8) GOFANN_KV_LAUNCH(64, 1);
         GOFANN_KV_LAUNCH(64, 2);

@@ -61,17 +61,17 @@ __device__ __forceinline__ void kv_invalid(const gofann_kv_batch& b)
 // the item's place in it.  Every lane of a warp calls it with the same
 // `flat`; sequences are taken 32 at a time (one lane each, a warp scan).
 // False where the items end before `flat`.
-template <class F>
-__device__ __forceinline__ bool kv_find(uint32_t n_seqs, uint32_t flat, F count, uint32_t& seq, uint32_t& at)
+template <class N, class F>
+__device__ __forceinline__ bool kv_find(uint32_t n_seqs, N flat, F count, uint32_t& seq, N& at)
 {
     const int lane = threadIdx.x & 31;
     for (uint32_t s0 = 0; s0 < n_seqs; s0 += 32) {
         const uint32_t s = s0 + lane;
-        const uint32_t c = s < n_seqs ? count(s) : 0u;
-        uint32_t sum = c;
+        const N c = s < n_seqs ? count(s) : N(0);
+        N sum = c;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const uint32_t v = __shfl_up_sync(kFull, sum, off);
+            const N v = __shfl_up_sync(kFull, sum, off);
             if (lane >= off) sum += v;
         }
         const unsigned past = __ballot_sync(kFull, flat < sum);
@@ -84,6 +84,16 @@ __device__ __forceinline__ bool kv_find(uint32_t n_seqs, uint32_t flat, F count,
         flat -= __shfl_sync(kFull, sum, 31);
     }
     return false;
+}
+// Sum of count(s) over the sequences, in every lane of the warp.
+template <class N, class F>
+__device__ __forceinline__ N kv_total(uint32_t n_seqs, F count)
+{
+    N sum = 0;
+    for (uint32_t s = threadIdx.x & 31; s < n_seqs; s += 32) sum += count(s);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+    return sum;
 }
 
 // ------------------------------------------------------------------- values
