@@ -27,21 +27,27 @@ __device__ __forceinline__ void barrier_arrive(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Waits for the phase of `parity`; false when the limit (some seconds) ran out.
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// Waits for the phase of `parity`; false when the limit of some 2 s ran out.
+constexpr long long kWaitCycles = 4ll << 30;
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity)
 {
-    for (int i = 0; i < (1 << 24); ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
+    if (barrier_try(bar, parity)) return true;
+    const long long start = clock64();
+    while (!barrier_try(bar, parity))
+        if (clock64() - start > kWaitCycles) return false;
+    return true;
 }
 // Contiguous global -> shared copy; both addresses and the size multiples of 16.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)

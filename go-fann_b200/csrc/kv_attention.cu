@@ -5,9 +5,10 @@
 //   sum_j p_j v_j = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (m_j + 8 s_j)
 // so the matrix instructions read the codes themselves.  A code word masked
 // to nibbles is already a pair of f16 numbers: 0x000c is the subnormal
-// c * 2^-24 and 0x00c0 is c * 2^-20, both exact, so two ANDs and a shift turn
-// 32 bits into half of an A operand.  The 2^-24 goes into the f32 scale, the
-// extra 2^4 of the odd nibbles into the other operand.
+// c * 2^-24 and 0x00c0 is c * 2^-20, both exact, so four ANDs and a shift turn
+// a word of eight codes into the lane's A operand of a 16 x 8 x 16 product.
+// The 2^-24 goes into an f32 scale, the extra 2^4 of the odd nibbles into the
+// other operand.
 //
 // Tokens are the rows (M = 16) and query heads the columns (N = 8) of both
 // products: S^T = K Q^T, then O^T = V^T P^T; the transposition of P between
@@ -17,17 +18,16 @@
 namespace gofann {
 namespace {
 
-constexpr int kAttendThreads = 256;
-constexpr int kAttendWarps = kAttendThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                        const float* c)
 {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
@@ -51,13 +51,9 @@ __device__ __forceinline__ void code_operand(uint32_t w, uint32_t (&a)[4])
     a[1] = w & 0x000f000fu;
     a[3] = w & 0x00f000f0u;
 }
-__device__ __forceinline__ float low_half(uint32_t w)
+__device__ __forceinline__ float2 both_halves(uint32_t w)
 {
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xffffu)));
-}
-__device__ __forceinline__ float high_half(uint32_t w)
-{
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 // N (1, 2 or 4) words from an address that is a multiple of 4 N.
 template <int N>
@@ -79,15 +75,13 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The query columns that a block works on at a time: rows of a sequence x
-// query heads of one key/value head, and the cache blocks that any of them
-// sees.
+// The query columns that a warp works on at a time: rows of a sequence x
+// query heads of one key/value head.
 struct Tile {
     uint32_t seq;
     int first_row, n_rows, len;  // of the sequence
     int col0, cols;              // columns of the sequence (dense) or of the row (selected)
     int row;                     // selected: the row inside the sequence
-    int block_lo, block_hi;      // cache blocks (dense) or slots of the list (selected)
 };
 
 // Cache blocks that the columns [col0, col0 + cols) of a sequence see.
@@ -127,12 +121,18 @@ __device__ __forceinline__ SeqWork seq_work(const gofann_kv_batch& b, const gofa
     return w;
 }
 
-// Blocks [b0, b1) of one tile and head, and its place among all units.
-struct Segment {
+// A (tile, head) and its place among all units.
+struct Item {
     Tile tile;
     uint32_t head;
-    int b0, b1;
-    uint64_t item_begin, item_end, end;  // units of the whole (tile, head), and where this part ends
+    uint64_t begin, end;
+};
+
+// The sequence that the units around a point belong to.
+struct SeqCursor {
+    uint32_t seq;
+    uint64_t begin, end;
+    int lo, span;
 };
 
 template <bool kSelected>
@@ -147,52 +147,79 @@ __device__ __forceinline__ void make_tile(const gofann_kv_batch& b, const gofann
         tile.row = at / per_row;
         tile.col0 = at % per_row * width;
         tile.cols = group - tile.col0 < width ? group - tile.col0 : width;
-        tile.block_lo = 0;
-        tile.block_hi = static_cast<int>(p.n_select);
     } else {
         const int total = tile.n_rows * group;
         tile.row = 0;
         tile.col0 = at * width;
         tile.cols = total - tile.col0 < width ? total - tile.col0 : width;
-        dense_blocks(p, group, tile.len, tile.n_rows, tile.col0, tile.cols, tile.block_lo, tile.block_hi);
     }
 }
 
-// The segment of units [flat, limit) that starts at `flat`; false at the end.
 template <bool kSelected>
-__device__ __forceinline__ bool segment_at(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
-                                           int group, int width, uint64_t flat, uint64_t limit, Segment& sg)
+__device__ __forceinline__ uint64_t total_units(const gofann_kv_batch& b, const gofann_kv_attention_params& p,
+                                                uint32_t n_kv, int group, int width)
 {
-    if (flat >= limit) return false;
-    uint32_t seq;
+    return kv_total<uint64_t>(b.n_seqs, [&](uint32_t s) {
+        const SeqWork w = seq_work<kSelected>(b, p, group, width, s);
+        return static_cast<uint64_t>(w.tiles) * n_kv * w.span;
+    });
+}
+// The sequence of unit `flat`; false past the end.
+template <bool kSelected>
+__device__ __forceinline__ bool seek(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+                                     int group, int width, uint64_t flat, SeqCursor& c)
+{
     uint64_t at;
     const auto units = [&](uint32_t s) {
         const SeqWork w = seq_work<kSelected>(b, p, group, width, s);
         return static_cast<uint64_t>(w.tiles) * n_kv * w.span;
     };
-    if (!kv_find<uint64_t>(b.n_seqs, flat, units, seq, at)) return false;
-    const SeqWork w = seq_work<kSelected>(b, p, group, width, seq);
-    const uint64_t item = at / w.span;
-    const int off = static_cast<int>(at % w.span);
-    sg.head = static_cast<uint32_t>(item % n_kv);
-    make_tile<kSelected>(b, p, group, width, seq, static_cast<int>(item / n_kv), sg.tile);
-    sg.item_begin = flat - off;
-    sg.item_end = sg.item_begin + w.span;
-    sg.end = sg.item_end < limit ? sg.item_end : limit;
-    const int b0 = w.lo + off, b1 = w.lo + static_cast<int>(sg.end - sg.item_begin);
-    sg.b0 = b0 > sg.tile.block_lo ? b0 : sg.tile.block_lo;
-    sg.b1 = b1 < sg.tile.block_hi ? b1 : sg.tile.block_hi;
+    if (!kv_find<uint64_t>(b.n_seqs, flat, units, c.seq, at)) return false;
+    const SeqWork w = seq_work<kSelected>(b, p, group, width, c.seq);
+    c.begin = flat - at;
+    c.end = c.begin + static_cast<uint64_t>(w.tiles) * n_kv * w.span;
+    c.lo = w.lo;
+    c.span = w.span;
     return true;
 }
+// The next sequence that has units (the caller knows that there is one).
+template <bool kSelected>
+__device__ __forceinline__ void next_sequence(const gofann_kv_batch& b, const gofann_kv_attention_params& p,
+                                              uint32_t n_kv, int group, int width, SeqCursor& c)
+{
+    while (c.seq + 1 < b.n_seqs) {
+        const SeqWork w = seq_work<kSelected>(b, p, group, width, ++c.seq);
+        if (w.tiles == 0) continue;
+        c.begin = c.end;
+        c.end = c.begin + static_cast<uint64_t>(w.tiles) * n_kv * w.span;
+        c.lo = w.lo;
+        c.span = w.span;
+        return;
+    }
+}
+template <bool kSelected>
+__device__ __forceinline__ void make_item(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+                                          int group, int width, uint64_t flat, const SeqCursor& c, Item& item)
+{
+    const uint64_t i = (flat - c.begin) / c.span;
+    item.begin = c.begin + i * c.span;
+    item.end = item.begin + c.span;
+    item.head = static_cast<uint32_t>(i % n_kv);
+    make_tile<kSelected>(b, p, group, width, c.seq, static_cast<int>(i / n_kv), item.tile);
+}
 
-// Running softmax state of one warp: columns 2t, 2t + 1 of each 8-column
-// tile, dimensions 16 dt + g, + 8.
+// Running softmax state of one warp for columns 2t, 2t + 1 of each 8-column
+// tile and dimensions 16 dt + g, + 8.  All sums are in units of the weights
+// 2^(logit - base), base = max - (26 - e) in log2 units: e is the largest
+// exponent of a value scale so far, so the products weight * scale stay below
+// 2^12 and f16 holds them down to 2^-24 whatever the values' magnitude.
 template <int D, int NT>
 struct State {
-    float m[NT][2], l[NT][2];            // max (log2 units) and this lane's part of the sum
-    float z[NT][2][KvChunk<D>::kGroups]; // this lane's part of sum p * (minimum + 8 scale)
-    float o[D / 16][NT][4];              // sum (p * scale * 2^(26 - e)) * (code - 8) * 2^-24
-    int e;                               // largest exponent of a value scale so far
+    float m[NT][2];                      // largest logit, in the query column's own unit
+    float l[NT][2];                      // this lane's part of the sum of weights
+    float z[NT][2][KvChunk<D>::kGroups]; // this lane's part of sum w * (minimum + 8 scale)
+    float o[D / 16][NT][4];              // sum (w * scale) * (code - 8) * 2^-24
+    int e;
 };
 
 template <int D, int NT>
@@ -216,64 +243,66 @@ __device__ __forceinline__ void clear(State<D, NT>& st)
     st.e = 1;
 }
 
-// The query columns as B operands and their f32 companions.
+// The query columns as B operands and their f32 companions.  A column's
+// logits are `unit` (log2 units) times its product with the key.
 template <int D, int NT>
 struct Query {
     uint32_t b[D / 16][NT][2];
-    float scale[NT][2];                        // logits in log2 units per unit of the product with codes
-    float sum[NT][2][KvChunk<D>::kGroups];     // sum of the column over a group, in log2 units
-    int limit[NT][2], low[NT][2];              // keys seen: low < key <= limit
+    float unit[NT][2];
+    float sum[NT][2][KvChunk<D>::kGroups];  // sum of the column over a group
+    int limit[NT][2], low[NT][2];           // keys seen: low < key <= limit
 };
 
-// One page: scores, softmax update, weighted values.  `masked`: some token
-// of the page is hidden from some column; `shown` has a bit per token.
+// Scores of a page's 64 tokens x 8 NT columns from the key half of a chunk.
+// This lane's tokens are first + 2 i, i = 0 .. 7.  `masked`: some token of
+// the page is hidden from some column; `shown` has a bit per token.
 template <int D, int NT>
-__device__ __forceinline__ void attend_page(const unsigned char* chunk, const Query<D, NT>& q, State<D, NT>& st,
-                                            int key0, bool masked, uint64_t shown)
+__device__ __forceinline__ void page_scores(const unsigned char* keys, const Query<D, NT>& q, int key0, bool masked,
+                                            uint64_t shown, float (&s)[4][NT][4])
 {
-    using Chunk = KvChunk<D>;
-    constexpr int G = Chunk::kGroups;
+    constexpr int G = KvChunk<D>::kGroups;
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    const int first = 16 * (g >> 1) + (g & 1);  // this lane's tokens: first + 2 i, i = 0 .. 7
-    float s[4][NT][4];
-
-    // ---- scores of 64 tokens x 8 NT columns
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[kt][n][i] = 0.0f;
         uint32_t kp[2 * G];  // tokens first + 4 kt, + 2
-        load_words<2 * G>(chunk + Chunk::kKeyParams + (g * 4 + kt) * 8 * G, kp);
+        load_words<2 * G>(keys + KvChunk<D>::kKeyParams + (g * 4 + kt) * 8 * G, kp);
+        float acc[G][NT][4];
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-            const uint4 w4 = reinterpret_cast<const uint4*>(chunk)[(kt * G + grp) * 32 + lane];
+            const uint4 w4 = reinterpret_cast<const uint4*>(keys)[(kt * G + grp) * 32 + lane];
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-            float acc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t a[4];
                 code_operand(w[j], a);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, q.b[grp * 4 + j][n][0], q.b[grp * 4 + j][n][1]);
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t(&b)[2] = q.b[grp * 4 + j][n];
+                    mma_f16(acc[grp][n], a, b[0], b[1], j == 0 ? zero : acc[grp][n]);
+                }
             }
+        }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float ks = low_half(kp[r * G + grp]), km = high_half(kp[r * G + grp]);
+        for (int r = 0; r < 2; ++r) {
+            float2 sm[G];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int grp = 0; grp < G; ++grp) sm[grp] = both_halves(kp[r * G + grp]);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        s[kt][n][2 * r + c] += fmaf(acc[n][2 * r + c] * q.scale[n][c], ks, km * q.sum[n][c][grp]);
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = sm[0].y * q.sum[n][c][0];
+#pragma unroll
+                    for (int grp = 1; grp < G; ++grp) x = fmaf(sm[grp].y, q.sum[n][c][grp], x);
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp) x = fmaf(sm[grp].x, acc[grp][n][2 * r + c], x);
+                    s[kt][n][2 * r + c] = x;
+                }
         }
     }
     if (masked) {
+        const int first = 16 * (g >> 1) + (g & 1);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -287,24 +316,36 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
                         if (!on || key > q.limit[n][c] || key <= q.low[n][c]) s[kt][n][2 * r + c] = kNegInf;
             }
     }
+}
+
+// Softmax update and weighted values from the value half of a chunk.
+template <int D, int NT>
+__device__ __forceinline__ void page_values(const unsigned char* values, const Query<D, NT>& q, bool masked,
+                                            uint64_t shown, float (&s)[4][NT][4], State<D, NT>& st)
+{
+    constexpr int G = KvChunk<D>::kGroups, kAt = KvChunk<D>::kCodes;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const int first = 16 * (g >> 1) + (g & 1);
 
     // ---- the largest value scale; a hidden token's params may be anything,
     // so they count as 0 here and below
-    uint32_t top = 0;
+    const uint32_t* params = reinterpret_cast<const uint32_t*>(values + kAt) + g * 8 * G;
+    __half2 top = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        uint32_t w[G];
-        load_words<G>(chunk + Chunk::kValueParams + (g * 8 + i) * 4 * G, w);
+    for (int i = 0; i < 2 * G; ++i) {
+        uint32_t w[4];
+        load_words<4>(reinterpret_cast<const unsigned char*>(params + 4 * i), w);
 #pragma unroll
-        for (int grp = 0; grp < G; ++grp)
-            if (!masked || ((shown >> (first + 2 * i)) & 1)) top = max(top, w[grp] & 0x7c00u);
+        for (int k = 0; k < 4; ++k) {
+            if (masked && !((shown >> (first + 2 * ((4 * i + k) / G))) & 1)) w[k] = 0;
+            top = __hmax2(top, *reinterpret_cast<const __half2*>(&w[k]));
+        }
     }
-    // The weights p * scale become f16 operands.  They are taken relative to
-    // the largest scale exponent so far (2^26-e below), so that f16 holds
-    // them from 2^12 down to 2^-24 whatever the values' magnitude.
-    const int e = max(st.e, static_cast<int>(__reduce_max_sync(kFull, top) >> 10));
+    const uint32_t top_bits = *reinterpret_cast<const uint32_t*>(&top) & 0x7c00u;
+    const int e = max(st.e, static_cast<int>(__reduce_max_sync(kFull, top_bits) >> 10));
+    const float shift = static_cast<float>(e - st.e), up = static_cast<float>(26 - e);
+    st.e = e;
     float rescale[NT][2];
-    const float shift = exp2f(static_cast<float>(st.e - e));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -315,42 +356,44 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-            const float use = mx == kNegInf ? 0.0f : mx;
-            const float f = exp2_fast(st.m[n][c] - use);
+            const float use = mx == kNegInf ? 0.0f : mx, unit = q.unit[n][c];
+            const float f = exp2_fast(fmaf(st.m[n][c] - use, unit, -shift));
+            const float base = fmaf(use, unit, -up);
             st.m[n][c] = mx;
-            st.l[n][c] *= f;
-#pragma unroll
-            for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] *= f;
-            rescale[n][c] = f * shift;
+            rescale[n][c] = f;
+            float l = st.l[n][c] * f;
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float x = exp2_fast(s[kt][n][2 * r + c] - use);
+                    const float x = exp2_fast(fmaf(s[kt][n][2 * r + c], unit, -base));
                     s[kt][n][2 * r + c] = x;
-                    st.l[n][c] += x;
+                    l += x;
                 }
+            st.l[n][c] = l;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] *= f;
         }
-    st.e = e;
 
     // ---- weighted values.  The matrix instruction truncates its sums, so a
     // long chain of the codes' one-sided products would drift: codes are
     // centred (8 times the sum of the weights is taken off by the same
-    // instructions on a constant operand) and a page's sum joins the running
+    // instruction on a constant operand) and a page's sum joins the running
     // one by an f32 fma that also rescales it.
     const uint32_t eight[4] = {0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u};  // -8 * 2^-24, -8 * 2^-20
-    const float up = exp2f(static_cast<float>(26 - e));
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
         uint32_t b[4][NT][2];
+        float centre[NT][4];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
+        for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                uint32_t w = reinterpret_cast<const uint32_t*>(chunk + Chunk::kValueParams)[(g * 8 + 2 * kt + r) * G + grp];
+                uint32_t w = params[(2 * kt + r) * G + grp];
                 if (masked && !((shown >> (first + 4 * kt + 2 * r)) & 1)) w = 0;
-                const float scale = low_half(w), vs = scale * (r ? up * 0.0625f : up);
-                const float vm = fmaf(8.0f, scale, high_half(w));
+                const float2 sm = both_halves(w);
+                const float vs = r ? sm.x * 0.0625f : sm.x, vm = fmaf(8.0f, sm.x, sm.y);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float p0 = s[kt][n][2 * r], p1 = s[kt][n][2 * r + 1];
@@ -359,30 +402,21 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
                     b[kt][n][r] = transpose8x8(pack_f16(p0 * vs, p1 * vs));
                 }
             }
-        float centre[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) centre[n][i] = 0.0f;
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) mma_f16(centre[n], eight, b[kt][n][0], b[kt][n][1]);
+            for (int n = 0; n < NT; ++n) mma_f16(centre[n], eight, b[kt][n][0], b[kt][n][1], kt == 0 ? zero : centre[n]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int dt = grp * 4 + i;
             float acc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[n][k] = centre[n][k];
-            const uint4 w4 = reinterpret_cast<const uint4*>(chunk + Chunk::kValueCodes)[dt * 32 + lane];
+            const uint4 w4 = reinterpret_cast<const uint4*>(values)[dt * 32 + lane];
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t a[4];
                 code_operand(w[kt], a);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, b[kt][n][0], b[kt][n][1]);
+                for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, b[kt][n][0], b[kt][n][1], kt == 0 ? centre[n] : acc[n]);
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -393,12 +427,13 @@ __device__ __forceinline__ void attend_page(const unsigned char* chunk, const Qu
 }
 
 template <int D, int NT>
-__device__ __forceinline__ void load_query(const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                                           const Tile& tile, uint32_t head, int group, bool selected, bool wide,
-                                           Query<D, NT>& q)
+__device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head,
+                                           int group, bool selected, bool wide, Query<D, NT>& q)
 {
     constexpr int G = KvChunk<D>::kGroups;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // a negative scale turns the query around, a scale of 0 makes it 0
+    const float sign = p.scale < 0.0f ? -1.0f : p.scale > 0.0f ? 1.0f : 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         // this lane's column g: 16 dimensions of each group
@@ -422,48 +457,49 @@ __device__ __forceinline__ void load_query(const gofann_kv_batch& batch, const g
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[grp][j][k] = 0.0f;
         }
-        float sum[G];
 #pragma unroll
-        for (int grp = 0; grp < G; ++grp) {
-            sum[grp] = 0.0f;
+        for (int grp = 0; grp < G; ++grp)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    top = fmaxf(top, fabsf(x[grp][j][k]));
-                    sum[grp] += x[grp][j][k];
-                }
-            sum[grp] += __shfl_xor_sync(kFull, sum[grp], 1);
-            sum[grp] += __shfl_xor_sync(kFull, sum[grp], 2);
-        }
+                for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[grp][j][k]));
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
         // a power of two brings the column's largest value to [2^13, 2^14):
         // every bf16 or f16 within 2^27 of it is then an exact f16
         int ex = static_cast<int>(__float_as_uint(top) >> 23);
         ex = ex < 28 ? 28 : ex > 240 ? 240 : ex;
-        const float down = __uint_as_float(static_cast<uint32_t>(267 - ex) << 23);  // 2^(140 - ex)
+        const float down = __uint_as_float(static_cast<uint32_t>(267 - ex) << 23) * sign;  // 2^(140 - ex)
+        float sum[G];
 #pragma unroll
-        for (int grp = 0; grp < G; ++grp)
+        for (int grp = 0; grp < G; ++grp) {
+            sum[grp] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float(&y)[4] = x[grp][j];
-                q.b[grp * 4 + j][n][0] = pack_f16(y[0] * down, y[1] * down);
-                q.b[grp * 4 + j][n][1] = pack_f16(y[2] * down * 0.0625f, y[3] * down * 0.0625f);
+                float y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    y[k] = x[grp][j][k] * down;
+                    sum[grp] += y[k];
+                }
+                q.b[grp * 4 + j][n][0] = pack_f16(y[0], y[1]);
+                q.b[grp * 4 + j][n][1] = pack_f16(y[2] * 0.0625f, y[3] * 0.0625f);
             }
-        const float unit = p.scale * kLog2e;
+            sum[grp] += __shfl_xor_sync(kFull, sum[grp], 1);
+            sum[grp] += __shfl_xor_sync(kFull, sum[grp], 2);
+            sum[grp] *= 0x1p-24f;  // the unit of the codes' products
+        }
         // 2^(ex - 140) undoes `down`, 2^24 the codes' subnormals
-        const float undo = unit * exp2f(static_cast<float>(ex - 140 + 24));
+        const float undo = p.scale == 0.0f ? 1.0f : fmaxf(fabsf(p.scale) * kLog2e * exp2f(static_cast<float>(ex - 140 + 24)), FLT_MIN);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            q.scale[n][e] = __shfl_sync(kFull, undo, 4 * (2 * t + e));
+            q.unit[n][e] = __shfl_sync(kFull, undo, 4 * (2 * t + e));
 #pragma unroll
-            for (int grp = 0; grp < G; ++grp) q.sum[n][e][grp] = __shfl_sync(kFull, sum[grp] * unit, 4 * (2 * t + e));
+            for (int grp = 0; grp < G; ++grp) q.sum[n][e][grp] = __shfl_sync(kFull, sum[grp], 4 * (2 * t + e));
             const int cc = n * 8 + 2 * t + e;
             const int row = selected ? tile.row : (tile.col0 + cc) / group;
             const int pos = tile.len - tile.n_rows + row;
-            // padding columns see what the tile's last column sees
-            int limit = p.causal ? (pos < tile.len ? pos : tile.len - 1) : tile.len - 1;
+            int limit = p.causal ? pos : tile.len - 1;
             if (pos < 0) limit = -1;
             const long long low = p.window ? static_cast<long long>(pos) - p.window : -1;
             q.limit[n][e] = limit;
@@ -476,26 +512,34 @@ __device__ __forceinline__ void load_query(const gofann_kv_batch& batch, const g
     }
 }
 
-// Shared memory of a block: a ring of kStages chunks per warp, the warps'
-// partial results of a segment, the ring's barriers.
+// A thread block's warps and shared memory: per warp a ring of half chunks
+// (keys or values), the place of a partial result, two heads; two sets of
+// partial results are enough because a warp's units are consecutive.
 template <int D, int NT>
-struct AttendShared {
+struct Attend {
     static constexpr int kCols = 8 * NT;
-    static constexpr int kStages = D == 64 ? 4 : 2;
-    static constexpr size_t kRing = static_cast<size_t>(kAttendWarps) * kStages * KvChunk<D>::kBytes;
-    static constexpr size_t kMerge = sizeof(float) * kAttendWarps * kCols * (D + 4 + 2);
-    static constexpr size_t kBytes = kRing + kMerge + sizeof(uint64_t) * kAttendWarps * kStages;
+    static constexpr int kWarps = D * NT <= 128 ? 12 : 8;  // 168 or 255 registers a thread
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kHalf = KvChunk<D>::kBytes / 2;
+    static constexpr int kSlots = D == 64 ? 6 : NT == 1 ? 3 : 4;
+    static constexpr int kPart = kCols * (D + 4) + 2 * kCols;  // floats: values, max, sum
+    static constexpr size_t kRing = static_cast<size_t>(kWarps) * kSlots * kHalf;
+    static constexpr size_t kFirst = sizeof(float) * kWarps * kPart;
+    static constexpr size_t kItems = sizeof(Item) * 2 * kWarps;
+    static constexpr size_t kBytes = kRing + kFirst + kItems + sizeof(uint64_t) * kWarps * kSlots;
+    static_assert(sizeof(float) * kPart <= kSlots * kHalf, "a warp's last partial result takes its ring's place");
+    static_assert(kBytes <= 227 * 1024, "shared memory of a block");
 };
 
 // Units of one block: a share of the total, at least one per warp.
-__device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks)
+__device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks, int warps)
 {
     const uint64_t c = (total + blocks - 1) / blocks;
-    return c > kAttendWarps ? c : kAttendWarps;
+    return c > warps ? c : warps;
 }
 
-// A partial result in scratch: [cols] max, [cols] sum, [cols][D] values; two
-// per block (its first segment, and its last if that is another).
+// A block's partial result in scratch: [cols] max, [cols] sum, [cols][D]
+// values; two per block (its first item, and its last if that is another).
 template <int D, int NT>
 constexpr size_t kPartFloats = 8 * NT * (D + 2);
 
@@ -513,137 +557,202 @@ __device__ __forceinline__ void store_row(const gofann_kv_attention_params& p, c
     if (d == 0 && p.lse) p.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
 }
 
-// The chunks that a warp reads, in order: its share (every kAttendWarps-th
-// block) of each segment of the thread block.  Page numbers are looked up 32
-// blocks at a time, one per lane.
-template <int D, bool kSelected>
-struct Reader {
-    Segment sg;
-    int next;       // this warp's next block (or slot) of the segment
-    int batch_at;   // `next` of lane 0's entry
-    int block, page;  // this lane's entry: cache block and page, -1 = nothing to read
-    bool more;
-
-    __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofann_kv_batch& b,
-                                            const gofann_kv_attention_params& p)
-    {
-        const int lane = threadIdx.x & 31;
-        const int i = next + lane * kAttendWarps;
-        batch_at = next;
-        block = page = -1;
-        if (i < sg.b1) {
-            const int seq_blocks = (sg.tile.len + kKvPage - 1) / kKvPage;
-            block = i;
-            if (kSelected)
-                block = __ldg(p.selected +
-                              (static_cast<size_t>(sg.tile.first_row + sg.tile.row) * cache.n_kv_heads + sg.head) * p.n_select + i);
-            if (block >= 0 && block < seq_blocks) {
-                page = __ldg(b.page_table + static_cast<size_t>(sg.tile.seq) * b.max_pages + block);
-                if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
-                    page = -1;
-                    kv_invalid(b);
-                }
-            }
+// The rows of a whole item from the lanes that hold them: pairs of columns
+// become pairs of dimensions by the transposition that P takes.
+template <int D, int NT, bool kSelected>
+__device__ __forceinline__ void store_item(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head, int group,
+                                           const State<D, NT>& st)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const auto place = [&](int c) {
+        const int col = tile.col0 + c;
+        const uint64_t row = tile.first_row + (kSelected ? tile.row : col / group);
+        return row * p.n_heads + head * group + (kSelected ? col : col % group);
+    };
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float inv[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float l = st.l[n][c];
+            inv[c] = l > 0.0f ? 1.0f / l : 0.0f;
+            if (g == 0 && p.lse && n * 8 + 2 * t + c < tile.cols)
+                p.lse[place(n * 8 + 2 * t + c)] = l > 0.0f ? (st.m[n][c] + log2f(l)) * kLn2 : kNegInf;
         }
+        const bool on = n * 8 + g < tile.cols;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + (on ? place(n * 8 + g) : 0) * D;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float a = inv[0] > 0.0f ? st.o[dt][n][2 * r] * inv[0] : 0.0f;
+                const float b = inv[1] > 0.0f ? st.o[dt][n][2 * r + 1] * inv[1] : 0.0f;
+                const uint32_t w = transpose8x8(kv_pack2(a, b, p.dtype));
+                if (on) *reinterpret_cast<uint32_t*>(out + dt * 16 + 8 * r + 2 * t) = w;
+            }
     }
+}
+
+// What the 32 units from a multiple of 32 after a warp's first one read: lane
+// i has unit i's chunk (or nullptr) and cache block; `valid` has their bits.
+struct Batch32 {
+    const unsigned char* chunk;
+    int block;
+    unsigned valid;
 };
 
 template <int D, int NT, bool kSelected>
-__global__ void __launch_bounds__(kAttendThreads, 1) kv_attend_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
-                                                                      gofann_kv_attention_params p, bool wide,
-                                                                      float* __restrict__ parts)
+__device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofann_kv_batch& b,
+                                        const gofann_kv_attention_params& p, int group, uint64_t flat0, uint64_t end,
+                                        SeqCursor& c, Batch32& got)
 {
-    using Chunk = KvChunk<D>;
-    using Shared = AttendShared<D, NT>;
-    constexpr int G = Chunk::kGroups, kCols = 8 * NT, kStages = Shared::kStages;
-    extern __shared__ __align__(128) unsigned char smem[];
-    float* merge_o = reinterpret_cast<float*>(smem + Shared::kRing);  // [warps][cols][D + 4]
-    float* merge_m = merge_o + kAttendWarps * kCols * (D + 4);        // [warps][cols]
-    float* merge_l = merge_m + kAttendWarps * kCols;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const unsigned char* ring = smem + static_cast<size_t>(warp) * kStages * Chunk::kBytes;
-    const uint32_t bars = shared_addr(smem + Shared::kRing + Shared::kMerge) + warp * kStages * 8;
-    const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
+    constexpr int kCols = 8 * NT;
+    const uint64_t flat = flat0 + (threadIdx.x & 31);
+    const uint32_t n_kv = cache.n_kv_heads;
+    bool todo = flat < end;
+    got.chunk = nullptr;
+    got.block = 0;
+    while (true) {
+        if (todo && flat < c.end) {
+            todo = false;
+            const uint64_t at = flat - c.begin, i = at / c.span;
+            const uint32_t head = static_cast<uint32_t>(i % n_kv);
+            int block = c.lo + static_cast<int>(at - i * c.span);
+            Tile tile;
+            make_tile<kSelected>(b, p, group, kCols, c.seq, static_cast<int>(i / n_kv), tile);
+            bool on = true;
+            if (kSelected) {
+                block = __ldg(p.selected +
+                              (static_cast<size_t>(tile.first_row + tile.row) * n_kv + head) * p.n_select + block);
+                on = block >= 0 && block < (tile.len + kKvPage - 1) / kKvPage;
+            } else {
+                int lo, hi;
+                dense_blocks(p, group, tile.len, tile.n_rows, tile.col0, tile.cols, lo, hi);
+                on = block >= lo && block < hi;
+            }
+            if (on) {
+                const int32_t page = __ldg(b.page_table + static_cast<size_t>(c.seq) * b.max_pages + block);
+                if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
+                    kv_invalid(b);
+                } else {
+                    got.chunk = cache.pages + (static_cast<size_t>(page) * n_kv + head) * KvChunk<D>::kBytes;
+                    got.block = block;
+                }
+            }
+        }
+        if (!__any_sync(kFull, todo)) break;
+        next_sequence<kSelected>(b, p, n_kv, group, kCols, c);
+    }
+    got.valid = __ballot_sync(kFull, got.chunk != nullptr);
+}
 
-    if (lane < kStages) barrier_init(bars + 8 * lane, 1);
+// Each thread block takes an equal share of all units, each warp an equal,
+// consecutive part of the share; a warp that has a whole item writes its rows
+// itself.
+template <int D, int NT, bool kSelected>
+__global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(gofann_kv_cache cache,
+                                                                               gofann_kv_batch batch,
+                                                                               gofann_kv_attention_params p, bool wide,
+                                                                               float* __restrict__ parts)
+{
+    using Cfg = Attend<D, NT>;
+    constexpr int G = KvChunk<D>::kGroups, kCols = Cfg::kCols, kWarps = Cfg::kWarps, kSlots = Cfg::kSlots;
+    constexpr int kHalf = Cfg::kHalf, kPart = Cfg::kPart;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char* ring = smem + static_cast<size_t>(warp) * kSlots * kHalf;
+    const auto first_part = [&](int w) { return reinterpret_cast<float*>(smem + Cfg::kRing) + w * kPart; };
+    const auto last_part = [&](int w) { return reinterpret_cast<float*>(smem + static_cast<size_t>(w) * kSlots * kHalf); };
+    Item* items = reinterpret_cast<Item*>(smem + Cfg::kRing + Cfg::kFirst);  // [warps][first, last]
+    const uint32_t bars = shared_addr(smem + Cfg::kRing + Cfg::kFirst + Cfg::kItems) + warp * kSlots * 8;
+    const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
+    const uint32_t n_kv = cache.n_kv_heads;
+
+    if (lane < kSlots) barrier_init(bars + 8 * lane, 1);
     barrier_fence();
     launch_next();
+    if (lane < 2) items[2 * warp + lane].end = 0;  // no partial result
     __syncwarp();
-    const auto units = [&](uint32_t s) {
-        const SeqWork w = seq_work<kSelected>(batch, p, group, kCols, s);
-        return static_cast<uint64_t>(w.tiles) * cache.n_kv_heads * w.span;
-    };
-    const uint64_t total = kv_total<uint64_t>(batch.n_seqs, units);
-    const uint64_t share = units_per_block(total, gridDim.x);
+    const uint64_t total = total_units<kSelected>(batch, p, n_kv, group, kCols);
+    const uint64_t share = units_per_block(total, gridDim.x, kWarps);
     const uint64_t u0 = share * blockIdx.x, u1 = u0 + share < total ? u0 + share : total;
     if (u0 >= u1) return;
+    const uint64_t per_warp = (u1 - u0 + kWarps - 1) / kWarps;
+    const uint64_t w0 = u0 + warp * per_warp, w1 = w0 + per_warp < u1 ? w0 + per_warp : u1;
 
-    // ---- the loads run ahead of the work by up to kStages chunks
-    Reader<D, kSelected> rd;
-    rd.more = segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, u0, u1, rd.sg);
-    rd.next = rd.sg.b0 + warp;
-    rd.look_up(cache, batch, p);
-    uint32_t issued = 0, taken = 0;  // chunks of this warp
-    const auto advance = [&]() {     // issues the next chunk's load, skipping entries with nothing to read
-        while (rd.more) {
-            if (rd.next >= rd.sg.b1) {
-                rd.more = segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, rd.sg.end, u1, rd.sg);
-                if (!rd.more) return;
-                rd.next = rd.sg.b0 + warp;
-                rd.look_up(cache, batch, p);
-                continue;
-            }
-            int l = (rd.next - rd.batch_at) / kAttendWarps;
-            if (l >= 32) {
-                rd.look_up(cache, batch, p);
-                l = 0;
-            }
-            const int page = __shfl_sync(kFull, rd.page, l);
-            rd.next += kAttendWarps;
-            if (page < 0) continue;
-            if (lane == 0) {
-                const uint32_t st = issued % kStages;
-                barrier_expect(bars + 8 * st, Chunk::kBytes);
-                bulk_load(shared_addr(ring + st * Chunk::kBytes),
-                          cache.pages + (static_cast<size_t>(page) * cache.n_kv_heads + rd.sg.head) * Chunk::kBytes,
-                          Chunk::kBytes, bars + 8 * st);
-            }
-            ++issued;
-            return;
-        }
-    };
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) advance();
-
-    // ---- segment by segment
     bool alive = true;  // false once a wait has run out
-    uint64_t flat = u0;
-    Reader<D, kSelected> use;
-    while (segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, flat, u1, use.sg)) {
-        const Segment& sg = use.sg;
-        const Tile& tile = sg.tile;
-        Query<D, NT> q;
-        load_query<D, NT>(batch, p, tile, sg.head, group, kSelected, wide, q);
-        int limit = 0x7fffffff, low = -1;  // keys in (low, limit] are seen by every column
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                limit = min(limit, q.limit[n][e]);
-                low = max(low, q.low[n][e]);
+    if (w0 < w1) {
+        SeqCursor ahead, here;
+        seek<kSelected>(batch, p, n_kv, group, kCols, w0, ahead);
+        here = ahead;
+        Batch32 now, then;
+        look_up<D, NT, kSelected>(cache, batch, p, group, w0, w1, ahead, now);
+        then.valid = 0;
+        // half chunks in order: the valid units' keys and values.  `todo` has
+        // the units of a batch that are still to be loaded.
+        uint32_t issued = 0, taken = 0;
+        unsigned todo = now.valid, todo_then = 0;
+        const unsigned char* src = nullptr;  // the chunk whose values come next
+        const auto fill = [&]() {  // loads what the free slots hold
+            while (issued - taken < kSlots) {
+                if (!(issued & 1)) {
+                    const bool in_now = todo != 0;
+                    const unsigned from = in_now ? todo : todo_then;
+                    if (!from) return;
+                    const int l = __ffs(from) - 1;
+                    if (in_now) todo &= todo - 1; else todo_then &= todo_then - 1;
+                    const uint64_t mine = reinterpret_cast<uint64_t>(in_now ? now.chunk : then.chunk);
+                    src = reinterpret_cast<const unsigned char*>(__shfl_sync(kFull, mine, l));
+                }
+                if (lane == 0) {
+                    const uint32_t slot = issued % kSlots;
+                    barrier_expect(bars + 8 * slot, kHalf);
+                    bulk_load(shared_addr(ring + slot * kHalf), src + (issued & 1 ? kHalf : 0), kHalf, bars + 8 * slot);
+                }
+                ++issued;
             }
-        limit = __reduce_min_sync(kFull, limit);
-        low = __reduce_max_sync(kFull, low);
-        State<D, NT> st;
-        clear(st);
-        use.next = sg.b0 + warp;
-        while (use.next < sg.b1) {
-            use.look_up(cache, batch, p);
+        };
+        fill();
+
+        uint64_t flat = w0;
+        while (flat < w1) {
+            // ---- one item, or this warp's part of it
+            while (flat >= here.end) next_sequence<kSelected>(batch, p, n_kv, group, kCols, here);
+            Item item;
+            make_item<kSelected>(batch, p, n_kv, group, kCols, flat, here, item);
+            const Tile& tile = item.tile;
+            const uint64_t start = flat, stop = item.end < w1 ? item.end : w1;
+            Query<D, NT> q;
+            load_query<D, NT>(p, tile, item.head, group, kSelected, wide, q);
+            int limit = 0x7fffffff, low = -1;  // keys in (low, limit] are seen by every column
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    limit = min(limit, q.limit[n][e]);
+                    low = max(low, q.low[n][e]);
+                }
+            limit = __reduce_min_sync(kFull, limit);
+            low = __reduce_max_sync(kFull, low);
+            State<D, NT> st;
+            clear(st);
             const uint32_t* bits = p.key_bits ? p.key_bits + static_cast<size_t>(tile.seq) * p.key_words : nullptr;
 #pragma unroll 1
-            for (int l = 0; l < 32 && use.next < sg.b1; ++l, use.next += kAttendWarps) {
-                if (__shfl_sync(kFull, use.page, l) < 0) continue;
-                const int block = __shfl_sync(kFull, use.block, l), key0 = block * kKvPage;
+            for (; flat < stop; ++flat) {
+                const int l = static_cast<int>(flat - w0) & 31;
+                if (l == 0) {
+                    // the next 32 units are looked up a batch ahead of their loads
+                    if (flat != w0) {
+                        now = then;
+                        todo = todo_then;
+                    }
+                    then.valid = 0;
+                    if (flat + 32 < w1) look_up<D, NT, kSelected>(cache, batch, p, group, flat + 32, w1, ahead, then);
+                    todo_then = then.valid;
+                    fill();  // there may have been nothing to load until here
+                }
+                if (!((now.valid >> l) & 1) || !alive) continue;
+                const int block = __shfl_sync(kFull, now.block, l), key0 = block * kKvPage;
                 uint64_t shown = ~0ull;
                 if (bits) {
                     const uint32_t w = 2u * block;
@@ -652,82 +761,119 @@ __global__ void __launch_bounds__(kAttendThreads, 1) kv_attend_kernel(gofann_kv_
                 }
                 if (tile.len - key0 < kKvPage) shown &= (1ull << (tile.len - key0)) - 1;
                 const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
-                const uint32_t stage = taken % kStages;
-                alive = alive && barrier_wait(bars + 8 * stage, (taken / kStages) & 1);
+                float s[4][NT][4];
+                uint32_t slot = taken % kSlots;
+                alive = barrier_wait(bars + 8 * slot, (taken / kSlots) & 1);
                 if (!alive) continue;
-                attend_page<D, NT>(ring + stage * Chunk::kBytes, q, st, key0, masked, shown);
+                page_scores<D, NT>(ring + slot * kHalf, q, key0, masked, shown, s);
                 ++taken;
                 __syncwarp();
-                advance();
+                fill();
+                slot = taken % kSlots;
+                alive = barrier_wait(bars + 8 * slot, (taken / kSlots) & 1);
+                if (!alive) continue;
+                page_values<D, NT>(ring + slot * kHalf, q, masked, shown, s, st);
+                ++taken;
+                __syncwarp();
+                fill();
             }
-        }
 
-        // ---- this warp's partial result, in units of its own maximum
+            // ---- sums over the lanes that share a column
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = n * 8 + 2 * t + c;
-                float l = st.l[n][c];
+                for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFull, l, off);
-                if (g == 0) {
-                    merge_m[warp * kCols + col] = st.m[n][c];
-                    merge_l[warp * kCols + col] = l;
-                }
-                const float unit = exp2f(static_cast<float>(st.e - 2));  // 2^24 of the codes, 2^(e - 26) of the weights
+                    for (int off = 4; off < 32; off <<= 1) {
+                        st.l[n][c] += __shfl_xor_sync(kFull, st.l[n][c], off);
 #pragma unroll
-                for (int grp = 0; grp < G; ++grp) {
-                    float z = st.z[n][c][grp];
+                        for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] += __shfl_xor_sync(kFull, st.z[n][c][grp], off);
+                    }
+                    // the maximum becomes the base of the weights, in log2 units
+                    st.m[n][c] = st.l[n][c] > 0.0f ? fmaf(st.m[n][c], q.unit[n][c], static_cast<float>(st.e - 26)) : kNegInf;
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) z += __shfl_xor_sync(kFull, z, off);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
                         for (int r = 0; r < 2; ++r)
-                            merge_o[(warp * kCols + col) * (D + 4) + (grp * 4 + i) * 16 + 8 * r + g] =
-                                fmaf(st.o[grp * 4 + i][n][2 * r + c], unit, z);
+                            st.o[dt][n][2 * r + c] = fmaf(st.o[dt][n][2 * r + c], 0x1p24f, st.z[n][c][dt / 4]);
                 }
+            const bool whole = start == item.begin && flat == item.end;
+            const bool last = flat == w1;
+            if (whole) {
+                store_item<D, NT, kSelected>(p, tile, item.head, group, st);
+                continue;
             }
-        __syncthreads();
+            // a partial result; the warp's last one takes the place of its
+            // ring, which holds nothing more
+            for (; last && alive && taken < issued; ++taken)
+                alive = barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+            float* part = last ? last_part(warp) : first_part(warp);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = n * 8 + 2 * t + c;
+                    if (g == 0) {
+                        part[kCols * (D + 4) + col] = st.m[n][c];
+                        part[kCols * (D + 5) + col] = st.l[n][c];
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) part[col * (D + 4) + dt * 16 + 8 * r + g] = st.o[dt][n][2 * r + c];
+                }
+            if (lane == 0) items[2 * warp + (last ? 1 : 0)] = item;
+        }
+        for (; alive && taken < issued; ++taken) alive = barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+        if (!alive) {
+            // what is still in flight may not outlive the block's shared memory
+            for (; taken < issued; ++taken) barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+            if (lane == 0) kv_timeout(batch);
+        }
+    }
+    __syncthreads();
 
-        // ---- join the warps: the output where the block has the whole item,
-        // else a partial result for the joining kernel
-        const bool whole = flat == sg.item_begin && sg.end == sg.item_end;
-        float* part = parts + (2ull * blockIdx.x + (flat == u0 ? 0 : 1)) * kPartFloats<D, NT>;
-        for (int i = threadIdx.x; i < tile.cols * (D / 4); i += kAttendThreads) {
+    // ---- join the warps' partial results of each item, in unit order: the
+    // rows where the block has the whole item, else a partial result for the
+    // joining kernel
+    for (int e0 = 0; e0 < 2 * kWarps;) {
+        if (items[e0].end == 0) {
+            ++e0;
+            continue;
+        }
+        const Item item = items[e0];
+        int e1 = e0 + 1;
+        while (e1 < 2 * kWarps && (items[e1].end == 0 || items[e1].begin == item.begin)) ++e1;
+        const bool whole = item.begin >= u0 && item.end <= u1;
+        float* out = parts + (2ull * blockIdx.x + (item.begin <= u0 ? 0 : 1)) * kPartFloats<D, NT>;
+        for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += Cfg::kThreads) {
             const int c = i / (D / 4), d = i % (D / 4) * 4;
-            float m = kNegInf;
-#pragma unroll
-            for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, merge_m[w * kCols + c]);
-            float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const float base = m == kNegInf ? 0.0f : m;
-#pragma unroll
-            for (int w = 0; w < kAttendWarps; ++w) {
-                const float f = exp2_fast(merge_m[w * kCols + c] - base);
-                const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * kCols + c) * (D + 4) + d]);
-                l = fmaf(merge_l[w * kCols + c], f, l);
-                o[0] = fmaf(v.x, f, o[0]);
-                o[1] = fmaf(v.y, f, o[1]);
-                o[2] = fmaf(v.z, f, o[2]);
-                o[3] = fmaf(v.w, f, o[3]);
+            float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int e = e0; e < e1; ++e) {
+                if (items[e].end == 0) continue;
+                const float* part = e & 1 ? last_part(e >> 1) : first_part(e >> 1);
+                const float pm = part[kCols * (D + 4) + c], top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
+                const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
+                const float4 v = *reinterpret_cast<const float4*>(part + c * (D + 4) + d);
+                l = l * f + part[kCols * (D + 5) + c] * h;
+                o[0] = o[0] * f + v.x * h;
+                o[1] = o[1] * f + v.y * h;
+                o[2] = o[2] * f + v.z * h;
+                o[3] = o[3] * f + v.w * h;
+                m = top;
             }
             if (whole) {
-                store_row<D>(p, tile, sg.head, group, kSelected, c, d, m, l, o);
+                store_row<D>(p, item.tile, item.head, group, kSelected, c, d, m, l, o);
             } else {
                 if (d == 0) {
-                    part[c] = m;
-                    part[kCols + c] = l;
+                    out[c] = m;
+                    out[kCols + c] = l;
                 }
-                *reinterpret_cast<float4*>(part + 2 * kCols + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<float4*>(out + 2 * kCols + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
             }
         }
-        __syncthreads();
-        flat = sg.end;
+        e0 = e1;
     }
-    // loads in flight may not outlive the block's shared memory
-    for (; taken < issued; ++taken) alive = barrier_wait(bars + 8 * (taken % kStages), (taken / kStages) & 1) && alive;
-    if (!alive && lane == 0) kv_timeout(batch);
 }
 
 // Items that several blocks share: their partial results in block order, so
@@ -739,26 +885,25 @@ __global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gof
 {
     constexpr int kCols = 8 * NT;
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
-    const auto units = [&](uint32_t s) {
-        const SeqWork w = seq_work<kSelected>(batch, p, group, kCols, s);
-        return static_cast<uint64_t>(w.tiles) * cache.n_kv_heads * w.span;
-    };
-    const uint64_t share = units_per_block(kv_total<uint64_t>(batch.n_seqs, units), blocks);
-    // the blocks' ends inside items: block i joins the item that end i falls into, if it is the item's first
+    const uint32_t n_kv = cache.n_kv_heads;
+    const uint64_t total = total_units<kSelected>(batch, p, n_kv, group, kCols);
+    const uint64_t share = units_per_block(total, blocks, Attend<D, NT>::kWarps);
+    // block i joins the item that the end of share i cuts, if that is the item's first cut
     const uint64_t cut = share * (blockIdx.x + 1);
-    Segment sg;
-    if (!segment_at<kSelected>(batch, p, cache.n_kv_heads, group, kCols, cut, ~0ull, sg)) return;
-    if (sg.item_begin >= cut || sg.item_begin < share * blockIdx.x) return;
+    SeqCursor c;
+    Item item;
+    if (cut >= total || !seek<kSelected>(batch, p, n_kv, group, kCols, cut, c)) return;
+    make_item<kSelected>(batch, p, n_kv, group, kCols, cut, c, item);
+    if (item.begin >= cut || item.begin < share * blockIdx.x) return;
     wait_previous();
-    const uint64_t first = blockIdx.x, last = (sg.item_end - 1) / share;
-    for (int i = threadIdx.x; i < sg.tile.cols * (D / 4); i += 128) {
-        const int c = i / (D / 4), d = i % (D / 4) * 4;
+    const uint64_t first = blockIdx.x, last = (item.end - 1) / share;
+    for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += 128) {
+        const int col = i / (D / 4), d = i % (D / 4) * 4;
         float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (uint64_t b = first; b <= last; ++b) {
-            const bool start = share * b >= sg.item_begin;  // the item is the block's first segment
-            const float* part = parts + (2 * b + (start ? 0 : 1)) * kPartFloats<D, NT>;
-            const float pm = __ldcg(part + c), pl = __ldcg(part + kCols + c);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * kCols + c * D + d));
+            const float* part = parts + (2 * b + (item.begin <= share * b ? 0 : 1)) * kPartFloats<D, NT>;
+            const float pm = __ldcg(part + col), pl = __ldcg(part + kCols + col);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * kCols + col * D + d));
             const float top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
             const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
             l = l * f + pl * h;
@@ -768,17 +913,16 @@ __global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gof
             o[3] = o[3] * f + v.w * h;
             m = top;
         }
-        store_row<D>(p, sg.tile, sg.head, group, kSelected, c, d, m, l, o);
+        store_row<D>(p, item.tile, item.head, group, kSelected, col, d, m, l, o);
     }
 }
 
 // Thread blocks of the attention kernel: one per SM (the ring takes most of
 // its shared memory), no more than there can be units.
-uint32_t attend_blocks(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
+uint32_t attend_blocks(const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
 {
     const uint64_t span = p.selected ? p.n_select : batch.max_pages;
-    const uint64_t units = static_cast<uint64_t>(batch.n_rows) * p.n_heads * (span ? span : 1);
-    const uint64_t most = (units + kAttendWarps - 1) / kAttendWarps;
+    const uint64_t most = static_cast<uint64_t>(batch.n_rows) * p.n_heads * (span ? span : 1);
     const int sms = sm_count();
     const uint64_t want = sms > 0 ? sms : 1;
     return static_cast<uint32_t>(most < want ? most : want);
@@ -788,14 +932,14 @@ template <int D, int NT, bool kSelected>
 int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
                   float* parts, cudaStream_t s)
 {
-    const size_t smem = AttendShared<D, NT>::kBytes;
+    using Cfg = Attend<D, NT>;
     auto* kernel = kv_attend_kernel<D, NT, kSelected>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kBytes));
     if (e != cudaSuccess) return cuda_status(e, "kv_attention: shared memory attribute");
     const uintptr_t q = reinterpret_cast<uintptr_t>(p.q);
     const bool wide = (q & 7) == 0 && (p.q_stride & 3) == 0;
-    const uint32_t blocks = attend_blocks(cache, batch, p);
-    kernel<<<blocks, kAttendThreads, smem, s>>>(cache, batch, p, wide, parts);
+    const uint32_t blocks = attend_blocks(batch, p);
+    kernel<<<blocks, Cfg::kThreads, Cfg::kBytes, s>>>(cache, batch, p, wide, parts);
     GOFANN_CHECK_LAUNCH("kv_attend_kernel");
     if (blocks == 1) return GOFANN_OK;
     cudaLaunchConfig_t cfg{};

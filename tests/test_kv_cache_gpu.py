@@ -443,6 +443,16 @@ def test_attend_selected_blocks(rows, d, dtype, heads):
     run_attend(case, selected=sel, causal=False)
 
 
+def test_attend_long_gaps_of_nothing_to_read():
+    """Runs of hundreds of -1 between the selected blocks, and rows whose causal ends are 100 blocks apart."""
+    case = R.Case([64 * 30], [3], 4, 2, 64, BF16)
+    sel = torch.full((3, 2, 700), -1, dtype=torch.int32, device="cuda")
+    sel[:, :, 3], sel[:, 0, 250], sel[0, 1, 251], sel[:, :, 699] = 4, 7, 9, 20
+    run_attend(case, selected=sel)
+    run_attend(R.Case([6500, 70], [6500, 2], 1, 1, 64, F16), window=200)
+    run_attend(R.Case([6500], [6400], 1, 1, 64, F16))
+
+
 def test_attend_selected_is_attend_where_all_is_selected():
     case = R.Case([64 * 9 + 1], [4], 8, 2, 128, BF16)
     pages, q = case.random_pages(), case.normal(4, 8, 128)
