@@ -42,6 +42,15 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// (a, b) = (a, b) * f + c, two f32 fmas in one instruction.
+__device__ __forceinline__ void fma_pair(float& a, float& b, const float* f, const float* c)
+{
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 z, {%4, %5};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(f[0]), "f"(f[1]), "f"(c[0]), "f"(c[1]));
+}
 // The A operand of 16 rows x 16 steps from one word of eight codes.
 __device__ __forceinline__ void code_operand(uint32_t w, uint32_t (&a)[4])
 {
@@ -254,11 +263,11 @@ struct Query {
 };
 
 // Scores of a page's 64 tokens x 8 NT columns from the key half of a chunk.
-// This lane's tokens are first + 2 i, i = 0 .. 7.  `masked`: some token of
+// This lane's tokens are first + 2 i, i = 0 .. 7.  kMasked: some token of
 // the page is hidden from some column; `shown` has a bit per token.
-template <int D, int NT>
-__device__ __forceinline__ void page_scores(const unsigned char* keys, const Query<D, NT>& q, int key0, bool masked,
-                                            uint64_t shown, float (&s)[4][NT][4])
+template <int D, int NT, bool kMasked>
+__device__ __forceinline__ void page_scores(const unsigned char* keys, const Query<D, NT>& q, int key0, uint64_t shown,
+                                            float (&s)[4][NT][4])
 {
     constexpr int G = KvChunk<D>::kGroups;
     const int lane = threadIdx.x & 31, g = lane >> 2;
@@ -301,7 +310,7 @@ __device__ __forceinline__ void page_scores(const unsigned char* keys, const Que
                 }
         }
     }
-    if (masked) {
+    if constexpr (kMasked) {
         const int first = 16 * (g >> 1) + (g & 1);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -319,9 +328,9 @@ __device__ __forceinline__ void page_scores(const unsigned char* keys, const Que
 }
 
 // Softmax update and weighted values from the value half of a chunk.
-template <int D, int NT>
-__device__ __forceinline__ void page_values(const unsigned char* values, const Query<D, NT>& q, bool masked,
-                                            uint64_t shown, float (&s)[4][NT][4], State<D, NT>& st)
+template <int D, int NT, bool kMasked>
+__device__ __forceinline__ void page_values(const unsigned char* values, const Query<D, NT>& q, uint64_t shown,
+                                            float (&s)[4][NT][4], State<D, NT>& st)
 {
     constexpr int G = KvChunk<D>::kGroups, kAt = KvChunk<D>::kCodes;
     const int lane = threadIdx.x & 31, g = lane >> 2;
@@ -337,7 +346,7 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
         load_words<4>(reinterpret_cast<const unsigned char*>(params + 4 * i), w);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (masked && !((shown >> (first + 2 * ((4 * i + k) / G))) & 1)) w[k] = 0;
+            if (kMasked && !((shown >> (first + 2 * ((4 * i + k) / G))) & 1)) w[k] = 0;
             top = __hmax2(top, *reinterpret_cast<const __half2*>(&w[k]));
         }
     }
@@ -391,7 +400,7 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 uint32_t w = params[(2 * kt + r) * G + grp];
-                if (masked && !((shown >> (first + 4 * kt + 2 * r)) & 1)) w = 0;
+                if (kMasked && !((shown >> (first + 4 * kt + 2 * r)) & 1)) w = 0;
                 const float2 sm = both_halves(w);
                 const float vs = r ? sm.x * 0.0625f : sm.x, vm = fmaf(8.0f, sm.x, sm.y);
 #pragma unroll
@@ -421,7 +430,7 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) st.o[dt][n][k] = fmaf(st.o[dt][n][k], rescale[n][k & 1], acc[n][k]);
+                for (int k = 0; k < 4; k += 2) fma_pair(st.o[dt][n][k], st.o[dt][n][k + 1], rescale[n], acc[n] + k);
         }
     }
 }
@@ -512,20 +521,43 @@ __device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, 
     }
 }
 
+// The place of the next half chunk in a ring and the parity of its barrier.
+template <int kSlots>
+struct Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++slot == kSlots) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// What a warp keeps in shared memory to spare registers: the items of its
+// partial results (end 0 = none), the one in work, where its loads and its
+// work are.
+struct WarpItems {
+    Item part[2], now;  // part: the first item, the last
+    SeqCursor ahead, here;
+};
+
 // A thread block's warps and shared memory: per warp a ring of half chunks
-// (keys or values), the place of a partial result, two heads; two sets of
-// partial results are enough because a warp's units are consecutive.
+// (keys or values), the place of its first partial result (the last one takes
+// the ring's), its items.  Two partial results a warp are enough because its
+// units are consecutive.
 template <int D, int NT>
 struct Attend {
     static constexpr int kCols = 8 * NT;
     static constexpr int kWarps = D * NT <= 128 ? 12 : 8;  // 168 or 255 registers a thread
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kHalf = KvChunk<D>::kBytes / 2;
-    static constexpr int kSlots = D == 64 ? 6 : NT == 1 ? 3 : 4;
+    static constexpr int kSlots = D == 64 || NT == 2 ? 4 : 3;
     static constexpr int kPart = kCols * (D + 4) + 2 * kCols;  // floats: values, max, sum
     static constexpr size_t kRing = static_cast<size_t>(kWarps) * kSlots * kHalf;
     static constexpr size_t kFirst = sizeof(float) * kWarps * kPart;
-    static constexpr size_t kItems = sizeof(Item) * 2 * kWarps;
+    static constexpr size_t kItems = sizeof(WarpItems) * kWarps;
     static constexpr size_t kBytes = kRing + kFirst + kItems + sizeof(uint64_t) * kWarps * kSlots;
     static_assert(sizeof(float) * kPart <= kSlots * kHalf, "a warp's last partial result takes its ring's place");
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
@@ -663,7 +695,8 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     unsigned char* ring = smem + static_cast<size_t>(warp) * kSlots * kHalf;
     const auto first_part = [&](int w) { return reinterpret_cast<float*>(smem + Cfg::kRing) + w * kPart; };
     const auto last_part = [&](int w) { return reinterpret_cast<float*>(smem + static_cast<size_t>(w) * kSlots * kHalf); };
-    Item* items = reinterpret_cast<Item*>(smem + Cfg::kRing + Cfg::kFirst);  // [warps][first, last]
+    WarpItems* warp_items = reinterpret_cast<WarpItems*>(smem + Cfg::kRing + Cfg::kFirst);
+    WarpItems& mine = warp_items[warp];
     const uint32_t bars = shared_addr(smem + Cfg::kRing + Cfg::kFirst + Cfg::kItems) + warp * kSlots * 8;
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
     const uint32_t n_kv = cache.n_kv_heads;
@@ -671,7 +704,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     if (lane < kSlots) barrier_init(bars + 8 * lane, 1);
     barrier_fence();
     launch_next();
-    if (lane < 2) items[2 * warp + lane].end = 0;  // no partial result
+    if (lane < 2) mine.part[lane].end = 0;
     __syncwarp();
     const uint64_t total = total_units<kSelected>(batch, p, n_kv, group, kCols);
     const uint64_t share = units_per_block(total, gridDim.x, kWarps);
@@ -682,45 +715,73 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
 
     bool alive = true;  // false once a wait has run out
     if (w0 < w1) {
-        SeqCursor ahead, here;
-        seek<kSelected>(batch, p, n_kv, group, kCols, w0, ahead);
-        here = ahead;
         Batch32 now, then;
-        look_up<D, NT, kSelected>(cache, batch, p, group, w0, w1, ahead, now);
+        {
+            SeqCursor c;
+            seek<kSelected>(batch, p, n_kv, group, kCols, w0, c);
+            if (lane == 0) mine.here = c;
+            look_up<D, NT, kSelected>(cache, batch, p, group, w0, w1, c, now);
+            if (lane == 0) mine.ahead = c;
+            __syncwarp();
+        }
         then.valid = 0;
         // half chunks in order: the valid units' keys and values.  `todo` has
-        // the units of a batch that are still to be loaded.
-        uint32_t issued = 0, taken = 0;
+        // the units of a batch that are still to be loaded; a unit's own lane
+        // issues its loads.
+        Ring<kSlots> in, out;
+        int flight = 0;           // halves issued and not yet taken
         unsigned todo = now.valid, todo_then = 0;
-        const unsigned char* src = nullptr;  // the chunk whose values come next
+        int values_lane = -1;     // the lane whose chunk's values come next
+        const unsigned char* src = nullptr;
         const auto fill = [&]() {  // loads what the free slots hold
-            while (issued - taken < kSlots) {
-                if (!(issued & 1)) {
+            while (flight < kSlots) {
+                int l = values_lane;
+                int half = kHalf;
+                if (l < 0) {
+                    if (!(todo | todo_then)) return;
                     const bool in_now = todo != 0;
-                    const unsigned from = in_now ? todo : todo_then;
-                    if (!from) return;
-                    const int l = __ffs(from) - 1;
+                    l = __ffs(in_now ? todo : todo_then) - 1;
                     if (in_now) todo &= todo - 1; else todo_then &= todo_then - 1;
-                    const uint64_t mine = reinterpret_cast<uint64_t>(in_now ? now.chunk : then.chunk);
-                    src = reinterpret_cast<const unsigned char*>(__shfl_sync(kFull, mine, l));
+                    if (lane == l) src = in_now ? now.chunk : then.chunk;
+                    half = 0;
+                    values_lane = l;
+                } else {
+                    values_lane = -1;
                 }
-                if (lane == 0) {
-                    const uint32_t slot = issued % kSlots;
-                    barrier_expect(bars + 8 * slot, kHalf);
-                    bulk_load(shared_addr(ring + slot * kHalf), src + (issued & 1 ? kHalf : 0), kHalf, bars + 8 * slot);
+                if (lane == l) {
+                    barrier_expect(bars + 8 * in.slot, kHalf);
+                    bulk_load(shared_addr(ring) + in.slot * kHalf, src + half, kHalf, bars + 8 * in.slot);
                 }
-                ++issued;
+                in.next();
+                ++flight;
             }
+        };
+        const auto take = [&]() { return barrier_wait(bars + 8 * out.slot, out.phase); };
+        const auto release = [&]() {
+            out.next();
+            --flight;
+            __syncwarp();
         };
         fill();
 
         uint64_t flat = w0;
         while (flat < w1) {
             // ---- one item, or this warp's part of it
-            while (flat >= here.end) next_sequence<kSelected>(batch, p, n_kv, group, kCols, here);
-            Item item;
-            make_item<kSelected>(batch, p, n_kv, group, kCols, flat, here, item);
+            {
+                SeqCursor c = mine.here;
+                Item item;
+                __syncwarp();
+                while (flat >= c.end) next_sequence<kSelected>(batch, p, n_kv, group, kCols, c);
+                make_item<kSelected>(batch, p, n_kv, group, kCols, flat, c, item);
+                if (lane == 0) {
+                    mine.here = c;
+                    mine.now = item;
+                }
+                __syncwarp();
+            }
+            const Item& item = mine.now;
             const Tile& tile = item.tile;
+            const int len = tile.len;
             const uint64_t start = flat, stop = item.end < w1 ? item.end : w1;
             Query<D, NT> q;
             load_query<D, NT>(p, tile, item.head, group, kSelected, wide, q);
@@ -747,7 +808,13 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
                         todo = todo_then;
                     }
                     then.valid = 0;
-                    if (flat + 32 < w1) look_up<D, NT, kSelected>(cache, batch, p, group, flat + 32, w1, ahead, then);
+                    if (flat + 32 < w1) {
+                        SeqCursor c = mine.ahead;
+                        __syncwarp();
+                        look_up<D, NT, kSelected>(cache, batch, p, group, flat + 32, w1, c, then);
+                        if (lane == 0) mine.ahead = c;
+                        __syncwarp();
+                    }
                     todo_then = then.valid;
                     fill();  // there may have been nothing to load until here
                 }
@@ -759,22 +826,24 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
                     shown = (w < p.key_words ? __ldg(bits + w) : 0u) |
                             (static_cast<uint64_t>(w + 1 < p.key_words ? __ldg(bits + w + 1) : 0u) << 32);
                 }
-                if (tile.len - key0 < kKvPage) shown &= (1ull << (tile.len - key0)) - 1;
+                if (len - key0 < kKvPage) shown &= (1ull << (len - key0)) - 1;
                 const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
                 float s[4][NT][4];
-                uint32_t slot = taken % kSlots;
-                alive = barrier_wait(bars + 8 * slot, (taken / kSlots) & 1);
+                alive = take();
                 if (!alive) continue;
-                page_scores<D, NT>(ring + slot * kHalf, q, key0, masked, shown, s);
-                ++taken;
-                __syncwarp();
+                if (masked)
+                    page_scores<D, NT, true>(ring + out.slot * kHalf, q, key0, shown, s);
+                else
+                    page_scores<D, NT, false>(ring + out.slot * kHalf, q, key0, shown, s);
+                release();
                 fill();
-                slot = taken % kSlots;
-                alive = barrier_wait(bars + 8 * slot, (taken / kSlots) & 1);
+                alive = take();
                 if (!alive) continue;
-                page_values<D, NT>(ring + slot * kHalf, q, masked, shown, s, st);
-                ++taken;
-                __syncwarp();
+                if (masked)
+                    page_values<D, NT, true>(ring + out.slot * kHalf, q, shown, s, st);
+                else
+                    page_values<D, NT, false>(ring + out.slot * kHalf, q, shown, s, st);
+                release();
                 fill();
             }
 
@@ -805,8 +874,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
             }
             // a partial result; the warp's last one takes the place of its
             // ring, which holds nothing more
-            for (; last && alive && taken < issued; ++taken)
-                alive = barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+            for (; last && alive && flight; release()) alive = take();
             float* part = last ? last_part(warp) : first_part(warp);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -822,12 +890,12 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
 #pragma unroll
                         for (int r = 0; r < 2; ++r) part[col * (D + 4) + dt * 16 + 8 * r + g] = st.o[dt][n][2 * r + c];
                 }
-            if (lane == 0) items[2 * warp + (last ? 1 : 0)] = item;
+            if (lane == 0) mine.part[last ? 1 : 0] = item;
         }
-        for (; alive && taken < issued; ++taken) alive = barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+        for (; alive && flight; release()) alive = take();
         if (!alive) {
             // what is still in flight may not outlive the block's shared memory
-            for (; taken < issued; ++taken) barrier_wait(bars + 8 * (taken % kSlots), (taken / kSlots) & 1);
+            for (; flight; release()) take();
             if (lane == 0) kv_timeout(batch);
         }
     }
@@ -836,21 +904,22 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     // ---- join the warps' partial results of each item, in unit order: the
     // rows where the block has the whole item, else a partial result for the
     // joining kernel
+    const auto part_item = [&](int e) -> const Item& { return warp_items[e >> 1].part[e & 1]; };
     for (int e0 = 0; e0 < 2 * kWarps;) {
-        if (items[e0].end == 0) {
+        if (part_item(e0).end == 0) {
             ++e0;
             continue;
         }
-        const Item item = items[e0];
+        const Item item = part_item(e0);
         int e1 = e0 + 1;
-        while (e1 < 2 * kWarps && (items[e1].end == 0 || items[e1].begin == item.begin)) ++e1;
+        while (e1 < 2 * kWarps && (part_item(e1).end == 0 || part_item(e1).begin == item.begin)) ++e1;
         const bool whole = item.begin >= u0 && item.end <= u1;
         float* out = parts + (2ull * blockIdx.x + (item.begin <= u0 ? 0 : 1)) * kPartFloats<D, NT>;
         for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += Cfg::kThreads) {
             const int c = i / (D / 4), d = i % (D / 4) * 4;
             float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int e = e0; e < e1; ++e) {
-                if (items[e].end == 0) continue;
+                if (part_item(e).end == 0) continue;
                 const float* part = e & 1 ? last_part(e >> 1) : first_part(e >> 1);
                 const float pm = part[kCols * (D + 4) + c], top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
                 const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
