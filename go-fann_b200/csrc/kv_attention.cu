@@ -13,13 +13,10 @@
 // Tokens are the rows (M = 16) and query heads the columns (N = 8) of both
 // products: S^T = K Q^T, then O^T = V^T P^T; the transposition of P between
 // the two layouts is one movmatrix per 8 x 8 tile.
-#include "kv_async.cuh"
+#include "kv_attention.cuh"
 
 namespace gofann {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                         const float* c)
@@ -33,13 +30,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-// 2^x by the special function unit (2 ulp; results below 2^-126 are 0).
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 // (a, b) = (a, b) * f + c, two f32 fmas in one instruction.
@@ -92,18 +82,6 @@ struct Tile {
     int col0, cols;              // columns of the sequence (dense) or of the row (selected)
     int row;                     // selected: the row inside the sequence
 };
-
-// Cache blocks that the columns [col0, col0 + cols) of a sequence see.
-__device__ __forceinline__ void dense_blocks(const gofann_kv_attention_params& p, int group, int len, int n_rows,
-                                             int col0, int cols, int& lo, int& hi)
-{
-    const int pos0 = len - n_rows + col0 / group, pos1 = len - n_rows + (col0 + cols - 1) / group;
-    const int end = p.causal ? pos1 + 1 : len;
-    hi = end > 0 && pos1 >= 0 ? (end + kKvPage - 1) / kKvPage : 0;
-    const long long low = p.window ? static_cast<long long>(pos0) - p.window + 1 : 0;
-    lo = low > 0 ? static_cast<int>(low / kKvPage) : 0;
-    if (lo > hi) lo = hi;
-}
 
 // A sequence's share of the work in units of one cache block for one tile and
 // key/value head: every tile counts `span` blocks from `lo` on (what all of
@@ -474,11 +452,8 @@ __device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, 
                 for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[grp][j][k]));
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-        // a power of two brings the column's largest value to [2^13, 2^14):
-        // every bf16 or f16 within 2^27 of it is then an exact f16
-        int ex = static_cast<int>(__float_as_uint(top) >> 23);
-        ex = ex < 28 ? 28 : ex > 240 ? 240 : ex;
-        const float down = __uint_as_float(static_cast<uint32_t>(267 - ex) << 23) * sign;  // 2^(140 - ex)
+        const int ex = query_exponent(top);
+        const float down = power_of_two(ex) * sign;
         float sum[G];
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
@@ -498,8 +473,8 @@ __device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, 
             sum[grp] += __shfl_xor_sync(kFull, sum[grp], 2);
             sum[grp] *= 0x1p-24f;  // the unit of the codes' products
         }
-        // 2^(ex - 140) undoes `down`, 2^24 the codes' subnormals
-        const float undo = p.scale == 0.0f ? 1.0f : fmaxf(fabsf(p.scale) * kLog2e * exp2f(static_cast<float>(ex - 140 + 24)), FLT_MIN);
+        // undoes `down` and the codes' subnormals
+        const float undo = p.scale == 0.0f ? 1.0f : fmaxf(fabsf(p.scale) * kLog2e * power_of_two(24 - ex), FLT_MIN);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             q.unit[n][e] = __shfl_sync(kFull, undo, 4 * (2 * t + e));
@@ -507,12 +482,7 @@ __device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, 
             for (int grp = 0; grp < G; ++grp) q.sum[n][e][grp] = __shfl_sync(kFull, sum[grp], 4 * (2 * t + e));
             const int cc = n * 8 + 2 * t + e;
             const int row = selected ? tile.row : (tile.col0 + cc) / group;
-            const int pos = tile.len - tile.n_rows + row;
-            int limit = p.causal ? pos : tile.len - 1;
-            if (pos < 0) limit = -1;
-            const long long low = p.window ? static_cast<long long>(pos) - p.window : -1;
-            q.limit[n][e] = limit;
-            q.low[n][e] = low > -1 ? static_cast<int>(low) : -1;
+            row_limits(p, tile.len - tile.n_rows + row, tile.len, q.low[n][e], q.limit[n][e]);
             if (cc >= tile.cols) {  // no mask of its own: nothing of it is written
                 q.limit[n][e] = 0x7fffffff;
                 q.low[n][e] = -1;
@@ -797,7 +767,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
             low = __reduce_max_sync(kFull, low);
             State<D, NT> st;
             clear(st);
-            const uint32_t* bits = p.key_bits ? p.key_bits + static_cast<size_t>(tile.seq) * p.key_words : nullptr;
+            const uint32_t seq = tile.seq;
 #pragma unroll 1
             for (; flat < stop; ++flat) {
                 const int l = static_cast<int>(flat - w0) & 31;
@@ -820,13 +790,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
                 }
                 if (!((now.valid >> l) & 1) || !alive) continue;
                 const int block = __shfl_sync(kFull, now.block, l), key0 = block * kKvPage;
-                uint64_t shown = ~0ull;
-                if (bits) {
-                    const uint32_t w = 2u * block;
-                    shown = (w < p.key_words ? __ldg(bits + w) : 0u) |
-                            (static_cast<uint64_t>(w + 1 < p.key_words ? __ldg(bits + w + 1) : 0u) << 32);
-                }
-                if (len - key0 < kKvPage) shown &= (1ull << (len - key0)) - 1;
+                const uint64_t shown = shown_tokens(p, seq, len, block);
                 const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
                 float s[4][NT][4];
                 alive = take();
@@ -986,6 +950,10 @@ __global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gof
     }
 }
 
+// Query columns (rows x query heads) of a key/value head from which the
+// tensor memory kernel runs.
+constexpr uint64_t kManyColumns = 128;
+
 // Thread blocks of the attention kernel: one per SM (the ring takes most of
 // its shared memory), no more than there can be units.
 uint32_t attend_blocks(const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
@@ -1067,6 +1035,7 @@ int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* bat
     const uint32_t group = p.n_heads / cache->n_kv_heads;
     const uint64_t cols = p.selected ? group : static_cast<uint64_t>(batch->max_rows) * group;
     cudaStream_t s = as_stream(stream);
+    if (!p.selected && cols >= kManyColumns) return attend_rows(*cache, *batch, p, s);
     float* parts = static_cast<float*>(scratch);
 #define GOFANN_KV_LAUNCH(D, NT)                                                   \
     return p.selected ? launch_attend<D, NT, true>(*cache, *batch, p, parts, s) \

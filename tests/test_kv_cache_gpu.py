@@ -370,8 +370,7 @@ def run_attend(case, q=None, pages=None, scale=None, value_scale=0.2, **kw):
     out, lse = KVCache(case.d, pages=pages).attend(batch, q, scale=scale, **kw)
     batch.check()
     bits = kw.pop("key_bits", None)
-    want, want_lse, slack = R.attention(case, pages, q, scale, bits=bits, **kw)
-    R.check_attention(out, lse, want, want_lse, slack)
+    R.check_attention(out, lse, *R.attention(case, pages, q, scale, bits=bits, **kw))
     return out, lse
 
 
