@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kTileRows = 128, kTiles = 2;
 constexpr int kStepKeys = 2 * kKvPage;
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;  // a decode warp has a quarter of every group
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kRowThreads = 32 * (kLoadWarp + 1);
 constexpr float kLag = 8.0f;   // log2 that a column's maximum may run ahead of its reference
@@ -133,6 +133,28 @@ __device__ __forceinline__ void tensor_store(uint32_t addr, const uint32_t* r)
 }
 __device__ __forceinline__ void tensor_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two f32 numbers in one 64-bit register, for instructions on both.
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float first_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float second_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 // ------------------------------------------------------------------ decoding
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
@@ -184,26 +206,31 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
 {
     constexpr int G = KvChunk<D>::kGroups;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t* params = reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kValueParams);
+    // scales and minima of this lane's 16 tokens 16 t .. 16 t + 15, in pairs
+    __half2 s[G][8], m[G][8];
+    {
+        const uint4* params = reinterpret_cast<const uint4*>(chunk + KvChunk<D>::kValueParams) + t * 4 * G;
+#pragma unroll
+        for (int q = 0; q < 2 * G; ++q) {
+            const uint4 a4 = params[q], b4 = params[2 * G + q];  // even, odd tokens
+            uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = (4 * q + k) / G, grp = (4 * q + k) % G;  // tokens 16 t + 2 i, + 1
+                if (shown != ~0ull) {
+                    const uint32_t two = static_cast<uint32_t>(shown >> (16 * t + 2 * i));
+                    if (!(two & 1u)) a[k] = 0;
+                    if (!(two & 2u)) b[k] = 0;
+                }
+                s[grp][i] = as_half2(__byte_perm(a[k], b[k], 0x5410));
+                m[grp][i] = as_half2(__byte_perm(a[k], b[k], 0x7632));
+            }
+        }
+    }
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
-        // scales and minima of this lane's 16 tokens 16 t .. 16 t + 15, in pairs
-        __half2 s[8], m[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // tokens 16 t + 2 i, + 1
-            const int at = (i >> 1) * 2 + (i & 1);
-            uint32_t a = params[((2 * t) * 8 + at) * G + grp], b = params[((2 * t + 1) * 8 + at) * G + grp];
-            const uint32_t two = static_cast<uint32_t>(shown >> (16 * t + 2 * i)) & 3u;
-            if (two != 3u) {
-                if (!(two & 1u)) a = 0;
-                if (!(two & 2u)) b = 0;
-            }
-            s[i] = as_half2(__byte_perm(a, b, 0x5410));
-            m[i] = as_half2(__byte_perm(a, b, 0x7632));
-        }
-#pragma unroll
-        for (int i = warp; i < 4 * G; i += kDecodeWarps) {
-            if (i / 4 != grp) continue;
+        {
+            const int i = 4 * grp + warp;
             const uint4 w4 = reinterpret_cast<const uint4*>(chunk + KvChunk<D>::kValueCodes)[i * 32 + lane];
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
@@ -213,8 +240,8 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
                 for (int kt = 0; kt < 4; ++kt) {
                     __half2 a, b;
                     code_pairs(r ? w[kt] >> 8 : w[kt], a, b);
-                    out[2 * kt] = as_word(__hfma2(a, s[2 * kt], m[2 * kt]));
-                    out[2 * kt + 1] = as_word(__hfma2(b, s[2 * kt + 1], m[2 * kt + 1]));
+                    out[2 * kt] = as_word(__hfma2(a, s[grp][2 * kt], m[grp][2 * kt]));
+                    out[2 * kt + 1] = as_word(__hfma2(b, s[grp][2 * kt + 1], m[grp][2 * kt + 1]));
                 }
                 const int row = 16 * i + 8 * r + g;
                 unsigned char* dst = values + row * 128;
@@ -471,7 +498,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         const int warp_low = __reduce_max_sync(kFull, on ? low : -1);
 
         const uint32_t s_at = tmem + lanes + Cfg::kScores + tile * kStepKeys, o_at = tmem + lanes + Cfg::kOut + tile * D;
-        float ref = kNegInf, l = 0.0f;
+        float ref = kNegInf;
+        uint64_t l2 = 0;  // two parts of the sum of weights
         bool ok = true;
         for (int j = 0; j < steps; ++j) {
             ok = wait(s_full + 8 * tile, j);
@@ -480,15 +508,25 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             const int key0 = (lo + 2 * j) * kKvPage;
             const uint64_t shown[2] = {step_shown[(j & 3) * 2], step_shown[(j & 3) * 2 + 1]};
             const bool masked = (shown[0] & shown[1]) != ~0ull || key0 + kStepKeys - 1 > warp_limit || key0 <= warp_low;
-            uint32_t see[4];  // bits of the tokens that this column sees
             if (masked) {
-#pragma unroll
+                // hidden tokens' scores become -inf in place; the rest of the
+                // step then knows no mask
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     const int a = limit - (key0 + 32 * c), b = low - (key0 + 32 * c);
-                    see[c] = static_cast<uint32_t>(shown[c / 2] >> (32 * (c & 1)));
-                    see[c] &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
-                    see[c] &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
+                    uint32_t see = static_cast<uint32_t>(shown[c >> 1] >> (32 * (c & 1)));
+                    see &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
+                    see &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
+                    float v[32];
+                    tensor_load(s_at + 32 * c, v);
+                    tensor_wait_load();
+                    tensor_ready(v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!((see >> i) & 1)) v[i] = kNegInf;
+                    tensor_store(s_at + 32 * c, reinterpret_cast<const uint32_t*>(v));
                 }
+                tensor_wait_store();
             }
             float v[64];
             float mx = kNegInf;
@@ -499,13 +537,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                 tensor_wait_load();
                 tensor_ready(v);
                 tensor_ready(v + 32);
-                if (masked) {
+                float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (!((see[2 * c + i / 32] >> (i % 32)) & 1)) v[i] = kNegInf;
-                }
+                for (int i = 4; i < 64; i += 8)
 #pragma unroll
-                for (int i = 0; i < 64; ++i) mx = fmaxf(mx, v[i]);
+                    for (int k = 0; k < 4; ++k) m4[k] = i + 4 + k < 64 ? fmaxf(fmaxf(m4[k], v[i + k]), v[i + 4 + k]) : fmaxf(m4[k], v[i + k]);
+                mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
             }
             // the reference follows the maximum where that is far ahead
             float f = 1.0f;
@@ -514,7 +551,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             } else if ((mx - ref) * unit > kLag) {
                 f = exp2_fast((ref - mx) * unit);
                 ref = mx;
-                l *= f;
+                l2 = fma_two(l2, pair(f, f), 0);
             }
             if (__any_sync(kFull, f != 1.0f)) {
                 ok = wait(o_done + 8 * tile, j - 1);
@@ -531,7 +568,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                     tensor_store(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
                 }
             }
-            const float base = fmaf(ref == kNegInf ? 0.0f : ref, unit, -kHead);
+            const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
+            const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 tensor_load(s_at + 64 * c, v);
@@ -540,19 +578,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                 tensor_ready(v);
                 tensor_ready(v + 32);
                 uint32_t w[32];
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
-                    if (masked) {
-                        if (!((see[2 * c + i / 32] >> (i % 32)) & 1)) v[i] = kNegInf;
-                        if (!((see[2 * c + i / 32] >> (i % 32 + 1)) & 1)) v[i + 1] = kNegInf;
-                    }
-                    const float a = exp2_fast(fmaf(v[i], unit, -base)), b = exp2_fast(fmaf(v[i + 1], unit, -base));
-                    sum[i & 2] += a;
-                    sum[(i & 2) + 1] += b;
+                    const uint64_t x = fma_two(pair(v[i], v[i + 1]), unit2, minus_base2);
+                    const float a = exp2_fast(first_of(x)), b = exp2_fast(second_of(x));
+                    sum[(i >> 1) & 1] = add_two(sum[(i >> 1) & 1], pair(a, b));
                     w[i / 2] = as_word(__floats2half2_rn(a, b));
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l2 = add_two(l2, add_two(sum[0], sum[1]));
                 // P takes the columns of S that have been read
                 tensor_store(s_at + 32 * c, w);
             }
@@ -566,7 +600,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             fence_after();
         }
         if (ok) {
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float l = first_of(l2) + second_of(l2), inv = l > 0.0f ? 1.0f / l : 0.0f;
             uint16_t* out = static_cast<uint16_t*>(p.out) + out_row * D;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
