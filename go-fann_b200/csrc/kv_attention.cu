@@ -953,6 +953,11 @@ __global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gof
 // Query columns (rows x query heads) of a key/value head from which the
 // tensor memory kernel runs.
 constexpr uint64_t kManyColumns = 128;
+bool many_columns(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
+{
+    return !p.selected && cache.n_kv_heads &&
+           static_cast<uint64_t>(batch.max_rows) * (p.n_heads / cache.n_kv_heads) >= kManyColumns;
+}
 
 // Thread blocks of the attention kernel: one per SM (the ring takes most of
 // its shared memory), no more than there can be units.
@@ -1005,8 +1010,9 @@ size_t gofann_kv_attention_scratch_bytes(const gofann_kv_cache* cache, const gof
 {
     if (!cache || !batch || !params) return 0;
     const size_t part = sizeof(float) * (cache->head_dim <= 64 ? kPartFloats<64, 2> : kPartFloats<128, 2>);
-    const int sms = sm_count();
-    return 2 * part * static_cast<size_t>(sms > 0 ? sms : 1);
+    const int sms = sm_count() > 0 ? sm_count() : 1;
+    if (many_columns(*cache, *batch, *params)) return attend_rows_scratch(cache->head_dim, sms);
+    return 2 * part * static_cast<size_t>(sms);
 }
 
 int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
@@ -1035,8 +1041,8 @@ int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* bat
     const uint32_t group = p.n_heads / cache->n_kv_heads;
     const uint64_t cols = p.selected ? group : static_cast<uint64_t>(batch->max_rows) * group;
     cudaStream_t s = as_stream(stream);
-    if (!p.selected && cols >= kManyColumns) return attend_rows(*cache, *batch, p, s);
     float* parts = static_cast<float*>(scratch);
+    if (many_columns(*cache, *batch, p)) return attend_rows(*cache, *batch, p, parts, s);
 #define GOFANN_KV_LAUNCH(D, NT)                                                   \
     return p.selected ? launch_attend<D, NT, true>(*cache, *batch, p, parts, s) \
                       : launch_attend<D, NT, false>(*cache, *batch, p, parts, s)

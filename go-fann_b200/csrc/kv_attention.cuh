@@ -67,6 +67,7 @@ __device__ __forceinline__ uint64_t shown_tokens(const gofann_kv_attention_param
 // Attention of many query columns per key/value head on the tensor memory
 // path (kv_attention_rows.cu).
 int attend_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                cudaStream_t s);
+                float* parts, cudaStream_t s);
+size_t attend_rows_scratch(uint32_t head_dim, int sms);
 
 }  // namespace gofann

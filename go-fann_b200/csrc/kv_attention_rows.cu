@@ -2,18 +2,22 @@
 // the products of 256 query columns with 128 tokens at a time on the 5th
 // generation tensor cores.
 //
-// A block has two tiles of 128 query columns (token rows x query heads of one
-// key/value head) and walks their blocks of the cache, two pages (128 tokens)
-// a step:
+// A block takes two tiles of 128 query columns (token rows x query heads of
+// one key/value head) at a time and walks their blocks of the cache, two pages
+// (128 tokens) a step:
 // * a loader copies packed chunks to a shared ring (bulk copies);
-// * four warps turn codes into f16 keys [token][dim] and transposed values
+// * six warps turn codes into f16 keys [token][dim] and transposed values
 //   [dim][token], both 128-byte swizzled and K-major, each page once for all
 //   256 columns;
 // * one thread issues S = Q K^T (tcgen05.mma, M = 128, N = 128) and
 //   O += P V (M = 128, N = head_dim, P from tensor memory);
-// * two warpgroups, one thread a query column, turn S into P: maximum, mask,
+// * two warpgroups, one thread a query column, turn S into P: mask, maximum,
 //   exponential; P takes the place of S in tensor memory as f16.
 // While one tile is in the exponentials the other has the tensor cores.
+//
+// The steps of all items (256 columns, head) are dealt out evenly, one block
+// per SM: a block does a run of them, and an item that a share's end cuts is
+// joined from partial results by a second, programmatic launch.
 //
 // Precision: keys and values c * s + m are rounded to f16 (at most 2^-11 of
 // the value; a quantisation step is at least 2^-4 of the group's range, so
@@ -28,7 +32,9 @@ namespace {
 
 constexpr int kTileRows = 128, kTiles = 2;
 constexpr int kStepKeys = 2 * kKvPage;
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;  // a decode warp has a quarter of every group
+// 16 warps have 128 registers a thread.  The six that decode share a step's
+// 16 tasks: the keys and the values of two pages, in quarters.
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 6, kTasks = 8;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kRowThreads = 32 * (kLoadWarp + 1);
 constexpr float kLag = 8.0f;   // log2 that a column's maximum may run ahead of its reference
@@ -36,7 +42,6 @@ constexpr float kHead = 7.0f;  // log2 of a weight at the reference
 
 template <int D>
 struct Rows {
-    static constexpr int kPanels = D / 64;                          // 64 dimensions = one 128-byte swizzled row
     static constexpr int kQTile = kTileRows * D * 2;
     static constexpr int kKeys = kStepKeys * D * 2;                 // [panel][128 tokens][64 dims]
     static constexpr int kValues = kStepKeys * D * 2;               // [page][D dims][64 tokens]
@@ -47,7 +52,7 @@ struct Rows {
     static constexpr int kOffRaw = kOffV + 2 * kValues;
     static constexpr int kOffShown = kOffRaw + kRaw * kChunk;       // u64 [kRaw] of the ring, [4][2] of the steps
     static constexpr int kOffBars = kOffShown + 8 * (kRaw + 8);
-    static constexpr int kBars = 2 * kRaw + 8 + 3 * kTiles + 2;
+    static constexpr int kBars = 2 * kRaw + 8 + 2 * kTiles + 2;
     static constexpr int kBytes = 1024 + kOffBars + 8 * kBars + 16;
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
     // tensor memory columns
@@ -129,6 +134,24 @@ __device__ __forceinline__ void tensor_store(uint32_t addr, const uint32_t* r)
         "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
         "r"(r[31]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tensor_load16(uint32_t addr, uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tensor_store16(uint32_t addr, const uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
         : "memory");
 }
 __device__ __forceinline__ void tensor_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -253,14 +276,171 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
     }
 }
 
+// 16 columns times f: f32 numbers of the output, or pairs of f16 weights.
+// Rare, so kept out of the step's code.
+__device__ __noinline__ void scale_output(uint32_t addr, float f)
+{
+    uint32_t r[16];
+    tensor_load16(addr, r);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+    tensor_store16(addr, r);
+}
+__device__ __noinline__ void scale_weights(uint32_t addr, float f)
+{
+    uint32_t r[16];
+    tensor_load16(addr, r);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 x = __half22float2(as_half2(r[i]));
+        r[i] = as_word(__floats2half2_rn(x.x * f, x.y * f));
+    }
+    tensor_store16(addr, r);
+}
+
+// --------------------------------------------------------------- the schedule
+constexpr int kWidth = kTiles * kTileRows;
+
+// Work is counted in steps of one item (256 columns, key/value head); every
+// item has at least one, so that it has an owner.
+__device__ __forceinline__ int item_steps(const gofann_kv_attention_params& p, int group, int len, int n_rows, int tile)
+{
+    const int total = n_rows * group, col0 = tile * kWidth;
+    int lo, hi;
+    dense_blocks(p, group, len, n_rows, col0, total - col0 < kWidth ? total - col0 : kWidth, lo, hi);
+    const int steps = (hi - lo + 1) / 2;
+    return steps > 0 ? steps : 1;
+}
+
+// Where unit `flat` is (the warp's lanes share the tiles of a sequence), or
+// with `flat` past the end the number of all units.
+struct Place {
+    uint32_t seq, head;
+    int tile, step;
+    uint64_t total;
+};
+__device__ __forceinline__ Place locate(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+                                        int group, uint64_t flat)
+{
+    const int lane = threadIdx.x & 31;
+    Place at{0, 0, 0, 0, 0};
+    for (uint32_t s0 = 0; s0 < b.n_seqs; s0 += 32) {
+        int first, n = 0, len = 0;
+        if (s0 + lane < b.n_seqs) {
+            kv_rows(b, s0 + lane, first, n);
+            len = kv_len(b, s0 + lane);
+        }
+        for (int k = 0; k < 32 && s0 + k < b.n_seqs; ++k) {
+            const int rows = __shfl_sync(kFull, n, k), length = __shfl_sync(kFull, len, k);
+            const int tiles = (rows * group + kWidth - 1) / kWidth;
+            uint64_t sum = 0;
+            for (int i = lane; i < tiles; i += 32) sum += item_steps(p, group, length, rows, i);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+            if (sum == 0) continue;
+            if (flat < sum * n_kv) {
+                at.seq = s0 + k;
+                at.head = static_cast<uint32_t>(flat / sum);
+                uint64_t rest = flat % sum;
+                for (int i0 = 0;; i0 += 32) {
+                    const uint64_t c = i0 + lane < tiles ? item_steps(p, group, length, rows, i0 + lane) : 0;
+                    uint64_t upto = c;
+#pragma unroll
+                    for (int off = 1; off < 32; off <<= 1) {
+                        const uint64_t v = __shfl_up_sync(kFull, upto, off);
+                        if (lane >= off) upto += v;
+                    }
+                    const unsigned past = __ballot_sync(kFull, rest < upto);
+                    if (past) {
+                        const int l = __ffs(past) - 1;
+                        at.tile = i0 + l;
+                        at.step = static_cast<int>(rest - __shfl_sync(kFull, upto - c, l));
+                        return at;
+                    }
+                    rest -= __shfl_sync(kFull, upto, 31);
+                }
+            }
+            flat -= sum * n_kv;
+            at.total += sum * n_kv;
+        }
+    }
+    return at;
+}
+
+// An item and the steps [from, to) of it that a block does.
+struct Item {
+    uint32_t seq, head;
+    int tile, tiles;
+    int first_row, n_rows, len, col0, cols;
+    int lo, hi, steps, from, to;
+    uint64_t flat, limit;  // units: where this part starts, where the block's share ends
+};
+
+__device__ __forceinline__ void open_item(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group, int step,
+                                          Item& it)
+{
+    kv_rows(b, it.seq, it.first_row, it.n_rows);
+    it.len = kv_len(b, it.seq);
+    const int total = it.n_rows * group;
+    it.tiles = (total + kWidth - 1) / kWidth;
+    it.col0 = it.tile * kWidth;
+    it.cols = total - it.col0 < kWidth ? total - it.col0 : kWidth;
+    dense_blocks(p, group, it.len, it.n_rows, it.col0, it.cols, it.lo, it.hi);
+    it.steps = item_steps(p, group, it.len, it.n_rows, it.tile);
+    it.from = step;
+    const uint64_t left = it.limit - it.flat;
+    it.to = left < static_cast<uint64_t>(it.steps - step) ? step + static_cast<int>(left) : it.steps;
+}
+// The block's next item; false at the end of its share.
+__device__ __forceinline__ bool next_item(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+                                          int group, Item& it)
+{
+    it.flat += it.to - it.from;
+    if (it.flat >= it.limit) return false;
+    if (++it.tile == it.tiles) {
+        it.tile = 0;
+        if (++it.head == n_kv) {
+            it.head = 0;
+            int first, n = 0;
+            while (n == 0 && it.seq + 1 < b.n_seqs) kv_rows(b, ++it.seq, first, n);
+            if (n == 0) return false;
+        }
+    }
+    open_item(b, p, group, 0, it);
+    return true;
+}
+
+// Steps of one block: a share of the total, at least four (a partial result
+// costs about as much as one step).
+__device__ __forceinline__ uint64_t steps_per_block(uint64_t total, uint32_t blocks)
+{
+    const uint64_t c = (total + blocks - 1) / blocks;
+    return c > 4 ? c : 4;
+}
+
+// A block's partial result in scratch: [256] base, [256] sum, [D][256]
+// values, so that the threads of a warp, a column each, write side by side;
+// two per block (its first item, and its last if that is another).
+template <int D>
+constexpr size_t kRowPartFloats = kWidth * (D + 2);
+
+// Place of a column's row in out and lse.
+__device__ __forceinline__ uint64_t output_row(const gofann_kv_attention_params& p, int group, int first_row, uint32_t head,
+                                               int col)
+{
+    return static_cast<uint64_t>(first_row + col / group) * p.n_heads + head * group + col % group;
+}
+
 // ------------------------------------------------------------------ the kernel
 template <int D>
 __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
-                                                                        gofann_kv_attention_params p, bool wide)
+                                                                        gofann_kv_attention_params p, bool wide,
+                                                                        float* __restrict__ parts)
 {
     using Cfg = Rows<D>;
     constexpr int kRaw = Cfg::kRaw;
     extern __shared__ unsigned char smem_raw[];
+    __shared__ Item start, warp_items[kSoftmaxWarps];  // of the softmax warps, to spare registers
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* raw_shown = reinterpret_cast<uint64_t*>(smem + Cfg::kOffShown);  // [kRaw]
@@ -269,51 +449,52 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * kRaw;
     const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
     const uint32_t s_full = v_empty + 16, p_full = s_full + 8 * kTiles, o_done = p_full + 8 * kTiles;
-    const uint32_t q_full = o_done + 8 * kTiles, all_done = q_full + 8;
+    const uint32_t q_full = o_done + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffBars + 8 * Cfg::kBars);
     volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a wait has run out
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
-    const uint32_t head = blockIdx.y;
-    // the sequence's last columns see most under a causal mask: they go first
-    uint32_t seq, tile_at;
-    const auto tiles = [&](uint32_t s) {
-        int first, n;
-        kv_rows(batch, s, first, n);
-        return static_cast<uint32_t>((n * group + kTiles * kTileRows - 1) / (kTiles * kTileRows));
-    };
-    if (!kv_find<uint32_t>(batch.n_seqs, gridDim.x - 1 - blockIdx.x, tiles, seq, tile_at)) return;
-    int first_row, n_rows;
-    kv_rows(batch, seq, first_row, n_rows);
-    const int len = kv_len(batch, seq);
-    const int col0 = static_cast<int>(tile_at) * kTiles * kTileRows, total = n_rows * group;
-    const int cols = total - col0 < kTiles * kTileRows ? total - col0 : kTiles * kTileRows;
-    int lo, hi;
-    dense_blocks(p, group, len, n_rows, col0, cols, lo, hi);
-    const int pages = hi - lo, steps = (pages + 1) / 2;
-
-    if (threadIdx.x == 0) {
+    const uint32_t n_kv = cache.n_kv_heads;
+    launch_next();
+    if (warp == 0) {
+        const uint64_t total = locate(batch, p, n_kv, group, ~0ull).total;
+        const uint64_t share = steps_per_block(total, gridDim.x), u0 = share * blockIdx.x;
+        Item it{};
+        if (u0 < total) {
+            const Place at = locate(batch, p, n_kv, group, u0);
+            it.seq = at.seq;
+            it.head = at.head;
+            it.tile = at.tile;
+            it.flat = u0;
+            it.limit = u0 + share < total ? u0 + share : total;
+            open_item(batch, p, group, at.step, it);
+        }
+        if (lane == 0) start = it;
+    }
+    if (warp == 1 && lane == 0) {
         for (int i = 0; i < kRaw; ++i) {
             barrier_init(raw_full + 8 * i, 1);
-            barrier_init(raw_empty + 8 * i, kDecodeWarps);
+            barrier_init(raw_empty + 8 * i, kTasks);  // four of keys, four of values
         }
         for (int i = 0; i < 2; ++i) {
-            barrier_init(k_full + 8 * i, kDecodeWarps);
+            barrier_init(k_full + 8 * i, kTasks);
             barrier_init(k_empty + 8 * i, 1);
-            barrier_init(v_full + 8 * i, kDecodeWarps);
+            barrier_init(v_full + 8 * i, kTasks);
             barrier_init(v_empty + 8 * i, 1);
         }
         for (int i = 0; i < kTiles; ++i) {
             barrier_init(s_full + 8 * i, 1);
             barrier_init(p_full + 8 * i, kTileRows);
-            barrier_init(o_done + 8 * i, 1);
         }
+        barrier_init(o_done, 1);
         barrier_init(q_full, kTiles * kTileRows);
-        barrier_init(all_done, 1);
         barrier_fence();
         *dead = 0;
     }
+    __syncthreads();
+    if (start.limit == 0) return;
+    const uint64_t u0 = start.flat;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(tmem_slot)),
                      "r"(Cfg::kColumns)
@@ -330,54 +511,60 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         *dead = 1;
         return false;
     };
-
     if (warp == kLoadWarp) {
+        Item it = start;
         // ---- loader: page numbers are looked up 32 blocks at a time
-        int page = -1, issued = 0;
-        uint64_t shown = 0;
-        for (int i = 0; i < 2 * steps; ++i) {
-            if ((i & 31) == 0) {
-                const int block = lo + i + lane;
-                page = -1;
-                shown = 0;
-                if (block < hi) {
-                    page = __ldg(batch.page_table + static_cast<size_t>(seq) * batch.max_pages + block);
-                    if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
-                        page = -1;
-                        kv_invalid(batch);
+        uint32_t i = 0;  // pages so far
+        bool ok = true;
+        do {
+            int page = -1;
+            uint64_t shown = 0;
+            const int block0 = it.lo + 2 * it.from, n = 2 * (it.to - it.from);
+            for (int k = 0; k < n; ++k, ++i) {
+                if ((k & 31) == 0) {
+                    const int block = block0 + k + lane;
+                    page = -1;
+                    shown = 0;
+                    if (block < it.hi && k + lane < n) {
+                        page = __ldg(batch.page_table + static_cast<size_t>(it.seq) * batch.max_pages + block);
+                        if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
+                            page = -1;
+                            kv_invalid(batch);
+                        } else {
+                            shown = shown_tokens(p, it.seq, it.len, block);
+                        }
+                    }
+                }
+                const uint32_t slot = i % kRaw;
+                const int from = __shfl_sync(kFull, page, k & 31);
+                const uint64_t bits = __shfl_sync(kFull, shown, k & 31);
+                ok = i < kRaw || wait(raw_empty + 8 * slot, i / kRaw - 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    raw_shown[slot] = bits;
+                    if (from >= 0) {
+                        barrier_expect(raw_full + 8 * slot, Cfg::kChunk);
+                        bulk_load(shared_addr(smem + Cfg::kOffRaw + slot * Cfg::kChunk),
+                                  cache.pages + (static_cast<size_t>(from) * n_kv + it.head) * Cfg::kChunk, Cfg::kChunk,
+                                  raw_full + 8 * slot);
                     } else {
-                        shown = shown_tokens(p, seq, len, block);
+                        barrier_arrive(raw_full + 8 * slot);
                     }
                 }
             }
-            const int slot = i % kRaw;
-            const int from = __shfl_sync(kFull, page, i & 31);
-            const uint64_t bits = __shfl_sync(kFull, shown, i & 31);
-            if (i >= kRaw && !wait(raw_empty + 8 * slot, i / kRaw - 1)) break;
-            if (lane == 0) {
-                raw_shown[slot] = bits;
-                if (from >= 0) {
-                    barrier_expect(raw_full + 8 * slot, Cfg::kChunk);
-                    bulk_load(shared_addr(smem + Cfg::kOffRaw + slot * Cfg::kChunk),
-                              cache.pages + (static_cast<size_t>(from) * cache.n_kv_heads + head) * Cfg::kChunk, Cfg::kChunk,
-                              raw_full + 8 * slot);
-                } else {
-                    barrier_arrive(raw_full + 8 * slot);
-                }
-            }
-            issued = i + 1;
-        }
+        } while (ok && next_item(batch, p, n_kv, group, it));
         // copies in flight may not outlive the block's shared memory
-        for (int i = issued > kRaw ? issued - kRaw : 0; i < issued; ++i)
-            if (!barrier_wait(raw_full + 8 * (i % kRaw), (i / kRaw) & 1)) *dead = 1;
+        for (uint32_t k = i > kRaw ? i - kRaw : 0; k < i; ++k)
+            if (!barrier_wait(raw_full + 8 * (k % kRaw), (k / kRaw) & 1)) *dead = 1;
     } else if (warp == kMmaWarp) {
         // ---- products, issued by one thread; the tensor cores take them in
         // order, so a tile's next S may be issued behind the product that
-        // still reads its P
-        if (lane == 0 && steps > 0) {
+        // still reads its P, and a commit behind S also stands for that product
+        if (lane == 0) {
+            Item it = start;
             const uint32_t base = shared_addr(smem);
-            const auto scores = [&](int tile, int j) {
-                const uint32_t q = base + tile * Cfg::kQTile, k = base + Cfg::kOffK + (j & 1) * Cfg::kKeys;
+            const auto scores = [&](int tile, uint32_t g) {
+                const uint32_t q = base + tile * Cfg::kQTile, k = base + Cfg::kOffK + (g & 1) * Cfg::kKeys;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
                     mma_shared(tmem + Cfg::kScores + tile * kStepKeys,
@@ -385,246 +572,271 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                                operand_desc(k + (i / 4) * (kStepKeys * 128) + (i % 4) * 32), mma_shape(kTileRows, kStepKeys),
                                i > 0);
                 mma_commit(s_full + 8 * tile);
+                if (tile == kTiles - 1) mma_commit(k_empty + 8 * (g & 1));
             };
-            bool ok = wait(q_full, 0) && wait(k_full, 0);
-            if (ok) {
+            uint32_t g = 0, items = 0;  // steps and items so far
+            bool ok = true;
+            do {
+                ok = wait(q_full, items) && wait(k_full + 8 * (g & 1), g >> 1);
+                if (!ok) break;
                 fence_after();
-                for (int tile = 0; tile < kTiles; ++tile) scores(tile, 0);
-                mma_commit(k_empty);
-            }
-            for (int j = 0; j < steps && ok; ++j) {
-                for (int tile = 0; tile < kTiles && ok; ++tile) {
-                    if (tile == 0) ok = wait(v_full + 8 * (j & 1), j >> 1);
-                    ok = ok && wait(p_full + 8 * tile, j);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t v = base + Cfg::kOffV + (j & 1) * Cfg::kValues;
+                for (int tile = 0; tile < kTiles; ++tile) scores(tile, g);
+                for (int j = it.from; j < it.to && ok; ++j, ++g) {
+                    for (int tile = 0; tile < kTiles; ++tile) {
+                        ok = (tile > 0 || wait(v_full + 8 * (g & 1), g >> 1)) && wait(p_full + 8 * tile, g);
+                        if (!ok) break;
+                        fence_after();
+                        const uint32_t v = base + Cfg::kOffV + (g & 1) * Cfg::kValues;
 #pragma unroll
-                    for (int i = 0; i < kStepKeys / 16; ++i)
-                        mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + 8 * i,
-                                   operand_desc(v + (i / 4) * (D * 128) + (i % 4) * 32), mma_shape(kTileRows, D),
-                                   j > 0 || i > 0);
-                    mma_commit(o_done + 8 * tile);
-                    if (tile == kTiles - 1) mma_commit(v_empty + 8 * (j & 1));
-                    if (j + 1 < steps) {
-                        if (tile == 0) {
-                            ok = wait(k_full + 8 * ((j + 1) & 1), (j + 1) >> 1);
-                            if (!ok) break;
-                            fence_after();
+                        for (int i = 0; i < kStepKeys / 16; ++i)
+                            mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + 8 * i,
+                                       operand_desc(v + (i / 4) * (D * 128) + (i % 4) * 32), mma_shape(kTileRows, D),
+                                       j > it.from || i > 0);
+                        if (tile == kTiles - 1) mma_commit(v_empty + 8 * (g & 1));
+                        if (j + 1 < it.to) {
+                            if (tile == 0) {
+                                ok = wait(k_full + 8 * ((g + 1) & 1), (g + 1) >> 1);
+                                if (!ok) break;
+                                fence_after();
+                            }
+                            scores(tile, g + 1);
                         }
-                        scores(tile, j + 1);
-                        if (tile == kTiles - 1) mma_commit(k_empty + 8 * ((j + 1) & 1));
                     }
                 }
-            }
-            mma_commit(all_done);
-            if (!barrier_wait(all_done, 0)) *dead = 1;
+                if (ok) mma_commit(o_done);
+                ++items;
+            } while (ok && next_item(batch, p, n_kv, group, it));
+            // nothing that was issued may outlive the block: the last commit
+            // stands for all of it
+            if (!ok) mma_commit(o_done);
+            if (!barrier_wait(o_done, (ok ? items - 1 : items) & 1)) *dead = 1;
         }
         __syncwarp();
     } else if (warp >= kSoftmaxWarps) {
         // ---- codes to f16 operands
         const int w = warp - kSoftmaxWarps;
-        for (int j = 0; j < steps; ++j) {
-            const int st = j & 1;
-            if (j >= 2 && !wait(k_empty + 8 * st, (j >> 1) - 1)) break;
-            unsigned char* keys = smem + Cfg::kOffK + st * Cfg::kKeys;
-            unsigned char* values = smem + Cfg::kOffV + st * Cfg::kValues;
-            bool ok = true;
-            for (int h = 0; h < 2 && ok; ++h) {
-                const int i = 2 * j + h, slot = i % kRaw;
-                ok = wait(raw_full + 8 * slot, i / kRaw);
-                if (!ok) break;
-                decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk, keys, h, w);
-                if (w == 0 && lane == 0) step_shown[(j & 3) * 2 + h] = raw_shown[slot];
+        Item it = start;
+        uint32_t g = 0;
+        bool ok = true;
+        do {
+            for (int j = it.from; j < it.to && ok; ++j, ++g) {
+                const uint32_t st = g & 1;
+                ok = g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1);
+                for (int task = w; task < kTasks && ok; task += kDecodeWarps) {
+                    const int page = task >> 2, quarter = task & 3;
+                    const uint32_t i = 2 * g + page, slot = i % kRaw;
+                    ok = wait(raw_full + 8 * slot, i / kRaw);
+                    if (!ok) break;
+                    decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
+                    if (quarter == 0 && lane == 0) step_shown[(g & 3) * 2 + page] = raw_shown[slot];
+                    fence_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        barrier_arrive(raw_empty + 8 * slot);
+                        barrier_arrive(k_full + 8 * st);
+                    }
+                }
+                ok = ok && (g < 2 || wait(v_empty + 8 * st, (g >> 1) - 1));
+                // from the other end, so that the warps with two tasks differ
+                for (int task = kDecodeWarps - 1 - w; task < kTasks && ok; task += kDecodeWarps) {
+                    const int page = task >> 2, quarter = task & 3;
+                    const uint32_t i = 2 * g + page, slot = i % kRaw;
+                    ok = wait(raw_full + 8 * slot, i / kRaw);
+                    if (!ok) break;
+                    decode_values<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk,
+                                     smem + Cfg::kOffV + st * Cfg::kValues + page * (D * 128), quarter, raw_shown[slot]);
+                    fence_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        barrier_arrive(raw_empty + 8 * slot);
+                        barrier_arrive(v_full + 8 * st);
+                    }
+                }
             }
-            if (!ok) break;
-            fence_shared();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(k_full + 8 * st);
-            if (j >= 2 && !wait(v_empty + 8 * st, (j >> 1) - 1)) break;
-            for (int h = 0; h < 2; ++h) {
-                const int slot = (2 * j + h) % kRaw;
-                decode_values<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk, values + h * (D * 128), w, raw_shown[slot]);
-                __syncwarp();
-                if (lane == 0) barrier_arrive(raw_empty + 8 * slot);
-            }
-            fence_shared();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(v_full + 8 * st);
-        }
+        } while (ok && next_item(batch, p, n_kv, group, it));
     } else {
         // ---- softmax: one thread a query column
-        const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int tile = warp >> 2, row = (warp & 3) * 32 + lane, col = tile * kTileRows + row;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const int col = tile * kTileRows + row;
-        const bool on = col < cols;
-        const int at_col = col0 + (on ? col : 0);
-        const uint64_t out_row =
-            static_cast<uint64_t>(first_row + at_col / group) * p.n_heads + head * group + at_col % group;
-        int low, limit;
-        row_limits(p, len - n_rows + at_col / group, len, low, limit);
-        float unit = 1.0f;
-        {
-            const uint64_t src = static_cast<uint64_t>(first_row + at_col / group) * p.q_stride +
-                                 static_cast<uint64_t>(head * group + at_col % group) * D;
-            float top = 0.0f;
-#pragma unroll 8
-            for (int d = 0; d < D; d += 4) {
-                float x[4];
-                kv_load4(p.q, src + d, p.dtype, wide, x);
-                top = fmaxf(fmaxf(fmaxf(top, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
-            }
-            const int ex = query_exponent(top);
-            // a negative scale turns the query around, a scale of 0 makes it 0
-            const float down = on ? power_of_two(ex) * (p.scale < 0.0f ? -1.0f : p.scale > 0.0f ? 1.0f : 0.0f) : 0.0f;
-            if (p.scale != 0.0f) unit = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(-ex), FLT_MIN);
-            unsigned char* q = smem + tile * Cfg::kQTile + row * 128;
-#pragma unroll 4
-            for (int d = 0; d < D; d += 8) {
-                float x[4], y[4];
-                kv_load4(p.q, src + d, p.dtype, wide, x);
-                kv_load4(p.q, src + d + 4, p.dtype, wide, y);
-                const uint4 w = make_uint4(as_word(__floats2half2_rn(x[0] * down, x[1] * down)),
-                                           as_word(__floats2half2_rn(x[2] * down, x[3] * down)),
-                                           as_word(__floats2half2_rn(y[0] * down, y[1] * down)),
-                                           as_word(__floats2half2_rn(y[2] * down, y[3] * down)));
-                *reinterpret_cast<uint4*>(q + (d / 64) * (kTileRows * 128) + (((d % 64 / 8) ^ (row & 7)) << 4)) = w;
-            }
-            fence_shared();
-            barrier_arrive(q_full);
-        }
-        // keys in (warp_low, warp_limit] are seen by every column of the warp
-        const int warp_limit = __reduce_min_sync(kFull, on ? limit : 0x7fffffff);
-        const int warp_low = __reduce_max_sync(kFull, on ? low : -1);
-
         const uint32_t s_at = tmem + lanes + Cfg::kScores + tile * kStepKeys, o_at = tmem + lanes + Cfg::kOut + tile * D;
-        float ref = kNegInf;
-        uint64_t l2 = 0;  // two parts of the sum of weights
+        if (lane == 0) warp_items[warp] = start;
+        __syncwarp();
+        const Item& it = warp_items[warp];
+        const auto advance = [&]() {
+            Item next = it;
+            __syncwarp();
+            const bool more = next_item(batch, p, n_kv, group, next);
+            if (lane == 0) warp_items[warp] = next;
+            __syncwarp();
+            return more;
+        };
+        uint32_t g = 0, items = 0;
         bool ok = true;
-        for (int j = 0; j < steps; ++j) {
-            ok = wait(s_full + 8 * tile, j);
-            if (!ok) break;
-            fence_after();
-            const int key0 = (lo + 2 * j) * kKvPage;
-            const uint64_t shown[2] = {step_shown[(j & 3) * 2], step_shown[(j & 3) * 2 + 1]};
-            const bool masked = (shown[0] & shown[1]) != ~0ull || key0 + kStepKeys - 1 > warp_limit || key0 <= warp_low;
-            if (masked) {
-                // hidden tokens' scores become -inf in place; the rest of the
-                // step then knows no mask
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    const int a = limit - (key0 + 32 * c), b = low - (key0 + 32 * c);
-                    uint32_t see = static_cast<uint32_t>(shown[c >> 1] >> (32 * (c & 1)));
-                    see &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
-                    see &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
-                    float v[32];
-                    tensor_load(s_at + 32 * c, v);
-                    tensor_wait_load();
-                    tensor_ready(v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (!((see >> i) & 1)) v[i] = kNegInf;
-                    tensor_store(s_at + 32 * c, reinterpret_cast<const uint32_t*>(v));
+        do {
+            const bool on = col < it.cols;
+            const int at_col = it.col0 + (on ? col : 0);
+            int low, limit;
+            row_limits(p, it.len - it.n_rows + at_col / group, it.len, low, limit);
+            float unit = 1.0f;
+            {
+                const uint64_t src = static_cast<uint64_t>(it.first_row + at_col / group) * p.q_stride +
+                                     static_cast<uint64_t>(it.head * group + at_col % group) * D;
+                float top = 0.0f;
+#pragma unroll 8
+                for (int d = 0; d < D; d += 4) {
+                    float x[4];
+                    kv_load4(p.q, src + d, p.dtype, wide, x);
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
                 }
-                tensor_wait_store();
+                const int ex = query_exponent(top);
+                // a negative scale turns the query around, a scale of 0 makes it 0
+                const float down = on ? power_of_two(ex) * (p.scale < 0.0f ? -1.0f : p.scale > 0.0f ? 1.0f : 0.0f) : 0.0f;
+                if (p.scale != 0.0f) unit = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(-ex), FLT_MIN);
+                unsigned char* q = smem + tile * Cfg::kQTile + row * 128;
+#pragma unroll 4
+                for (int d = 0; d < D; d += 8) {
+                    float x[4], y[4];
+                    kv_load4(p.q, src + d, p.dtype, wide, x);
+                    kv_load4(p.q, src + d + 4, p.dtype, wide, y);
+                    const uint4 w = make_uint4(as_word(__floats2half2_rn(x[0] * down, x[1] * down)),
+                                               as_word(__floats2half2_rn(x[2] * down, x[3] * down)),
+                                               as_word(__floats2half2_rn(y[0] * down, y[1] * down)),
+                                               as_word(__floats2half2_rn(y[2] * down, y[3] * down)));
+                    *reinterpret_cast<uint4*>(q + (d / 64) * (kTileRows * 128) + (((d % 64 / 8) ^ (row & 7)) << 4)) = w;
+                }
+                fence_shared();
+                barrier_arrive(q_full);
             }
-            float v[64];
-            float mx = kNegInf;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                tensor_load(s_at + 64 * c, v);
-                tensor_load(s_at + 64 * c + 32, v + 32);
-                tensor_wait_load();
-                tensor_ready(v);
-                tensor_ready(v + 32);
-                float m4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int i = 4; i < 64; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) m4[k] = i + 4 + k < 64 ? fmaxf(fmaxf(m4[k], v[i + k]), v[i + 4 + k]) : fmaxf(m4[k], v[i + k]);
-                mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-            }
-            // the reference follows the maximum where that is far ahead
-            float f = 1.0f;
-            if (ref == kNegInf) {
-                ref = mx;
-            } else if ((mx - ref) * unit > kLag) {
-                f = exp2_fast((ref - mx) * unit);
-                ref = mx;
-                l2 = fma_two(l2, pair(f, f), 0);
-            }
-            if (__any_sync(kFull, f != 1.0f)) {
-                ok = wait(o_done + 8 * tile, j - 1);
+            // keys in (warp_low, warp_limit] are seen by every column of the warp
+            const int warp_limit = __reduce_min_sync(kFull, on ? limit : 0x7fffffff);
+            const int warp_low = __reduce_max_sync(kFull, on ? low : -1);
+
+            float ref = kNegInf;
+            uint64_t l2 = 0;  // two parts of the sum of weights
+            const int from = it.from, to = it.to;
+            int key0 = (it.lo + 2 * from) * kKvPage;
+            for (int j = from; j < to; ++j, ++g, key0 += kStepKeys) {
+                ok = wait(s_full + 8 * tile, g);
                 if (!ok) break;
                 fence_after();
+                const uint64_t shown[2] = {step_shown[(g & 3) * 2], step_shown[(g & 3) * 2 + 1]};
+                const bool masked = (shown[0] & shown[1]) != ~0ull || key0 + kStepKeys - 1 > warp_limit || key0 <= warp_low;
+                if (masked) {
+                    // hidden tokens' scores become -inf in place; the rest of
+                    // the step then knows no mask
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        const int a = limit - (key0 + 32 * c), b = low - (key0 + 32 * c);
+                        uint32_t see = static_cast<uint32_t>(shown[c >> 1] >> (32 * (c & 1)));
+                        see &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
+                        see &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
+                        float v[32];
+                        tensor_load(s_at + 32 * c, v);
+                        tensor_wait_load();
+                        tensor_ready(v);
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
-                    tensor_load(o_at + 32 * c, o);
+                        for (int i = 0; i < 32; ++i)
+                            if (!((see >> i) & 1)) v[i] = kNegInf;
+                        tensor_store(s_at + 32 * c, reinterpret_cast<const uint32_t*>(v));
+                    }
+                    tensor_wait_store();
+                }
+                // 32 tokens at a time, the next ones on their way
+                float v[2][32];
+                tensor_load(s_at, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float(&x)[32] = v[c & 1];
                     tensor_wait_load();
-                    tensor_ready(o);
+                    tensor_ready(x);
+                    if (c < 3) tensor_load(s_at + 32 * (c + 1), v[(c + 1) & 1]);
+                    float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] *= f;
-                    tensor_store(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+                    for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], x[i + k]), x[i + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[28 + k]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    // the reference follows the maximum where that is far
+                    // ahead; what was weighed by the old one is rescaled (the
+                    // output is complete up to the step before: S came after)
+                    float f = 1.0f;
+                    if (ref == kNegInf) {
+                        ref = mx;
+                    } else if ((mx - ref) * unit > kLag) {
+                        f = exp2_fast((ref - mx) * unit);
+                        ref = mx;
+                    }
+                    if (__any_sync(kFull, f != 1.0f)) {
+                        l2 = fma_two(l2, pair(f, f), 0);
+                        if (c < 3) {  // the next scores' registers are in use
+                            tensor_wait_load();
+                            tensor_ready(v[(c + 1) & 1]);
+                        }
+                        if (c > 0) tensor_wait_store();
+                        for (int k = 0; k < c; ++k) scale_weights(s_at + 16 * k, f);
+                        if (j > from)
+                            for (int k = 0; k < D / 16; ++k) scale_output(o_at + 16 * k, f);
+                    }
+                    const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
+                    const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
+                    uint32_t w[16];
+                    uint64_t sum = 0;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const uint64_t y = fma_two(pair(x[i], x[i + 1]), unit2, minus_base2);
+                        const float a = exp2_fast(first_of(y)), b = exp2_fast(second_of(y));
+                        sum = add_two(sum, pair(a, b));
+                        w[i / 2] = as_word(__floats2half2_rn(a, b));
+                    }
+                    l2 = add_two(l2, sum);
+                    // P takes the columns of S that have been read
+                    tensor_store16(s_at + 16 * c, w);
                 }
+                tensor_wait_store();
+                fence_before();
+                barrier_arrive(p_full + 8 * tile);
             }
-            const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
-            const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                tensor_load(s_at + 64 * c, v);
-                tensor_load(s_at + 64 * c + 32, v + 32);
-                tensor_wait_load();
-                tensor_ready(v);
-                tensor_ready(v + 32);
-                uint32_t w[32];
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < 64; i += 2) {
-                    const uint64_t x = fma_two(pair(v[i], v[i + 1]), unit2, minus_base2);
-                    const float a = exp2_fast(first_of(x)), b = exp2_fast(second_of(x));
-                    sum[(i >> 1) & 1] = add_two(sum[(i >> 1) & 1], pair(a, b));
-                    w[i / 2] = as_word(__floats2half2_rn(a, b));
-                }
-                l2 = add_two(l2, add_two(sum[0], sum[1]));
-                // P takes the columns of S that have been read
-                tensor_store(s_at + 32 * c, w);
-            }
-            tensor_wait_store();
-            fence_before();
-            barrier_arrive(p_full + 8 * tile);
-        }
-        // ---- the output of this thread's column
-        if (ok && steps > 0) {
-            ok = wait(o_done + 8 * tile, steps - 1);
+            // ---- the output of this thread's column, or its partial result
+            ok = ok && wait(o_done, items);
+            if (!ok) break;
+            ++items;
             fence_after();
-        }
-        if (ok) {
             const float l = first_of(l2) + second_of(l2), inv = l > 0.0f ? 1.0f / l : 0.0f;
-            uint16_t* out = static_cast<uint16_t*>(p.out) + out_row * D;
-#pragma unroll
+            const float at = l > 0.0f ? fmaf(ref, unit, -kHead) : kNegInf;
+            const uint64_t out_row = output_row(p, group, it.first_row, it.head, at_col);
+            const bool whole = it.from == 0 && it.to == it.steps;
+            float* part = parts + (2ull * blockIdx.x + (it.flat == u0 ? 0 : 1)) * kRowPartFloats<D>;
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 float o[32];
-                if (steps > 0) {
-                    tensor_load(o_at + 32 * c, o);
-                    tensor_wait_load();
-                    tensor_ready(o);
-                }
-                if (on) {
+                tensor_load(o_at + 32 * c, o);
+                tensor_wait_load();
+                tensor_ready(o);
+                if (!on) continue;
+                if (whole) {
+                    uint16_t* out = static_cast<uint16_t*>(p.out) + out_row * D + 32 * c;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         uint2 w = make_uint2(0u, 0u);
                         if (l > 0.0f)
                             w = make_uint2(kv_pack2(o[i] * inv, o[i + 1] * inv, p.dtype),
                                            kv_pack2(o[i + 2] * inv, o[i + 3] * inv, p.dtype));
-                        *reinterpret_cast<uint2*>(out + 32 * c + i) = w;
+                        *reinterpret_cast<uint2*>(out + i) = w;
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * kWidth + col] = o[i];
                 }
             }
-            if (on && p.lse)
-                p.lse[out_row] = l > 0.0f ? (fmaf(ref, unit, -kHead) + log2f(l)) * kLn2 : kNegInf;
+            if (on && whole && p.lse) p.lse[out_row] = l > 0.0f ? (at + log2f(l)) * kLn2 : kNegInf;
+            if (on && !whole) {
+                part[col] = at;
+                part[kWidth + col] = l;
+            }
             fence_before();
-        }
+        } while (advance());
     }
 
     // every product has completed (or its wait has run out) before the tensor
@@ -637,32 +849,112 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     }
 }
 
+// Items that several blocks share: their partial results in block order, so
+// that the sum does not depend on which block was done first.  Eight blocks an
+// item, 32 columns each.
+constexpr int kJoinColumns = 32, kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_rows_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
+                                                                    gofann_kv_attention_params p, uint32_t blocks,
+                                                                    const float* __restrict__ parts)
+{
+    __shared__ float turn[kJoinColumns][D + 1];
+    const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
+    const uint32_t n_kv = cache.n_kv_heads;
+    const uint64_t total = locate(batch, p, n_kv, group, ~0ull).total;
+    const uint64_t share = steps_per_block(total, blocks);
+    // block i joins the item that the end of share i cuts, if that is the item's first cut
+    const uint64_t cut = share * (blockIdx.y + 1);
+    if (cut >= total) return;
+    const Place at = locate(batch, p, n_kv, group, cut);
+    Item it{};
+    it.seq = at.seq, it.head = at.head, it.tile = at.tile, it.flat = cut, it.limit = ~0ull;
+    open_item(batch, p, group, at.step, it);
+    const uint64_t begin = cut - at.step, end = begin + it.steps;
+    if (begin >= cut || begin < share * blockIdx.y) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = static_cast<int>(blockIdx.x) * kJoinColumns;
+    if (c0 >= it.cols) return;
+    wait_previous();
+    const uint64_t last = (end - 1) / share;
+    constexpr int kEach = D / (kJoinThreads / 32);
+    float m = kNegInf, l = 0.0f, o[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) o[k] = 0.0f;
+    if (c0 + lane < it.cols) {
+        for (uint64_t b = blockIdx.y; b <= last; ++b) {
+            const float* part = parts + (2 * b + (begin <= share * b ? 0 : 1)) * kRowPartFloats<D> + c0 + lane;
+            const float pm = __ldcg(part), pl = __ldcg(part + kWidth);
+            const float top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
+            const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
+            l = l * f + pl * h;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) o[k] = o[k] * f + __ldcg(part + (2 + warp * kEach + k) * kWidth) * h;
+            m = top;
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) turn[lane][warp * kEach + k] = l > 0.0f ? o[k] * inv : 0.0f;
+    if (warp == 0 && p.lse && c0 + lane < it.cols)
+        p.lse[output_row(p, group, it.first_row, it.head, it.col0 + c0 + lane)] = l > 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kJoinColumns * (D / 2); i += kJoinThreads) {
+        const int c = i / (D / 2), d = i % (D / 2) * 2;
+        if (c0 + c >= it.cols) break;
+        const uint64_t row = output_row(p, group, it.first_row, it.head, it.col0 + c0 + c);
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * D + d) =
+            kv_pack2(turn[c][d], turn[c][d + 1], p.dtype);
+    }
+}
+
+// One thread block per SM, no more than there can be items of one step.
+uint32_t row_blocks(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
+{
+    const uint64_t cols = static_cast<uint64_t>(batch.n_rows) * (p.n_heads / cache.n_kv_heads);
+    const uint64_t most = (cols / kWidth + batch.n_seqs) * cache.n_kv_heads * (batch.max_pages / 2 + 1ull);
+    const int sms = sm_count();
+    const uint64_t want = sms > 0 ? sms : 1;
+    return static_cast<uint32_t>(most < want ? most : want);
+}
+
 template <int D>
 int launch_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                cudaStream_t s)
+                float* parts, cudaStream_t s)
 {
-    const uint64_t group = p.n_heads / cache.n_kv_heads, width = kTiles * kTileRows;
-    // a sequence of n rows has at most n group / width + 1 tiles, and at most one per column
-    const uint64_t cols = static_cast<uint64_t>(batch.n_rows) * group;
-    uint64_t tiles = cols / width + batch.n_seqs;
-    if (tiles > cols) tiles = cols;
-    if (tiles > 0x7fffffffull)
-        return fail(GOFANN_ERR_UNSUPPORTED, "kv_attention: %llu tiles (at most 2^31 - 1)", static_cast<unsigned long long>(tiles));
     auto* kernel = kv_attend_rows_kernel<D>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<D>::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<D>::kBytes);
     if (e != cudaSuccess) return cuda_status(e, "kv_attention: shared memory attribute");
     const bool wide = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && (p.q_stride & 3) == 0;
-    kernel<<<dim3(static_cast<uint32_t>(tiles), cache.n_kv_heads), kRowThreads, Rows<D>::kBytes, s>>>(cache, batch, p, wide);
+    const uint32_t blocks = row_blocks(cache, batch, p);
+    kernel<<<blocks, kRowThreads, Rows<D>::kBytes, s>>>(cache, batch, p, wide, parts);
     GOFANN_CHECK_LAUNCH("kv_attend_rows_kernel");
+    if (blocks == 1) return GOFANN_OK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kWidth / kJoinColumns, blocks - 1);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kv_join_rows_kernel<D>, cache, batch, p, blocks, static_cast<const float*>(parts));
+    if (e != cudaSuccess) return cuda_status(e, "kv_join_rows_kernel");
     return GOFANN_OK;
 }
 
 }  // namespace
 
-int attend_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                cudaStream_t s)
+size_t attend_rows_scratch(uint32_t head_dim, int sms)
 {
-    return cache.head_dim == 64 ? launch_rows<64>(cache, batch, p, s) : launch_rows<128>(cache, batch, p, s);
+    return 2 * sizeof(float) * (head_dim == 64 ? kRowPartFloats<64> : kRowPartFloats<128>) * static_cast<size_t>(sms);
+}
+
+int attend_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
+                float* parts, cudaStream_t s)
+{
+    return cache.head_dim == 64 ? launch_rows<64>(cache, batch, p, parts, s)
+                                : launch_rows<128>(cache, batch, p, parts, s);
 }
 
 }  // namespace gofann
