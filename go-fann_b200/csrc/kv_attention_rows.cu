@@ -52,7 +52,7 @@ struct Rows {
     static constexpr int kOffRaw = kOffV + 2 * kValues;
     static constexpr int kOffShown = kOffRaw + kRaw * kChunk;       // u64 [kRaw] of the ring, [4][2] of the steps
     static constexpr int kOffBars = kOffShown + 8 * (kRaw + 8);
-    static constexpr int kBars = 2 * kRaw + 8 + 2 * kTiles + 2;
+    static constexpr int kBars = 2 * kRaw + 8 + 4 * kTiles + 2;
     static constexpr int kBytes = 1024 + kOffBars + 8 * kBars + 16;
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
     // tensor memory columns
@@ -178,6 +178,14 @@ __device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b)
     return d;
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on != 0;
+}
+
 // ------------------------------------------------------------------ decoding
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
@@ -274,6 +282,33 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
             }
         }
     }
+}
+
+// Weights 2^(unit x - base) of 32 scores as f16 pairs and their sum (two
+// parts); returns the largest score.
+__device__ __forceinline__ float weigh(const float (&x)[32], float ref, float unit, uint32_t (&w)[16], uint64_t& sum)
+{
+    const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
+    const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
+    float m4[4] = {x[0], x[1], x[2], x[3]};
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        const uint64_t y = fma_two(pair(x[i], x[i + 1]), unit2, minus_base2);
+        const uint64_t z = fma_two(pair(x[i + 2], x[i + 3]), unit2, minus_base2);
+        const float a = exp2_fast(first_of(y)), b = exp2_fast(second_of(y));
+        const float c = exp2_fast(first_of(z)), d = exp2_fast(second_of(z));
+        if (i > 0) {
+            m4[0] = fmaxf(m4[0], x[i]);
+            m4[1] = fmaxf(m4[1], x[i + 1]);
+            m4[2] = fmaxf(m4[2], x[i + 2]);
+            m4[3] = fmaxf(m4[3], x[i + 3]);
+        }
+        sum = add_two(sum, add_two(pair(a, b), pair(c, d)));
+        w[i / 2] = as_word(__floats2half2_rn(a, b));
+        w[i / 2 + 1] = as_word(__floats2half2_rn(c, d));
+    }
+    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
 }
 
 // 16 columns times f: f32 numbers of the output, or pairs of f16 weights.
@@ -448,8 +483,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     const uint32_t bars = shared_addr(smem + Cfg::kOffBars);
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * kRaw;
     const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
-    const uint32_t s_full = v_empty + 16, p_full = s_full + 8 * kTiles, o_done = p_full + 8 * kTiles;
-    const uint32_t q_full = o_done + 8;
+    // [tile][half] of S and P
+    const uint32_t s_full = v_empty + 16, p_full = s_full + 16 * kTiles, q_full = p_full + 16 * kTiles;
+    const uint32_t all_done = q_full + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffBars + 8 * Cfg::kBars);
     volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a wait has run out
 
@@ -483,12 +519,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             barrier_init(v_full + 8 * i, kTasks);
             barrier_init(v_empty + 8 * i, 1);
         }
-        for (int i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < 2 * kTiles; ++i) {
             barrier_init(s_full + 8 * i, 1);
             barrier_init(p_full + 8 * i, kTileRows);
         }
-        barrier_init(o_done, 1);
         barrier_init(q_full, kTiles * kTileRows);
+        barrier_init(all_done, 1);
         barrier_fence();
         *dead = 0;
     }
@@ -557,60 +593,78 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         for (uint32_t k = i > kRaw ? i - kRaw : 0; k < i; ++k)
             if (!barrier_wait(raw_full + 8 * (k % kRaw), (k / kRaw) & 1)) *dead = 1;
     } else if (warp == kMmaWarp) {
-        // ---- products, issued by one thread; the tensor cores take them in
-        // order, so a tile's next S may be issued behind the product that
-        // still reads its P, and a commit behind S also stands for that product
-        if (lane == 0) {
-            Item it = start;
-            const uint32_t base = shared_addr(smem);
-            const auto scores = [&](int tile, uint32_t g) {
-                const uint32_t q = base + tile * Cfg::kQTile, k = base + Cfg::kOffK + (g & 1) * Cfg::kKeys;
+        // ---- products, issued by one thread, page by page of a step: S of a
+        // tile's page of the next step goes behind the product that reads this
+        // step's P.  The tensor cores take one thread's products in order, so
+        // S may be written where P was, and a commit behind S also stands for
+        // the product before it.  At an item's end a commit without S does.
+        // The whole warp runs this code and one elected lane issues: descriptors
+        // are then warp-uniform values, which the instruction takes them as.
+        Item it = start;
+        const uint32_t base = shared_addr(smem);
+        const uint64_t q_desc = operand_desc(base);
+        const auto scores = [&](int tile, int h, uint32_t stage) {
+            const uint64_t q = q_desc + tile * (Cfg::kQTile >> 4);
+            const uint64_t k = q_desc + ((Cfg::kOffK + h * (kKvPage * 128)) >> 4) + stage * (Cfg::kKeys >> 4);
+            if (elect_one()) {
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
-                    mma_shared(tmem + Cfg::kScores + tile * kStepKeys,
-                               operand_desc(q + (i / 4) * (kTileRows * 128) + (i % 4) * 32),
-                               operand_desc(k + (i / 4) * (kStepKeys * 128) + (i % 4) * 32), mma_shape(kTileRows, kStepKeys),
-                               i > 0);
-                mma_commit(s_full + 8 * tile);
-                if (tile == kTiles - 1) mma_commit(k_empty + 8 * (g & 1));
-            };
-            uint32_t g = 0, items = 0;  // steps and items so far
-            bool ok = true;
-            do {
-                ok = wait(q_full, items) && wait(k_full + 8 * (g & 1), g >> 1);
-                if (!ok) break;
-                fence_after();
-                for (int tile = 0; tile < kTiles; ++tile) scores(tile, g);
-                for (int j = it.from; j < it.to && ok; ++j, ++g) {
-                    for (int tile = 0; tile < kTiles; ++tile) {
-                        ok = (tile > 0 || wait(v_full + 8 * (g & 1), g >> 1)) && wait(p_full + 8 * tile, g);
-                        if (!ok) break;
-                        fence_after();
-                        const uint32_t v = base + Cfg::kOffV + (g & 1) * Cfg::kValues;
+                    mma_shared(tmem + Cfg::kScores + tile * kStepKeys + h * kKvPage,
+                               q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4),
+                               k + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kKvPage), i > 0);
+                mma_commit(s_full + 16 * tile + 8 * h);
+                if (tile == kTiles - 1 && h == 1) mma_commit(k_empty + 8 * stage);
+            }
+        };
+        const auto output = [&](int tile, int h, uint32_t stage, uint32_t add) {
+            const uint64_t v = q_desc + ((Cfg::kOffV + h * (D * 128)) >> 4) + stage * (Cfg::kValues >> 4);
+            if (elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < kStepKeys / 16; ++i)
-                            mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + 8 * i,
-                                       operand_desc(v + (i / 4) * (D * 128) + (i % 4) * 32), mma_shape(kTileRows, D),
-                                       j > it.from || i > 0);
-                        if (tile == kTiles - 1) mma_commit(v_empty + 8 * (g & 1));
-                        if (j + 1 < it.to) {
-                            if (tile == 0) {
-                                ok = wait(k_full + 8 * ((g + 1) & 1), (g + 1) >> 1);
-                                if (!ok) break;
-                                fence_after();
-                            }
-                            scores(tile, g + 1);
+                for (int k = 0; k < kKvPage / 16; ++k)
+                    mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + h * kKvPage + 8 * k,
+                               v + (k * 32 >> 4), mma_shape(kTileRows, D), k > 0 ? 1u : add);
+                if (tile == kTiles - 1 && h == 1) mma_commit(v_empty + 8 * stage);
+            }
+        };
+        const auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(kFull, wait(bar, parity)) != 0; };
+        uint32_t g = 0, items = 0;  // steps and items so far
+        bool ok = true;
+        do {
+            const int steps = __shfl_sync(kFull, it.to - it.from, 0);
+            ok = all_wait(q_full, items) && all_wait(k_full + 8 * (g & 1), g >> 1);
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int i = 0; i < 2 * kTiles; ++i) scores(i % kTiles, i / kTiles, g & 1);
+            for (int j = 0; j < steps && ok; ++j, ++g) {
+                const uint32_t st = g & 1, next = st ^ 1;
+                const bool more = j + 1 < steps;
+                ok = all_wait(v_full + 8 * st, g >> 1);
+#pragma unroll
+                for (int i = 0; i < 2 * kTiles; ++i) {
+                    const int tile = i % kTiles, h = i / kTiles;
+                    ok = ok && all_wait(p_full + 16 * tile + 8 * h, g);
+                    if (!ok) break;
+                    fence_after();
+                    output(tile, h, st, j > 0 || h > 0);
+                    if (more) {
+                        if (i == 0) {
+                            ok = all_wait(k_full + 8 * next, (g + 1) >> 1);
+                            if (!ok) break;
+                            fence_after();
                         }
+                        scores(tile, h, next);
+                    } else if (elect_one()) {
+                        mma_commit(s_full + 16 * tile + 8 * h);
                     }
                 }
-                if (ok) mma_commit(o_done);
-                ++items;
-            } while (ok && next_item(batch, p, n_kv, group, it));
-            // nothing that was issued may outlive the block: the last commit
-            // stands for all of it
-            if (!ok) mma_commit(o_done);
-            if (!barrier_wait(o_done, (ok ? items - 1 : items) & 1)) *dead = 1;
-        }
+            }
+            ++items;
+        } while (ok && next_item(batch, p, n_kv, group, it));
+        // nothing that was issued may outlive the block: a last commit stands
+        // for all of it
+        if (elect_one()) mma_commit(all_done);
+        if (!barrier_wait(all_done, 0)) *dead = 1;
         __syncwarp();
     } else if (warp >= kSoftmaxWarps) {
         // ---- codes to f16 operands
@@ -670,7 +724,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             __syncwarp();
             return more;
         };
-        uint32_t g = 0, items = 0;
+        uint32_t g = 0, sg = 0;  // steps, and commits of a page's S, so far
         bool ok = true;
         do {
             const bool on = col < it.cols;
@@ -715,93 +769,86 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             uint64_t l2 = 0;  // two parts of the sum of weights
             const int from = it.from, to = it.to;
             int key0 = (it.lo + 2 * from) * kKvPage;
-            for (int j = from; j < to; ++j, ++g, key0 += kStepKeys) {
-                ok = wait(s_full + 8 * tile, g);
-                if (!ok) break;
-                fence_after();
-                const uint64_t shown[2] = {step_shown[(g & 3) * 2], step_shown[(g & 3) * 2 + 1]};
-                const bool masked = (shown[0] & shown[1]) != ~0ull || key0 + kStepKeys - 1 > warp_limit || key0 <= warp_low;
-                if (masked) {
-                    // hidden tokens' scores become -inf in place; the rest of
-                    // the step then knows no mask
+            for (int j = from; j < to && ok; ++j, ++g, ++sg) {
+                for (int h = 0; h < 2; ++h, key0 += kKvPage) {
+                    ok = wait(s_full + 16 * tile + 8 * h, sg);
+                    if (!ok) break;
+                    fence_after();
+                    const uint32_t sh = s_at + h * kKvPage;
+                    const uint64_t shown = step_shown[(g & 3) * 2 + h];
+                    if (shown != ~0ull || key0 + kKvPage - 1 > warp_limit || key0 <= warp_low) {
+                        // hidden tokens' scores become -inf in place; the rest
+                        // of the page's work then knows no mask
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        const int a = limit - (key0 + 32 * c), b = low - (key0 + 32 * c);
-                        uint32_t see = static_cast<uint32_t>(shown[c >> 1] >> (32 * (c & 1)));
-                        see &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
-                        see &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
-                        float v[32];
-                        tensor_load(s_at + 32 * c, v);
-                        tensor_wait_load();
-                        tensor_ready(v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!((see >> i) & 1)) v[i] = kNegInf;
-                        tensor_store(s_at + 32 * c, reinterpret_cast<const uint32_t*>(v));
-                    }
-                    tensor_wait_store();
-                }
-                // 32 tokens at a time, the next ones on their way
-                float v[2][32];
-                tensor_load(s_at, v[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float(&x)[32] = v[c & 1];
-                    tensor_wait_load();
-                    tensor_ready(x);
-                    if (c < 3) tensor_load(s_at + 32 * (c + 1), v[(c + 1) & 1]);
-                    float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                    for (int i = 4; i < 28; i += 8)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], x[i + k]), x[i + 4 + k]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[28 + k]);
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    // the reference follows the maximum where that is far
-                    // ahead; what was weighed by the old one is rescaled (the
-                    // output is complete up to the step before: S came after)
-                    float f = 1.0f;
-                    if (ref == kNegInf) {
-                        ref = mx;
-                    } else if ((mx - ref) * unit > kLag) {
-                        f = exp2_fast((ref - mx) * unit);
-                        ref = mx;
-                    }
-                    if (__any_sync(kFull, f != 1.0f)) {
-                        l2 = fma_two(l2, pair(f, f), 0);
-                        if (c < 3) {  // the next scores' registers are in use
+                        for (int c = 0; c < 2; ++c) {
+                            const int a = limit - (key0 + 32 * c), b = low - (key0 + 32 * c);
+                            uint32_t see = static_cast<uint32_t>(shown >> (32 * c));
+                            see &= a < 0 ? 0u : a >= 31 ? ~0u : (2u << a) - 1u;
+                            see &= b < 0 ? ~0u : b >= 31 ? 0u : ~((2u << b) - 1u);
+                            float v[32];
+                            tensor_load(sh + 32 * c, v);
                             tensor_wait_load();
-                            tensor_ready(v[(c + 1) & 1]);
-                        }
-                        if (c > 0) tensor_wait_store();
-                        for (int k = 0; k < c; ++k) scale_weights(s_at + 16 * k, f);
-                        if (j > from)
-                            for (int k = 0; k < D / 16; ++k) scale_output(o_at + 16 * k, f);
-                    }
-                    const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
-                    const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
-                    uint32_t w[16];
-                    uint64_t sum = 0;
+                            tensor_ready(v);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const uint64_t y = fma_two(pair(x[i], x[i + 1]), unit2, minus_base2);
-                        const float a = exp2_fast(first_of(y)), b = exp2_fast(second_of(y));
-                        sum = add_two(sum, pair(a, b));
-                        w[i / 2] = as_word(__floats2half2_rn(a, b));
+                            for (int i = 0; i < 32; ++i)
+                                if (!((see >> i) & 1)) v[i] = kNegInf;
+                            tensor_store(sh + 32 * c, reinterpret_cast<const uint32_t*>(v));
+                        }
+                        tensor_wait_store();
                     }
-                    l2 = add_two(l2, sum);
-                    // P takes the columns of S that have been read
-                    tensor_store16(s_at + 16 * c, w);
+                    // 32 tokens at a time, the next ones on their way
+                    float v[2][32];
+                    tensor_load(sh, v[0]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float(&x)[32] = v[c];
+                        tensor_wait_load();
+                        tensor_ready(x);
+                        if (c == 0) tensor_load(sh + 32, v[1]);
+                        // weights by the reference so far, the maximum next to them
+                        uint32_t w[16];
+                        uint64_t sum;
+                        float mx = weigh(x, ref, unit, w, sum);
+                        const bool far = (mx - ref) * unit > kLag;  // also where there was no reference
+                        if (__any_sync(kFull, far)) {
+                            // the reference follows the maximum; what was
+                            // weighed by the old one is rescaled
+                            float f = 1.0f;
+                            if (far) {
+                                f = ref == kNegInf ? 1.0f : exp2_fast((ref - mx) * unit);
+                                ref = mx;
+                            }
+                            l2 = fma_two(l2, pair(f, f), 0);
+                            if (c == 0) {
+                                tensor_wait_load();
+                                tensor_ready(v[1]);
+                            } else {
+                                tensor_wait_store();
+                                scale_weights(sh, f);
+                            }
+                            if (j > from || h > 0) {
+                                // behind the product of the page before
+                                ok = wait(s_full + 16 * tile + 8 * (h ^ 1), sg + h);
+                                fence_after();
+                                if (ok)
+                                    for (int k = 0; k < D / 16; ++k) scale_output(o_at + 16 * k, f);
+                            }
+                            weigh(x, ref, unit, w, sum);
+                        }
+                        l2 = add_two(l2, sum);
+                        // P takes the columns of S that have been read
+                        tensor_store16(sh + 16 * c, w);
+                    }
+                    if (!ok) break;
+                    tensor_wait_store();
+                    fence_before();
+                    barrier_arrive(p_full + 16 * tile + 8 * h);
                 }
-                tensor_wait_store();
-                fence_before();
-                barrier_arrive(p_full + 8 * tile);
             }
             // ---- the output of this thread's column, or its partial result
-            ok = ok && wait(o_done, items);
+            ok = ok && wait(s_full + 16 * tile, sg) && wait(s_full + 16 * tile + 8, sg);
             if (!ok) break;
-            ++items;
+            ++sg;
             fence_after();
             const float l = first_of(l2) + second_of(l2), inv = l > 0.0f ? 1.0f / l : 0.0f;
             const float at = l > 0.0f ? fmaf(ref, unit, -kHead) : kNegInf;
@@ -839,8 +886,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         } while (advance());
     }
 
-    // every product has completed (or its wait has run out) before the tensor
-    // memory goes back
     __syncthreads();
     if (threadIdx.x == 0 && *dead) kv_timeout(batch);
     if (warp == kMmaWarp) {
