@@ -6,7 +6,7 @@
 // one key/value head) at a time and walks their blocks of the cache, two pages
 // (128 tokens) a step:
 // * a loader copies packed chunks to a shared ring (bulk copies);
-// * six warps turn codes into f16 keys [token][dim] and transposed values
+// * eight warps turn codes into f16 keys [token][dim] and transposed values
 //   [dim][token], both 128-byte swizzled and K-major, each page once for all
 //   256 columns;
 // * one thread issues S = Q K^T (tcgen05.mma, M = 128, N = 128) and
@@ -32,11 +32,14 @@ namespace {
 
 constexpr int kTileRows = 128, kTiles = 2;
 constexpr int kStepKeys = 2 * kKvPage;
-// 16 warps have 128 registers a thread.  The six that decode share a step's
-// 16 tasks: the keys and the values of two pages, in quarters.
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 6, kTasks = 8;
+// Eight warps decode: a quarter of the keys and of the values of one of a
+// step's two pages each.
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
-constexpr int kRowThreads = 32 * (kLoadWarp + 1);
+constexpr int kRowThreads = 32 * (kLoadWarp + 3);  // whole warpgroups
+// Registers a thread: 96 at launch for 640 threads, 61440 in all; the split
+// below takes 256 x 120 + 256 x 80 + 128 x 56 = 58368.
+constexpr int kSoftmaxRegs = 120, kDecodeRegs = 80, kOtherRegs = 56;
 constexpr float kLag = 8.0f;   // log2 that a column's maximum may run ahead of its reference
 constexpr float kHead = 7.0f;  // log2 of a weight at the reference
 
@@ -45,13 +48,13 @@ struct Rows {
     static constexpr int kQTile = kTileRows * D * 2;
     static constexpr int kKeys = kStepKeys * D * 2;                 // [panel][128 tokens][64 dims]
     static constexpr int kValues = kStepKeys * D * 2;               // [page][D dims][64 tokens]
-    static constexpr int kChunk = KvChunk<D>::kBytes;
-    static constexpr int kRaw = D == 64 ? 6 : 3;
+    static constexpr int kHalf = KvChunk<D>::kBytes / 2;            // keys or values of a page
+    static constexpr int kRaw = D == 64 ? 12 : 6;
     static constexpr int kOffK = kTiles * kQTile;
     static constexpr int kOffV = kOffK + 2 * kKeys;
     static constexpr int kOffRaw = kOffV + 2 * kValues;
-    static constexpr int kOffShown = kOffRaw + kRaw * kChunk;       // u64 [kRaw] of the ring, [4][2] of the steps
-    static constexpr int kOffBars = kOffShown + 8 * (kRaw + 8);
+    static constexpr int kOffShown = kOffRaw + kRaw * kHalf;        // u64 [8 steps][2 pages]
+    static constexpr int kOffBars = kOffShown + 8 * 16;
     static constexpr int kBars = 2 * kRaw + 8 + 4 * kTiles + 2;
     static constexpr int kBytes = 1024 + kOffBars + 8 * kBars + 16;
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
@@ -198,14 +201,14 @@ __device__ __forceinline__ void code_pairs(uint32_t w, __half2& low, __half2& hi
     high = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, back);  // / 16 - 64
 }
 
-// Keys of one page: this warp's quarter (16 tokens) as rows of 64 dimensions.
+// Keys of one page from the key half of its chunk: this warp's quarter (16 tokens) as rows of 64 dimensions.
 template <int D>
 __device__ __forceinline__ void decode_keys(const unsigned char* chunk, unsigned char* keys, int page, int warp)
 {
     constexpr int G = KvChunk<D>::kGroups;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, kt = warp;
     const int token0 = 16 * (g >> 1) + 4 * kt + (g & 1);
-    const uint32_t* params = reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kKeyParams) + (g * 4 + kt) * 2 * G;
+    const uint32_t* params = reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kCodes) + (g * 4 + kt) * 2 * G;
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
         const uint4 w4 = reinterpret_cast<const uint4*>(chunk)[(kt * G + grp) * 32 + lane];
@@ -230,7 +233,7 @@ __device__ __forceinline__ void decode_keys(const unsigned char* chunk, unsigned
     }
 }
 
-// Values of one page, transposed: this warp's 16-dimension tiles as rows of 64
+// Values of one page from the value half, transposed: this warp's 16-dimension tiles as rows of 64
 // tokens.  A hidden token's value is 0 whatever the page holds there.
 template <int D>
 __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsigned char* values, int warp, uint64_t shown)
@@ -240,7 +243,7 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
     // scales and minima of this lane's 16 tokens 16 t .. 16 t + 15, in pairs
     __half2 s[G][8], m[G][8];
     {
-        const uint4* params = reinterpret_cast<const uint4*>(chunk + KvChunk<D>::kValueParams) + t * 4 * G;
+        const uint4* params = reinterpret_cast<const uint4*>(chunk + KvChunk<D>::kCodes) + t * 4 * G;
 #pragma unroll
         for (int q = 0; q < 2 * G; ++q) {
             const uint4 a4 = params[q], b4 = params[2 * G + q];  // even, odd tokens
@@ -262,7 +265,7 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
     for (int grp = 0; grp < G; ++grp) {
         {
             const int i = 4 * grp + warp;
-            const uint4 w4 = reinterpret_cast<const uint4*>(chunk + KvChunk<D>::kValueCodes)[i * 32 + lane];
+            const uint4 w4 = reinterpret_cast<const uint4*>(chunk)[i * 32 + lane];
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -478,8 +481,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     __shared__ Item start, warp_items[kSoftmaxWarps];  // of the softmax warps, to spare registers
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t* raw_shown = reinterpret_cast<uint64_t*>(smem + Cfg::kOffShown);  // [kRaw]
-    uint64_t* step_shown = raw_shown + kRaw;                                   // [4][2]
+    uint64_t* step_shown = reinterpret_cast<uint64_t*>(smem + Cfg::kOffShown);  // [step & 7][page]
     const uint32_t bars = shared_addr(smem + Cfg::kOffBars);
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * kRaw;
     const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
@@ -511,12 +513,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     if (warp == 1 && lane == 0) {
         for (int i = 0; i < kRaw; ++i) {
             barrier_init(raw_full + 8 * i, 1);
-            barrier_init(raw_empty + 8 * i, kTasks);  // four of keys, four of values
+            barrier_init(raw_empty + 8 * i, kDecodeWarps / 2);
         }
         for (int i = 0; i < 2; ++i) {
-            barrier_init(k_full + 8 * i, kTasks);
+            barrier_init(k_full + 8 * i, kDecodeWarps);
             barrier_init(k_empty + 8 * i, 1);
-            barrier_init(v_full + 8 * i, kTasks);
+            barrier_init(v_full + 8 * i, kDecodeWarps);
             barrier_init(v_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2 * kTiles; ++i) {
@@ -547,21 +549,23 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         *dead = 1;
         return false;
     };
+    if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kLoadWarp) {
+        // ---- loader: a step's keys of both pages, then their values; page
+        // numbers are looked up 32 blocks at a time
         Item it = start;
-        // ---- loader: page numbers are looked up 32 blocks at a time
-        uint32_t i = 0;  // pages so far
+        uint32_t i = 0, g = 0;  // halves and steps so far
         bool ok = true;
         do {
             int page = -1;
             uint64_t shown = 0;
-            const int block0 = it.lo + 2 * it.from, n = 2 * (it.to - it.from);
-            for (int k = 0; k < n; ++k, ++i) {
-                if ((k & 31) == 0) {
-                    const int block = block0 + k + lane;
+            const int n = it.to - it.from;
+            for (int j = 0; j < n && ok; ++j, ++g) {
+                if ((j & 15) == 0) {
+                    const int block = it.lo + 2 * (it.from + j) + lane;
                     page = -1;
                     shown = 0;
-                    if (block < it.hi && k + lane < n) {
+                    if (block < it.hi && 2 * j + lane < 2 * n) {
                         page = __ldg(batch.page_table + static_cast<size_t>(it.seq) * batch.max_pages + block);
                         if (page < 0 || static_cast<uint32_t>(page) >= cache.n_pages) {
                             page = -1;
@@ -571,20 +575,22 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                         }
                     }
                 }
-                const uint32_t slot = i % kRaw;
-                const int from = __shfl_sync(kFull, page, k & 31);
-                const uint64_t bits = __shfl_sync(kFull, shown, k & 31);
-                ok = i < kRaw || wait(raw_empty + 8 * slot, i / kRaw - 1);
-                if (!ok) break;
-                if (lane == 0) {
-                    raw_shown[slot] = bits;
-                    if (from >= 0) {
-                        barrier_expect(raw_full + 8 * slot, Cfg::kChunk);
-                        bulk_load(shared_addr(smem + Cfg::kOffRaw + slot * Cfg::kChunk),
-                                  cache.pages + (static_cast<size_t>(from) * n_kv + it.head) * Cfg::kChunk, Cfg::kChunk,
-                                  raw_full + 8 * slot);
-                    } else {
-                        barrier_arrive(raw_full + 8 * slot);
+                for (int k = 0; k < 4; ++k, ++i) {
+                    const uint32_t slot = i % kRaw;
+                    const int from = __shfl_sync(kFull, page, (2 * j + (k & 1)) & 31);
+                    const uint64_t bits = __shfl_sync(kFull, shown, (2 * j + (k & 1)) & 31);
+                    ok = i < kRaw || wait(raw_empty + 8 * slot, i / kRaw - 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        if (k < 2) step_shown[(g & 7) * 2 + k] = bits;
+                        if (from >= 0) {
+                            barrier_expect(raw_full + 8 * slot, Cfg::kHalf);
+                            bulk_load(shared_addr(smem + Cfg::kOffRaw + slot * Cfg::kHalf),
+                                      cache.pages + ((static_cast<size_t>(from) * n_kv + it.head) * 2 + (k >> 1)) * Cfg::kHalf,
+                                      Cfg::kHalf, raw_full + 8 * slot);
+                        } else {
+                            barrier_arrive(raw_full + 8 * slot);
+                        }
                     }
                 }
             }
@@ -666,50 +672,40 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         if (elect_one()) mma_commit(all_done);
         if (!barrier_wait(all_done, 0)) *dead = 1;
         __syncwarp();
-    } else if (warp >= kSoftmaxWarps) {
+    } else if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
         // ---- codes to f16 operands
-        const int w = warp - kSoftmaxWarps;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegs));
+        const int page = (warp - kSoftmaxWarps) >> 2, quarter = warp & 3;
         Item it = start;
         uint32_t g = 0;
         bool ok = true;
         do {
-            for (int j = it.from; j < it.to && ok; ++j, ++g) {
-                const uint32_t st = g & 1;
-                ok = g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1);
-                for (int task = w; task < kTasks && ok; task += kDecodeWarps) {
-                    const int page = task >> 2, quarter = task & 3;
-                    const uint32_t i = 2 * g + page, slot = i % kRaw;
-                    ok = wait(raw_full + 8 * slot, i / kRaw);
-                    if (!ok) break;
-                    decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
-                    if (quarter == 0 && lane == 0) step_shown[(g & 3) * 2 + page] = raw_shown[slot];
-                    fence_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        barrier_arrive(raw_empty + 8 * slot);
-                        barrier_arrive(k_full + 8 * st);
-                    }
+            for (int j = it.from; j < it.to; ++j, ++g) {
+                const uint32_t st = g & 1, i = 4 * g + page, slot = i % kRaw, slot2 = (i + 2) % kRaw;
+                ok = wait(raw_full + 8 * slot, i / kRaw) && (g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1));
+                if (!ok) break;
+                decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
+                fence_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    barrier_arrive(k_full + 8 * st);
+                    barrier_arrive(raw_empty + 8 * slot);
                 }
-                ok = ok && (g < 2 || wait(v_empty + 8 * st, (g >> 1) - 1));
-                // from the other end, so that the warps with two tasks differ
-                for (int task = kDecodeWarps - 1 - w; task < kTasks && ok; task += kDecodeWarps) {
-                    const int page = task >> 2, quarter = task & 3;
-                    const uint32_t i = 2 * g + page, slot = i % kRaw;
-                    ok = wait(raw_full + 8 * slot, i / kRaw);
-                    if (!ok) break;
-                    decode_values<D>(smem + Cfg::kOffRaw + slot * Cfg::kChunk,
-                                     smem + Cfg::kOffV + st * Cfg::kValues + page * (D * 128), quarter, raw_shown[slot]);
-                    fence_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        barrier_arrive(raw_empty + 8 * slot);
-                        barrier_arrive(v_full + 8 * st);
-                    }
+                ok = wait(raw_full + 8 * slot2, (i + 2) / kRaw) && (g < 2 || wait(v_empty + 8 * st, (g >> 1) - 1));
+                if (!ok) break;
+                decode_values<D>(smem + Cfg::kOffRaw + slot2 * Cfg::kHalf,
+                                 smem + Cfg::kOffV + st * Cfg::kValues + page * (D * 128), quarter, step_shown[(g & 7) * 2 + page]);
+                fence_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    barrier_arrive(v_full + 8 * st);
+                    barrier_arrive(raw_empty + 8 * slot2);
                 }
             }
         } while (ok && next_item(batch, p, n_kv, group, it));
-    } else {
+    } else if (warp < kSoftmaxWarps) {
         // ---- softmax: one thread a query column
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane, col = tile * kTileRows + row;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + Cfg::kScores + tile * kStepKeys, o_at = tmem + lanes + Cfg::kOut + tile * D;
@@ -775,7 +771,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                     if (!ok) break;
                     fence_after();
                     const uint32_t sh = s_at + h * kKvPage;
-                    const uint64_t shown = step_shown[(g & 3) * 2 + h];
+                    const uint64_t shown = step_shown[(g & 7) * 2 + h];
                     if (shown != ~0ull || key0 + kKvPage - 1 > warp_limit || key0 <= warp_low) {
                         // hidden tokens' scores become -inf in place; the rest
                         // of the page's work then knows no mask
