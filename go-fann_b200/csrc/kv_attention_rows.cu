@@ -38,8 +38,8 @@ constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kRowThreads = 32 * (kLoadWarp + 3);  // whole warpgroups
 // Registers a thread: 96 at launch for 640 threads, 61440 in all; the split
-// below takes 256 x 120 + 256 x 80 + 128 x 56 = 58368.
-constexpr int kSoftmaxRegs = 120, kDecodeRegs = 80, kOtherRegs = 56;
+// below takes 256 x 112 + 256 x 88 + 128 x 72 = 60416.
+constexpr int kSoftmaxRegs = 112, kDecodeRegs = 88, kOtherRegs = 72;
 constexpr float kLag = 8.0f;   // log2 that a column's maximum may run ahead of its reference
 constexpr float kHead = 7.0f;  // log2 of a weight at the reference
 
