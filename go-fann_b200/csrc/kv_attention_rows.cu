@@ -55,7 +55,7 @@ struct Rows {
     static constexpr int kOffRaw = kOffV + 2 * kValues;
     static constexpr int kOffShown = kOffRaw + kRaw * kHalf;        // u64 [8 steps][2 pages]
     static constexpr int kOffBars = kOffShown + 8 * 16;
-    static constexpr int kBars = 2 * kRaw + 8 + 4 * kTiles + 2;
+    static constexpr int kBars = 2 * kRaw + 8 + 5 * kTiles + 2;
     static constexpr int kBytes = 1024 + kOffBars + 8 * kBars + 16;
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
     // tensor memory columns
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
     // [tile][half] of S and P
     const uint32_t s_full = v_empty + 16, p_full = s_full + 16 * kTiles, q_full = p_full + 16 * kTiles;
-    const uint32_t all_done = q_full + 8;
+    const uint32_t all_done = q_full + 8, o_half = all_done + 8;  // o_half: [tile] the first page's product
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffBars + 8 * Cfg::kBars);
     volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a wait has run out
 
@@ -527,6 +527,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         }
         barrier_init(q_full, kTiles * kTileRows);
         barrier_init(all_done, 1);
+        for (int i = 0; i < kTiles; ++i) barrier_init(o_half + 8 * i, 1);
         barrier_fence();
         *dead = 0;
     }
@@ -609,17 +610,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         Item it = start;
         const uint32_t base = shared_addr(smem);
         const uint64_t q_desc = operand_desc(base);
-        const auto scores = [&](int tile, int h, uint32_t stage) {
+        const auto scores = [&](int tile, uint32_t stage) {
             const uint64_t q = q_desc + tile * (Cfg::kQTile >> 4);
-            const uint64_t k = q_desc + ((Cfg::kOffK + h * (kKvPage * 128)) >> 4) + stage * (Cfg::kKeys >> 4);
+            const uint64_t k = q_desc + (Cfg::kOffK >> 4) + stage * (Cfg::kKeys >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
-                    mma_shared(tmem + Cfg::kScores + tile * kStepKeys + h * kKvPage,
-                               q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4),
-                               k + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kKvPage), i > 0);
-                mma_commit(s_full + 16 * tile + 8 * h);
-                if (tile == kTiles - 1 && h == 1) mma_commit(k_empty + 8 * stage);
+                    mma_shared(tmem + Cfg::kScores + tile * kStepKeys, q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4),
+                               k + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kStepKeys), i > 0);
+                mma_commit(s_full + 16 * tile);
+                mma_commit(s_full + 16 * tile + 8);
+                if (tile == kTiles - 1) mma_commit(k_empty + 8 * stage);
             }
         };
         const auto output = [&](int tile, int h, uint32_t stage, uint32_t add) {
@@ -629,6 +630,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                 for (int k = 0; k < kKvPage / 16; ++k)
                     mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + h * kKvPage + 8 * k,
                                v + (k * 32 >> 4), mma_shape(kTileRows, D), k > 0 ? 1u : add);
+                if (h == 0) mma_commit(o_half + 8 * tile);
                 if (tile == kTiles - 1 && h == 1) mma_commit(v_empty + 8 * stage);
             }
         };
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             if (!ok) break;
             fence_after();
 #pragma unroll
-            for (int i = 0; i < 2 * kTiles; ++i) scores(i % kTiles, i / kTiles, g & 1);
+            for (int tile = 0; tile < kTiles; ++tile) scores(tile, g & 1);
             for (int j = 0; j < steps && ok; ++j, ++g) {
                 const uint32_t st = g & 1, next = st ^ 1;
                 const bool more = j + 1 < steps;
@@ -653,15 +655,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                     if (!ok) break;
                     fence_after();
                     output(tile, h, st, j > 0 || h > 0);
+                    if (h == 0) continue;
                     if (more) {
-                        if (i == 0) {
+                        if (tile == 0) {
                             ok = all_wait(k_full + 8 * next, (g + 1) >> 1);
                             if (!ok) break;
                             fence_after();
                         }
-                        scores(tile, h, next);
+                        scores(tile, next);
                     } else if (elect_one()) {
-                        mma_commit(s_full + 16 * tile + 8 * h);
+                        mma_commit(s_full + 16 * tile);
+                        mma_commit(s_full + 16 * tile + 8);
                     }
                 }
             }
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                             }
                             if (j > from || h > 0) {
                                 // behind the product of the page before
-                                ok = wait(s_full + 16 * tile + 8 * (h ^ 1), sg + h);
+                                ok = h == 0 || wait(o_half + 8 * tile, g);
                                 fence_after();
                                 if (ok)
                                     for (int k = 0; k < D / 16; ++k) scale_output(o_at + 16 * k, f);
