@@ -11,7 +11,7 @@
 //   256 columns;
 // * one thread issues S = Q K^T (tcgen05.mma, M = 128, N = 128) and
 //   O += P V (M = 128, N = head_dim, P from tensor memory);
-// * two warpgroups, one thread a query column, turn S into P: mask, maximum,
+// * two warpgroups, one thread a query column, turn S into P: mask and
 //   exponential; P takes the place of S in tensor memory as f16.
 // While one tile is in the exponentials the other has the tensor cores.
 //
@@ -22,9 +22,10 @@
 // Precision: keys and values c * s + m are rounded to f16 (at most 2^-11 of
 // the value; a quantisation step is at least 2^-4 of the group's range, so
 // this is below 2^-7 of what the cache has already rounded), weights to f16;
-// logits, maxima, sums and the output are f32.  The reference point of a
-// column's weights follows its maximum only once it is 2^8 behind, so the
-// output is rarely rescaled; weights are at most 2^15, which f16 holds.
+// logits, sums and the output are f32.  A column's weights are relative to a
+// reference, its first maximum, times 2^7; the reference moves up to the
+// maximum only where 32 weights sum to more than 2^15 (f16 ends at 2^16), so
+// the maximum is rarely looked for and the output rarely rescaled.
 #include "kv_attention.cuh"
 
 namespace gofann {
@@ -40,8 +41,8 @@ constexpr int kRowThreads = 32 * (kLoadWarp + 3);  // whole warpgroups
 // Registers a thread: 96 at launch for 640 threads, 61440 in all; the split
 // below takes 256 x 112 + 256 x 88 + 128 x 72 = 60416.
 constexpr int kSoftmaxRegs = 112, kDecodeRegs = 88, kOtherRegs = 72;
-constexpr float kLag = 8.0f;   // log2 that a column's maximum may run ahead of its reference
-constexpr float kHead = 7.0f;  // log2 of a weight at the reference
+constexpr float kHead = 7.0f;      // log2 of a weight at the reference
+constexpr float kMost = 32768.0f;  // sum of 32 weights from which the reference moves up
 
 template <int D>
 struct Rows {
@@ -287,31 +288,28 @@ __device__ __forceinline__ void decode_values(const unsigned char* chunk, unsign
     }
 }
 
-// Weights 2^(unit x - base) of 32 scores as f16 pairs and their sum (two
-// parts); returns the largest score.
-__device__ __forceinline__ float weigh(const float (&x)[32], float ref, float unit, uint32_t (&w)[16], uint64_t& sum)
+// Weights 2^(unit x - base) of 32 scores as f16 pairs; returns their sum (two
+// parts).
+__device__ __forceinline__ uint64_t weigh(const float (&x)[32], float ref, float unit, uint32_t (&w)[16])
 {
     const float minus_base = fmaf(ref == kNegInf ? 0.0f : -ref, unit, kHead);
     const uint64_t unit2 = pair(unit, unit), minus_base2 = pair(minus_base, minus_base);
-    float m4[4] = {x[0], x[1], x[2], x[3]};
-    sum = 0;
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
+    for (int i = 0; i < 32; i += 2) {
         const uint64_t y = fma_two(pair(x[i], x[i + 1]), unit2, minus_base2);
-        const uint64_t z = fma_two(pair(x[i + 2], x[i + 3]), unit2, minus_base2);
         const float a = exp2_fast(first_of(y)), b = exp2_fast(second_of(y));
-        const float c = exp2_fast(first_of(z)), d = exp2_fast(second_of(z));
-        if (i > 0) {
-            m4[0] = fmaxf(m4[0], x[i]);
-            m4[1] = fmaxf(m4[1], x[i + 1]);
-            m4[2] = fmaxf(m4[2], x[i + 2]);
-            m4[3] = fmaxf(m4[3], x[i + 3]);
-        }
-        sum = add_two(sum, add_two(pair(a, b), pair(c, d)));
+        sum[(i >> 1) & 1] = add_two(sum[(i >> 1) & 1], pair(a, b));
         w[i / 2] = as_word(__floats2half2_rn(a, b));
-        w[i / 2 + 1] = as_word(__floats2half2_rn(c, d));
     }
-    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    return add_two(sum[0], sum[1]);
+}
+__device__ __forceinline__ float largest(const float (&x)[32])
+{
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) m = fmaxf(m, x[i]);
+    return m;
 }
 
 // 16 columns times f: f32 numbers of the output, or pairs of f16 weights.
@@ -805,16 +803,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                         tensor_wait_load();
                         tensor_ready(x);
                         if (c == 0) tensor_load(sh + 32, v[1]);
-                        // weights by the reference so far, the maximum next to them
+                        // weights by the reference so far: their sum tells
+                        // whether one may be too large for that
                         uint32_t w[16];
-                        uint64_t sum;
-                        float mx = weigh(x, ref, unit, w, sum);
-                        const bool far = (mx - ref) * unit > kLag;  // also where there was no reference
+                        uint64_t sum = weigh(x, ref, unit, w);
+                        const bool far = ref == kNegInf || !(first_of(sum) + second_of(sum) <= kMost);
                         if (__any_sync(kFull, far)) {
                             // the reference follows the maximum; what was
                             // weighed by the old one is rescaled
                             float f = 1.0f;
-                            if (far) {
+                            const float mx = largest(x);
+                            if (far && mx > ref) {
                                 f = ref == kNegInf ? 1.0f : exp2_fast((ref - mx) * unit);
                                 ref = mx;
                             }
@@ -833,7 +832,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                                 if (ok)
                                     for (int k = 0; k < D / 16; ++k) scale_output(o_at + 16 * k, f);
                             }
-                            weigh(x, ref, unit, w, sum);
+                            sum = weigh(x, ref, unit, w);
                         }
                         l2 = add_two(l2, sum);
                         // P takes the columns of S that have been read
