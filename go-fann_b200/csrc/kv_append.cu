@@ -49,40 +49,153 @@ __device__ __forceinline__ uint32_t touched_pages(const gofann_kv_batch& b, uint
     return static_cast<uint32_t>((len + kKvPage - 1) / kKvPage - start / kKvPage);
 }
 
-// Rotates the vector in `x` (shared, one warp or half warp of lanes per
-// vector) and returns the lane's four dimensions d0 .. d0 + 3.
-template <int D>
-__device__ __forceinline__ void rotate4(const float* x, int d0, const float* cos, const float* sin, int rotary,
-                                        bool interleaved, float (&y)[4])
+// Eight consecutive elements as they lie; `wide`: the address is a multiple
+// of 16 bytes.
+__device__ __forceinline__ uint4 load8(const void* p, uint64_t i, bool wide)
 {
+    const uint16_t* q = static_cast<const uint16_t*>(p) + i;
+    if (wide) return *reinterpret_cast<const uint4*>(q);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = q[2 * k] | (static_cast<uint32_t>(q[2 * k + 1]) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void unpack8(const uint4& v, int dtype, float (&x)[8])
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const int d = d0 + k;
-        float v = x[d];
-        if (d < rotary) {
-            const int half = rotary >> 1;
-            const int i = interleaved ? d >> 1 : (d < half ? d : d - half);
-            const bool low = interleaved ? (d & 1) == 0 : d < half;
-            const int other = interleaved ? d ^ 1 : (low ? d + half : d - half);
-            const float c = __ldg(cos + i), s = __ldg(sin + i), o = x[other];
-            v = low ? __fsub_rn(__fmul_rn(v, c), __fmul_rn(o, s)) : __fadd_rn(__fmul_rn(v, c), __fmul_rn(o, s));
+        if (dtype == GOFANN_DTYPE_BF16) {
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            x[2 * k] = f.x;
+            x[2 * k + 1] = f.y;
         }
-        y[k] = v;
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8], int dtype)
+{
+    return make_uint4(kv_pack2(x[0], x[1], dtype), kv_pack2(x[2], x[3], dtype), kv_pack2(x[4], x[5], dtype),
+                      kv_pack2(x[6], x[7], dtype));
+}
+
+// How a call's rows are rotated.
+enum { kRotateNone, kRotateHalf, kRotatePairs, kRotateAny };
+
+// cos and sin of this lane's eight dimensions (entries beyond the rotated
+// ones are not set).
+template <int kMode>
+__device__ __forceinline__ void load_angles(const gofann_kv_append_params& p, int pos, int d0, float (&c)[8], float (&s)[8])
+{
+    const int half = static_cast<int>(p.rotary_dim >> 1);
+    const size_t row = static_cast<size_t>(pos) * half;
+    if (kMode == kRotateHalf) {
+        // the eight angles of a lane are consecutive, on both sides of the half
+        const int i = d0 < half ? d0 : d0 - half;
+        if (d0 < static_cast<int>(p.rotary_dim)) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row + i + k));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row + i + k));
+                c[k] = a.x, c[k + 1] = a.y, c[k + 2] = a.z, c[k + 3] = a.w;
+                s[k] = b.x, s[k + 1] = b.y, s[k + 2] = b.z, s[k + 3] = b.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int d = d0 + k;
+            if (d < static_cast<int>(p.rotary_dim)) {
+                const int i = p.interleaved ? d >> 1 : (d < half ? d : d - half);
+                c[k] = __ldg(p.cos + row + i);
+                s[k] = __ldg(p.sin + row + i);
+            }
+        }
     }
 }
 
-template <int D>
+// Rotates this lane's eight dimensions of a vector that LV lanes hold.
+template <int kMode>
+__device__ __forceinline__ void rotate8(const gofann_kv_append_params& p, const uint4& raw, int d0, const float (&c)[8],
+                                        const float (&s)[8], float* stage, float (&x)[8])
+{
+    const int rotary = static_cast<int>(p.rotary_dim), half = rotary >> 1;
+    float o[8];  // the other element of each pair
+    if (kMode == kRotateHalf) {
+        const int lane = threadIdx.x & 31, from = d0 < half ? lane + half / 8 : lane - half / 8;
+        const int src = d0 < rotary ? from : lane;
+        uint4 w;
+        w.x = __shfl_sync(kFull, raw.x, src);
+        w.y = __shfl_sync(kFull, raw.y, src);
+        w.z = __shfl_sync(kFull, raw.z, src);
+        w.w = __shfl_sync(kFull, raw.w, src);
+        unpack8(w, p.dtype, o);
+    } else if (kMode == kRotatePairs) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = x[k ^ 1];
+    } else {
+        __syncwarp();
+        *reinterpret_cast<float4*>(stage + d0) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(stage + d0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int d = d0 + k;
+            o[k] = d < rotary ? stage[d < half ? d + half : d - half] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int d = d0 + k;
+        const bool low = kMode == kRotatePairs ? (k & 1) == 0 : d < half;
+        // x_a cos - x_b sin, x_b cos + x_a sin; every step rounded by itself
+        const float a = __fmul_rn(x[k], c[k]), b = __fmul_rn(o[k], s[k]);
+        const float y = low ? __fsub_rn(a, b) : __fadd_rn(a, b);
+        x[k] = d < rotary ? y : x[k];
+    }
+}
+
+// The page words [i] of this thread, and the nibbles of them that the rows
+// [lo, hi) of the page write.
+__device__ __forceinline__ uint32_t key_mask(int i, int G, int lo, int hi)
+{
+    const int g = (i >> 4) & 7, kt = (i >> 7) / G, k0 = 16 * (g >> 1) + 4 * kt + (g & 1);
+    return (k0 >= lo && k0 < hi ? 0x00ff00ffu : 0u) | (k0 + 2 >= lo && k0 + 2 < hi ? 0xff00ff00u : 0u);
+}
+__device__ __forceinline__ uint32_t value_mask(int i, int lo, int hi)
+{
+    const int k1 = 16 * ((i >> 2) & 3) + 4 * (i & 3);  // tokens k1 .. k1 + 3: 2 n + e
+    uint32_t m = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (k1 + q >= lo && k1 + q < hi) m |= 0x0f0fu << (16 * (q & 1) + 4 * (q >> 1));
+    return m;
+}
+
+// What bounds it: a full page is a stream (q, k, v in, q, k, v out, codes),
+// a decode step's single rows are the chain of dependent loads: sequence, page
+// number, then everything else at once.  So all that a block reads is asked
+// for before it is used: page words that are only partly written, the keys
+// that the page holds, the rows.
+template <int D, int kMode>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
                                                                    gofann_kv_append_params p, bool q_wide,
                                                                    bool kv_wide)
 {
     using Chunk = KvChunk<D>;
     constexpr int G = Chunk::kGroups;
-    constexpr int kLanes = D / 4;                       // lanes of one vector
-    constexpr int kVectors = kAppendThreads / kLanes;   // vectors at a time
-    __shared__ uint8_t codes[2][kKvPage][D];            // keys, values
+    constexpr int kLanes = D / 8;                           // lanes of one vector
+    constexpr int kVectors = kAppendThreads / kLanes;       // vectors at a time
+    constexpr int kWords = Chunk::kCodes / 4 / kAppendThreads;  // of keys (and of values) per thread
+    constexpr int kParts = kAppendThreads / (16 * G);       // threads that share four dimensions of the old keys
+    constexpr int kKeyRow = D == 128 ? 192 : 64;            // bytes: rows of two tokens in different banks
+    constexpr int kValueRow = kKvPage + 4;
+    __shared__ __align__(16) uint8_t key_codes[kKvPage * kKeyRow];  // [token][dim]
+    __shared__ __align__(16) uint8_t value_codes[D * kValueRow];    // [dim][token]
     __shared__ uint32_t params[2][kKvPage][G];
-    __shared__ __align__(16) float stage[kVectors][D];
+    __shared__ __align__(16) float high_of[kVectors + kParts][D], low_of[kVectors + kParts][D];
     __shared__ float top[kAppendThreads / 32];
 
     const uint32_t head = blockIdx.y;
@@ -102,193 +215,274 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cac
     const int start = len - n_rows;  // position of the first row; negative where rows exceed the length
     const int block = (start > 0 ? start / kKvPage : 0) + static_cast<int>(at);
     const int base = block * kKvPage;
-    const int lo = start > base ? start - base : 0;           // first new token of the page
+    const int lo = start > base ? start - base : 0;              // first new token of the page
     const int hi = len - base < kKvPage ? len - base : kKvPage;  // tokens that the page holds
     const int32_t page = __ldg(batch.page_table + static_cast<size_t>(seq) * batch.max_pages + block);
     const bool page_ok = page >= 0 && static_cast<uint32_t>(page) < cache.n_pages;
     if (!page_ok && threadIdx.x == 0) kv_invalid(batch);
     uint8_t* chunk = cache.pages + (static_cast<size_t>(page_ok ? page : 0) * cache.n_kv_heads + head) * Chunk::kBytes;
+    uint32_t* kw = reinterpret_cast<uint32_t*>(chunk);
+    uint32_t* vw = reinterpret_cast<uint32_t*>(chunk + Chunk::kValueCodes);
+    uint32_t* kp = reinterpret_cast<uint32_t*>(chunk + Chunk::kKeyParams);
+    uint32_t* vp = reinterpret_cast<uint32_t*>(chunk + Chunk::kValueParams);
 
-    // ---- rotate and quantise, one vector per kLanes lanes
-    const uint32_t group = p.n_heads / cache.n_kv_heads;
-    const int n_q = p.q ? static_cast<int>(group) : 0;
-    const int per_token = n_q + 2;
-    const int work = (hi - lo) * per_token;
-    const int vec = threadIdx.x / kLanes, d0 = (threadIdx.x % kLanes) * 4;
-    for (int w0 = 0; w0 < work; w0 += kVectors) {
-        const int w = w0 + vec;
-        const bool on = w < work;
-        const int token = on ? lo + w / per_token : lo, kind = on ? w % per_token : 0;
-        const int row = first_row + base + token - start;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const bool is_q = kind < n_q, is_k = kind == n_q;
-        if (on) {
-            if (is_q)
-                kv_load4(p.q, static_cast<uint64_t>(row) * p.q_stride + (head * group + kind) * D + d0, p.dtype, q_wide, x);
-            else if (is_k)
-                kv_load4(p.k, static_cast<uint64_t>(row) * p.k_stride + head * D + d0, p.dtype, kv_wide, x);
-            else
-                kv_load4(p.v, static_cast<uint64_t>(row) * p.v_stride + head * D + d0, p.dtype, kv_wide, x);
+    // ---- words that keep some of their nibbles
+    uint32_t old_k[kWords], old_v[kWords];
+#pragma unroll
+    for (int n = 0; n < kWords; ++n) {
+        const int i = threadIdx.x + n * kAppendThreads;
+        const uint32_t mk = key_mask(i, G, lo, hi), mv = value_mask(i, lo, hi);
+        old_k[n] = page_ok && mk && mk != ~0u ? kw[i] : 0u;
+        old_v[n] = page_ok && mv && mv != ~0u ? vw[i] : 0u;
+    }
+    // ---- largest and smallest of the keys that the page held before: four
+    // dimensions a thread, of every kParts-th pair of tokens
+    if (cache.bounds) {
+        const int combo = threadIdx.x % (16 * G), part = threadIdx.x / (16 * G);
+        const int grp = combo / 16, tj = combo % 16;
+        float h[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = kNegInf, l[k] = -kNegInf;
+        if (lo > 0 && page_ok) {
+#pragma unroll
+            for (int n = 0; n < 32 / kParts; ++n) {
+                const int pairs = part + n * kParts, g = pairs & 7, kt = pairs >> 3;
+                const int token = 16 * (g >> 1) + 4 * kt + (g & 1);
+                if (token >= lo) continue;
+                const uint32_t w = kw[((kt * G + grp) * 8 + g) * 16 + tj];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if (token + 2 * r >= lo) continue;
+                    const uint32_t sm = kp[((g * 4 + kt) * 2 + r) * G + grp], b = w >> (8 * r);
+                    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffff)));
+                    const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
+                    const uint32_t c[4] = {b & 0xf, (b >> 16) & 0xf, (b >> 4) & 0xf, (b >> 20) & 0xf};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = __fadd_rn(__fmul_rn(static_cast<float>(c[k]), s), m);
+                        h[k] = fmaxf(h[k], x);
+                        l[k] = fminf(l[k], x);
+                    }
+                }
+            }
         }
-        __syncwarp();
-        *reinterpret_cast<float4*>(&stage[vec][d0]) = make_float4(x[0], x[1], x[2], x[3]);
-        __syncwarp();
-        if (on && (is_q || is_k) && p.rotary_dim) {
-            int pos = p.positions ? __ldg(p.positions + row) : base + token;
+        const int d = 64 * grp + 4 * tj;  // dimension 64 grp + 16 t + 4 j
+        *reinterpret_cast<float4*>(&high_of[kVectors + part][d]) = make_float4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<float4*>(&low_of[kVectors + part][d]) = make_float4(l[0], l[1], l[2], l[3]);
+    }
+
+    // ---- rotate and quantise: a lane group takes a token and its vectors one
+    // after the other (query heads, key, value); where there are fewer tokens
+    // than groups, a token's vectors are dealt out to several groups
+    const uint32_t group = p.n_heads / cache.n_kv_heads;
+    const int n_q = p.q ? static_cast<int>(group) : 0, kinds = n_q + 2, tokens = hi - lo;
+    const int vec = threadIdx.x / kLanes, d0 = (threadIdx.x % kLanes) * 8;
+    const int share = tokens < kVectors ? kVectors / tokens : 1;  // groups of a token
+    const int kind0 = share > 1 ? vec / tokens : 0;
+    const int step = share > 1 ? tokens : kVectors;
+    float high[8], low[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) high[k] = kNegInf, low[k] = -kNegInf;
+    for (int t0 = 0; t0 < tokens; t0 += step) {
+        const int token = lo + t0 + (share > 1 ? vec % tokens : vec);
+        const bool on = token < hi && kind0 < share;
+        const int row = first_row + base + (on ? token : lo) - start;
+        float c[8], s[8];
+        if (kMode != kRotateNone) {
+            int pos = p.positions ? __ldg(p.positions + row) : base + (on ? token : lo);
             if (pos < 0 || static_cast<uint32_t>(pos) >= p.n_positions) {
                 if (d0 == 0) kv_invalid(batch);
                 pos = 0;
             }
-            const size_t t = static_cast<size_t>(pos) * (p.rotary_dim >> 1);
-            rotate4<D>(stage[vec], d0, p.cos + t, p.sin + t, static_cast<int>(p.rotary_dim), p.interleaved != 0, x);
+            load_angles<kMode>(p, pos, d0, c, s);
         }
-        if (on && is_q) {
-            uint2* out = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.q_out) +
-                                                  (static_cast<uint64_t>(row) * p.n_heads + head * group + kind) * D + d0);
-            *out = make_uint2(kv_pack2(x[0], x[1], p.dtype), kv_pack2(x[2], x[3], p.dtype));
-        }
-        // min and max over the 16 lanes of a group (every lane takes part)
-        float mn = 0.0f, mx = 0.0f;
+        const uint64_t q_at = static_cast<uint64_t>(row) * p.q_stride + head * group * D + d0;
+        const uint64_t k_at = static_cast<uint64_t>(row) * p.k_stride + head * D + d0;
+        const uint64_t v_at = static_cast<uint64_t>(row) * p.v_stride + head * D + d0;
+        const auto fetch = [&](int kind) {
+            if (!on || kind >= kinds) return make_uint4(0u, 0u, 0u, 0u);
+            return kind < n_q ? load8(p.q, q_at + static_cast<uint64_t>(kind) * D, q_wide)
+                              : kind == n_q ? load8(p.k, k_at, kv_wide) : load8(p.v, v_at, kv_wide);
+        };
+        constexpr int kAhead = 3;  // vectors on their way
+        uint4 next[kAhead];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[k] = x[k] == x[k] ? fminf(fmaxf(x[k], -GOFANN_KV_CLAMP), GOFANN_KV_CLAMP) : 0.0f;
-            mn = k ? fminf(mn, x[k]) : x[k];
-            mx = k ? fmaxf(mx, x[k]) : x[k];
-        }
+        for (int a = 0; a < kAhead; ++a) next[a] = fetch(kind0 + a * share);
+        // every lane of the warp makes the same turns (the shuffles need them)
+        for (int turn = 0; turn * share < kinds; ++turn) {
+            const int kind = kind0 + turn * share;
+            const uint4 raw = next[0];
 #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) {
-            mn = fminf(mn, __shfl_xor_sync(kFull, mn, off));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
-        }
-        if (on && !is_q) {
+            for (int a = 0; a + 1 < kAhead; ++a) next[a] = next[a + 1];
+            next[kAhead - 1] = fetch(kind + kAhead * share);
+            const bool is_q = kind < n_q, is_k = kind == n_q, live = on && kind < kinds;
+            float x[8];
+            unpack8(raw, p.dtype, x);
+            if (kMode != kRotateNone) {
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = x[k];
+                // (low_of's row is free until the bounds are written)
+                rotate8<kMode>(p, raw, d0, c, s, low_of[vec], y);
+                if (kind <= n_q) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = y[k];
+                }
+            }
+            if (live && is_q)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.q_out) +
+                                          (static_cast<uint64_t>(row) * p.n_heads + head * group + kind) * D + d0) =
+                    pack8(x, p.dtype);
+            if (__all_sync(kFull, !live || is_q)) continue;
+            // minimum and maximum over the eight lanes of a group of 64
+            float mn, mx;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                x[k] = x[k] == x[k] ? fminf(fmaxf(x[k], -GOFANN_KV_CLAMP), GOFANN_KV_CLAMP) : 0.0f;
+                mn = k ? fminf(mn, x[k]) : x[k];
+                mx = k ? fmaxf(mx, x[k]) : x[k];
+            }
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) {
+                mn = fminf(mn, __shfl_xor_sync(kFull, mn, off));
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
+            }
+            if (!live || is_q) continue;
             const __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.0f)), hm = __float2half_rn(mn);
-            const float s = __half2float(hs), m = __half2float(hm);
-            uint32_t c4 = 0;
-            float val[4];
+            const float scale = __half2float(hs), m = __half2float(hm);
+            // rint of the quotient: by the reciprocal, unless that is so near
+            // a half that the rounded quotient might fall to the other side
+            const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+            float code[8];
+            bool near = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float c = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[k], m), s)), 0.0f), 15.0f) : 0.0f;
-                c4 |= static_cast<uint32_t>(c) << (8 * k);
-                val[k] = __fadd_rn(__fmul_rn(c, s), m);
+            for (int k = 0; k < 8; ++k) {
+                const float t = (x[k] - m) * inv;
+                code[k] = rintf(t);
+                near |= fabsf(t - code[k]) > 0.4995f;
             }
-            const int which = is_k ? 0 : 1;
-            *reinterpret_cast<uint32_t*>(&codes[which][token][d0]) = c4;
-            if ((d0 & (kKvGroup - 1)) == 0) {
-                params[which][token][d0 / kKvGroup] = static_cast<uint32_t>(__half_as_ushort(hs)) |
-                                                     (static_cast<uint32_t>(__half_as_ushort(hm)) << 16);
+            if (near) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) code[k] = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x[k], m), scale)) : 0.0f;
             }
+            uint32_t c8[2] = {0, 0};
+            float val[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                code[k] = fminf(fmaxf(code[k], 0.0f), 15.0f);
+                c8[k >> 2] |= static_cast<uint32_t>(code[k]) << (8 * (k & 3));
+                val[k] = __fadd_rn(__fmul_rn(code[k], scale), m);
+            }
+            if (is_k) {
+                *reinterpret_cast<uint2*>(&key_codes[token * kKeyRow + d0]) = make_uint2(c8[0], c8[1]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    high[k] = fmaxf(high[k], val[k]);
+                    low[k] = fminf(low[k], val[k]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) value_codes[(d0 + k) * kValueRow + token] = (c8[k >> 2] >> (8 * (k & 3))) & 0xff;
+            }
+            if ((d0 & (kKvGroup - 1)) == 0)
+                params[is_k ? 0 : 1][token][d0 / kKvGroup] = static_cast<uint32_t>(__half_as_ushort(hs)) |
+                                                            (static_cast<uint32_t>(__half_as_ushort(hm)) << 16);
             void* out = is_k ? p.k_out : p.v_out;
             if (out)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) +
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) +
                                           (static_cast<uint64_t>(row) * cache.n_kv_heads + head) * D + d0) =
-                    make_uint2(kv_pack2(val[0], val[1], p.dtype), kv_pack2(val[2], val[3], p.dtype));
+                    pack8(val, p.dtype);
         }
     }
     if (!page_ok) return;
+    if (kMode == kRotateAny) __syncwarp();  // the stage was low_of's row
+    if (cache.bounds) {
+        *reinterpret_cast<float4*>(&high_of[vec][d0]) = make_float4(high[0], high[1], high[2], high[3]);
+        *reinterpret_cast<float4*>(&high_of[vec][d0 + 4]) = make_float4(high[4], high[5], high[6], high[7]);
+        *reinterpret_cast<float4*>(&low_of[vec][d0]) = make_float4(low[0], low[1], low[2], low[3]);
+        *reinterpret_cast<float4*>(&low_of[vec][d0 + 4]) = make_float4(low[4], low[5], low[6], low[7]);
+    }
     __syncthreads();
 
     // ---- merge the codes into the page's words
-    uint32_t* kw = reinterpret_cast<uint32_t*>(chunk);
-    uint32_t* vw = reinterpret_cast<uint32_t*>(chunk + Chunk::kValueCodes);
-    for (int i = threadIdx.x; i < Chunk::kCodes / 4; i += kAppendThreads) {
-        // key word [kt][grp][g][t][j]: tokens k0 (even bytes) and k0 + 2, dimensions d .. d + 3
-        const int j = i & 3, t = (i >> 2) & 3, g = (i >> 4) & 7, grp = (i >> 7) % G, kt = (i >> 7) / G;
-        const int k0 = 16 * (g >> 1) + 4 * kt + (g & 1), d = 64 * grp + 16 * t + 4 * j;
-        uint32_t mask = 0, word = 0;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int token = k0 + 2 * r;
-            if (token >= lo && token < hi) {
-                const uint32_t c = *reinterpret_cast<const uint32_t*>(&codes[0][token][d]);
-                mask |= 0x00ff00ffu << (8 * r);
-                word |= ((c & 0xf) | ((c >> 12) & 0xf0) | ((c << 8) & 0x000f0000) | ((c >> 4) & 0x00f00000)) << (8 * r);
-            }
-        }
-        if (mask) kw[i] = mask == 0xffffffffu ? word : ((kw[i] & ~mask) | word);
-        // value word [dt][g][t][kt]: dimensions dv and dv + 8, tokens k1 .. k1 + 3
-        const int vkt = i & 3, vt = (i >> 2) & 3, vg = (i >> 4) & 7, dt = i >> 7;
-        const int k1 = 16 * vt + 4 * vkt, dv = 16 * dt + vg;
-        mask = 0, word = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // token k1 + q = 2 n + e: nibble n of the bytes 2 e + r
-            const int token = k1 + q;
-            if (token >= lo && token < hi) {
-                const int shift = 16 * (q & 1) + 4 * (q >> 1);
-                mask |= 0x0f0fu << shift;
-                word |= (static_cast<uint32_t>(codes[1][token][dv]) |
-                         (static_cast<uint32_t>(codes[1][token][dv + 8]) << 8)) << shift;
-            }
-        }
-        if (mask) vw[i] = mask == 0xffffffffu ? word : ((vw[i] & ~mask) | word);
-    }
-    uint32_t* kp = reinterpret_cast<uint32_t*>(chunk + Chunk::kKeyParams);
-    uint32_t* vp = reinterpret_cast<uint32_t*>(chunk + Chunk::kValueParams);
-    for (int i = threadIdx.x; i < kKvPage * G; i += kAppendThreads) {
-        const int token = i / G, grp = i % G, w = kv_param_word<D>(token) + grp;
-        if (token >= lo && token < hi) {
-            kp[w] = params[0][token][grp];
-            vp[w] = params[1][token][grp];
-        } else if (token < lo) {
-            params[0][token][grp] = kp[w];
-        }
-    }
-    // the codes of the keys that the page held before
-    if (lo > 0) {
-        for (int i = threadIdx.x; i < Chunk::kCodes / 4; i += kAppendThreads) {
+    for (int n = 0; n < kWords; ++n) {
+        const int i = threadIdx.x + n * kAppendThreads;
+        const uint32_t mk = key_mask(i, G, lo, hi), mv = value_mask(i, lo, hi);
+        if (mk) {
+            // key word [kt][grp][g][t][j]: tokens k0 (even bytes) and k0 + 2, dimensions d .. d + 3
             const int j = i & 3, t = (i >> 2) & 3, g = (i >> 4) & 7, grp = (i >> 7) % G, kt = (i >> 7) / G;
             const int k0 = 16 * (g >> 1) + 4 * kt + (g & 1), d = 64 * grp + 16 * t + 4 * j;
-            if (k0 >= lo) continue;
-            const uint32_t word = kw[i];
+            uint32_t word = 0;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if (k0 + 2 * r < lo) {
-                    const uint32_t b = word >> (8 * r);
-                    *reinterpret_cast<uint32_t*>(&codes[0][k0 + 2 * r][d]) =
-                        (b & 0xf) | ((b >> 8) & 0xf00) | ((b << 12) & 0xf0000) | ((b << 4) & 0xf000000);
-                }
+                const uint32_t c = *reinterpret_cast<const uint32_t*>(&key_codes[(k0 + 2 * r) * kKeyRow + d]);
+                word |= ((c & 0xf) | ((c >> 12) & 0xf0) | ((c << 8) & 0x000f0000) | ((c >> 4) & 0x00f00000)) << (8 * r);
             }
+            kw[i] = (word & mk) | (old_k[n] & ~mk);
+        }
+        if (mv) {
+            // value word [dt][g][t][kt]: dimensions dv and dv + 8, tokens k1 .. k1 + 3 = 2 n + e: nibble n of bytes 2 e + r
+            const int vkt = i & 3, vt = (i >> 2) & 3, vg = (i >> 4) & 7, dt = i >> 7;
+            const int k1 = 16 * vt + 4 * vkt, dv = 16 * dt + vg;
+            uint32_t word = 0;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t c = *reinterpret_cast<const uint32_t*>(&value_codes[(dv + 8 * r) * kValueRow + k1]);
+                word |= ((c & 0xf) | ((c >> 12) & 0xf0) | ((c << 8) & 0x000f0000) | ((c >> 4) & 0x00f00000)) << (8 * r);
+            }
+            vw[i] = (word & mv) | (old_v[n] & ~mv);
         }
     }
-    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * G; i += kAppendThreads) {
+        const int token = lo + i / G, grp = i % G, w = kv_param_word<D>(token) + grp;
+        kp[w] = params[0][token][grp];
+        vp[w] = params[1][token][grp];
+    }
 
-    // ---- bounds of the page's tokens: kThreadsPerDim threads share a dimension
+    // ---- bounds of the page's tokens: a thread a dimension
     if (!cache.bounds) return;
-    constexpr int kShare = kAppendThreads / D;
-    const int d = threadIdx.x / kShare, part = threadIdx.x % kShare;
-    float high = kNegInf, low = -kNegInf;
-    for (int token = part; token < hi; token += kShare) {
-        const uint32_t sm = params[0][token][d / kKvGroup];
-        const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffff)));
-        const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
-        const float x = __fadd_rn(__fmul_rn(static_cast<float>(codes[0][token][d]), s), m);
-        high = fmaxf(high, x);
-        low = fminf(low, x);
-    }
+    float h = kNegInf, l = -kNegInf;
+    if (threadIdx.x < D) {
 #pragma unroll
-    for (int off = 1; off < kShare; off <<= 1) {
-        high = fmaxf(high, __shfl_xor_sync(kFull, high, off));
-        low = fminf(low, __shfl_xor_sync(kFull, low, off));
+        for (int v = 0; v < kVectors + kParts; ++v) {
+            h = fmaxf(h, high_of[v][threadIdx.x]);
+            l = fminf(l, low_of[v][threadIdx.x]);
+        }
     }
-    float a = fmaxf(fabsf(high), fabsf(low));
+    float a = threadIdx.x < D ? fmaxf(fabsf(h), fabsf(l)) : 0.0f;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(kFull, a, off));
     if (lane == 0) top[threadIdx.x >> 5] = a;
     __syncthreads();
+    if (threadIdx.x >= D) return;
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) a = fmaxf(a, top[w]);
+    for (int w = 0; w < D / 32; ++w) a = fmaxf(a, top[w]);
     const float scale = __fdiv_rn(a, 127.0f);
     const size_t entry = static_cast<size_t>(page) * cache.n_kv_heads + head;
-    if (part == 0) {
-        float h8 = 0.0f, l8 = 0.0f;
-        if (scale > 0.0f) {
-            h8 = fminf(fmaxf(ceilf(__fdiv_rn(high, scale)), -127.0f), 127.0f);
-            l8 = fminf(fmaxf(floorf(__fdiv_rn(low, scale)), -127.0f), 127.0f);
-        }
-        int8_t* bounds = cache.bounds + entry * 2 * D;
-        bounds[d] = static_cast<int8_t>(h8);
-        bounds[D + d] = static_cast<int8_t>(l8);
+    float h8 = 0.0f, l8 = 0.0f;
+    if (scale > 0.0f) {
+        h8 = fminf(fmaxf(ceilf(__fdiv_rn(h, scale)), -127.0f), 127.0f);
+        l8 = fminf(fmaxf(floorf(__fdiv_rn(l, scale)), -127.0f), 127.0f);
     }
+    int8_t* bounds = cache.bounds + entry * 2 * D;
+    bounds[threadIdx.x] = static_cast<int8_t>(h8);
+    bounds[D + threadIdx.x] = static_cast<int8_t>(l8);
     if (threadIdx.x == 0) cache.bound_scale[entry] = scale;
+}
+
+template <int D>
+void launch_append(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_append_params& p, int mode,
+                   bool q_wide, bool kv_wide, dim3 grid, cudaStream_t s)
+{
+    if (mode == kRotateNone)
+        kv_append_kernel<D, kRotateNone><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+    else if (mode == kRotateHalf)
+        kv_append_kernel<D, kRotateHalf><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+    else if (mode == kRotatePairs)
+        kv_append_kernel<D, kRotatePairs><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+    else
+        kv_append_kernel<D, kRotateAny><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
 }
 
 }  // namespace
@@ -326,8 +520,8 @@ int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
     auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     if ((bits(cache->pages) & 15) || (bits(cache->bounds) & 15))
         return fail(GOFANN_ERR_INVALID, "kv_append: pages and bounds must be 16-byte aligned");
-    if ((bits(p.q_out) | bits(p.k_out) | bits(p.v_out)) & 7)
-        return fail(GOFANN_ERR_INVALID, "kv_append: outputs must be 8-byte aligned");
+    if ((bits(p.q_out) | bits(p.k_out) | bits(p.v_out)) & 15)
+        return fail(GOFANN_ERR_INVALID, "kv_append: outputs must be 16-byte aligned");
     if ((bits(p.q) | bits(p.k) | bits(p.v)) & 1)
         return fail(GOFANN_ERR_INVALID, "kv_append: inputs must be 2-byte aligned");
     if (p.q && p.q == p.q_out && p.q_stride != static_cast<uint64_t>(p.n_heads) * d)
@@ -336,13 +530,19 @@ int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
     // a sequence of n rows touches at most n / 64 + 2 pages, and at most n
     const uint64_t bound = static_cast<uint64_t>(batch->n_rows) / GOFANN_KV_PAGE + 2ull * batch->n_seqs;
     const uint32_t units = static_cast<uint32_t>(bound < batch->n_rows ? bound : batch->n_rows);
-    const bool q_wide = (bits(p.q) & 7) == 0 && (p.q_stride & 3) == 0;
-    const bool kv_wide = ((bits(p.k) | bits(p.v)) & 7) == 0 && ((p.k_stride | p.v_stride) & 3) == 0;
+    const bool q_wide = (bits(p.q) & 15) == 0 && (p.q_stride & 7) == 0;
+    const bool kv_wide = ((bits(p.k) | bits(p.v)) & 15) == 0 && ((p.k_stride | p.v_stride) & 7) == 0;
+    // the two halves of a pair in lanes of their own need whole lanes and
+    // 16-byte table rows; adjacent pairs never cross a lane
+    const int mode = p.rotary_dim == 0 ? kRotateNone
+                     : p.interleaved   ? kRotatePairs
+                     : p.rotary_dim % 16 == 0 && ((bits(p.cos) | bits(p.sin)) & 15) == 0 ? kRotateHalf
+                                                                                         : kRotateAny;
     const dim3 grid(units, cache->n_kv_heads);
     if (d == 64)
-        kv_append_kernel<64><<<grid, kAppendThreads, 0, as_stream(stream)>>>(*cache, *batch, p, q_wide, kv_wide);
+        launch_append<64>(*cache, *batch, p, mode, q_wide, kv_wide, grid, as_stream(stream));
     else
-        kv_append_kernel<128><<<grid, kAppendThreads, 0, as_stream(stream)>>>(*cache, *batch, p, q_wide, kv_wide);
+        launch_append<128>(*cache, *batch, p, mode, q_wide, kv_wide, grid, as_stream(stream));
     GOFANN_CHECK_LAUNCH("kv_append_kernel");
     return GOFANN_OK;
 }
