@@ -36,8 +36,6 @@ int kv_check(const char* who, const gofann_kv_cache* cache, const gofann_kv_batc
 
 namespace {
 
-constexpr int kAppendThreads = 256;
-
 // Pages that sequence s's rows touch.
 __device__ __forceinline__ uint32_t touched_pages(const gofann_kv_batch& b, uint32_t s)
 {
@@ -60,12 +58,13 @@ __device__ __forceinline__ uint4 load8(const void* p, uint64_t i, bool wide)
     for (int k = 0; k < 4; ++k) w[k] = q[2 * k] | (static_cast<uint32_t>(q[2 * k + 1]) << 16);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void unpack8(const uint4& v, int dtype, float (&x)[8])
+template <bool kBf16>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
 {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        if (dtype == GOFANN_DTYPE_BF16) {
+        if (kBf16) {
             x[2 * k] = __uint_as_float(w[k] << 16);
             x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
         } else {
@@ -75,63 +74,72 @@ __device__ __forceinline__ void unpack8(const uint4& v, int dtype, float (&x)[8]
         }
     }
 }
-__device__ __forceinline__ uint4 pack8(const float (&x)[8], int dtype)
+template <bool kBf16>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8])
 {
-    return make_uint4(kv_pack2(x[0], x[1], dtype), kv_pack2(x[2], x[3], dtype), kv_pack2(x[4], x[5], dtype),
-                      kv_pack2(x[6], x[7], dtype));
+    constexpr int t = kBf16 ? GOFANN_DTYPE_BF16 : GOFANN_DTYPE_F16;
+    return make_uint4(kv_pack2(x[0], x[1], t), kv_pack2(x[2], x[3], t), kv_pack2(x[4], x[5], t), kv_pack2(x[6], x[7], t));
 }
 
-// How a call's rows are rotated.
+// How a call's rows are rotated.  Half and Pairs: whole lanes of eight
+// dimensions are rotated or not; Any: every other form, through shared memory.
 enum { kRotateNone, kRotateHalf, kRotatePairs, kRotateAny };
 
-// cos and sin of this lane's eight dimensions (entries beyond the rotated
-// ones are not set).
+// cos and sin of this lane's eight dimensions; sin with the sign that it has
+// in x_a cos - x_b sin, x_b cos + x_a sin.
 template <int kMode>
 __device__ __forceinline__ void load_angles(const gofann_kv_append_params& p, int pos, int d0, float (&c)[8], float (&s)[8])
 {
-    const int half = static_cast<int>(p.rotary_dim >> 1);
+    const int rotary = static_cast<int>(p.rotary_dim), half = rotary >> 1;
     const size_t row = static_cast<size_t>(pos) * half;
     if (kMode == kRotateHalf) {
-        // the eight angles of a lane are consecutive, on both sides of the half
-        const int i = d0 < half ? d0 : d0 - half;
-        if (d0 < static_cast<int>(p.rotary_dim)) {
+        if (d0 >= rotary) return;
+        const bool low = d0 < half;
+        const int i = low ? d0 : d0 - half;
 #pragma unroll
-            for (int k = 0; k < 8; k += 4) {
-                const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row + i + k));
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row + i + k));
-                c[k] = a.x, c[k + 1] = a.y, c[k + 2] = a.z, c[k + 3] = a.w;
-                s[k] = b.x, s[k + 1] = b.y, s[k + 2] = b.z, s[k + 3] = b.w;
-            }
+        for (int k = 0; k < 8; k += 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row + i + k));
+            const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row + i + k));
+            c[k] = a.x, c[k + 1] = a.y, c[k + 2] = a.z, c[k + 3] = a.w;
+            s[k] = low ? -b.x : b.x, s[k + 1] = low ? -b.y : b.y, s[k + 2] = low ? -b.z : b.z, s[k + 3] = low ? -b.w : b.w;
         }
+    } else if (kMode == kRotatePairs) {
+        if (d0 >= rotary) return;
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + row + d0 / 2));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(p.sin + row + d0 / 2));
+        c[0] = c[1] = a.x, c[2] = c[3] = a.y, c[4] = c[5] = a.z, c[6] = c[7] = a.w;
+        s[0] = -b.x, s[1] = b.x, s[2] = -b.y, s[3] = b.y, s[4] = -b.z, s[5] = b.z, s[6] = -b.w, s[7] = b.w;
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int d = d0 + k;
-            if (d < static_cast<int>(p.rotary_dim)) {
-                const int i = p.interleaved ? d >> 1 : (d < half ? d : d - half);
-                c[k] = __ldg(p.cos + row + i);
-                s[k] = __ldg(p.sin + row + i);
-            }
+            if (d >= rotary) continue;
+            const bool low = p.interleaved ? (d & 1) == 0 : d < half;
+            const int i = p.interleaved ? d >> 1 : (d < half ? d : d - half);
+            c[k] = __ldg(p.cos + row + i);
+            const float b = __ldg(p.sin + row + i);
+            s[k] = low ? -b : b;
         }
     }
 }
 
-// Rotates this lane's eight dimensions of a vector that LV lanes hold.
-template <int kMode>
+// Rotates this lane's eight dimensions of a vector that consecutive lanes
+// hold; every product and sum rounded by itself.  All lanes of the warp call
+// it.
+template <int kMode, bool kBf16>
 __device__ __forceinline__ void rotate8(const gofann_kv_append_params& p, const uint4& raw, int d0, const float (&c)[8],
                                         const float (&s)[8], float* stage, float (&x)[8])
 {
     const int rotary = static_cast<int>(p.rotary_dim), half = rotary >> 1;
     float o[8];  // the other element of each pair
     if (kMode == kRotateHalf) {
-        const int lane = threadIdx.x & 31, from = d0 < half ? lane + half / 8 : lane - half / 8;
-        const int src = d0 < rotary ? from : lane;
+        const int lane = threadIdx.x & 31, src = d0 >= rotary ? lane : d0 < half ? lane + half / 8 : lane - half / 8;
         uint4 w;
         w.x = __shfl_sync(kFull, raw.x, src);
         w.y = __shfl_sync(kFull, raw.y, src);
         w.z = __shfl_sync(kFull, raw.z, src);
         w.w = __shfl_sync(kFull, raw.w, src);
-        unpack8(w, p.dtype, o);
+        unpack8<kBf16>(w, o);
     } else if (kMode == kRotatePairs) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] = x[k ^ 1];
@@ -143,18 +151,67 @@ __device__ __forceinline__ void rotate8(const gofann_kv_append_params& p, const 
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int d = d0 + k;
-            o[k] = d < rotary ? stage[d < half ? d + half : d - half] : 0.0f;
+            o[k] = d < rotary ? stage[p.interleaved ? d ^ 1 : d < half ? d + half : d - half] : 0.0f;
         }
+    }
+    if (kMode != kRotateAny && d0 >= rotary) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (kMode != kRotateAny || d0 + k < rotary) x[k] = __fadd_rn(__fmul_rn(x[k], c[k]), __fmul_rn(o[k], s[k]));
+}
+
+// Eight values of a group that eight lanes hold: their codes, the values that
+// those stand for and the group's params (f16 scale below, minimum above).
+// All lanes of the warp call it.
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], float (&code)[8])
+{
+    float mn, mx;
+    const auto range = [&]() {
+        mn = mx = x[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            mn = fminf(mn, x[k]);
+            mx = fmaxf(mx, x[k]);
+        }
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) {
+            mn = fminf(mn, __shfl_xor_sync(kFull, mn, off));
+            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
+        }
+    };
+    range();
+    bool bad = mn < -GOFANN_KV_CLAMP || mx > GOFANN_KV_CLAMP;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bad |= x[k] != x[k];
+    if (__any_sync(kFull, bad)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            x[k] = x[k] == x[k] ? fminf(fmaxf(x[k], -GOFANN_KV_CLAMP), GOFANN_KV_CLAMP) : 0.0f;
+        range();
+    }
+    const __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.0f)), hm = __float2half_rn(mn);
+    const float scale = __half2float(hs), m = __half2float(hm);
+    // rint of the quotient: by the reciprocal (off by less than 3e-6 below 16),
+    // unless that is so near a half that the rounded quotient might fall to
+    // the other side
+    const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float t = __fmul_rn(__fsub_rn(x[k], m), inv);
+        code[k] = rintf(t);
+        near |= fabsf(t - code[k]) > 0.49998f;
+    }
+    if (near) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) code[k] = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x[k], m), scale)) : 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const int d = d0 + k;
-        const bool low = kMode == kRotatePairs ? (k & 1) == 0 : d < half;
-        // x_a cos - x_b sin, x_b cos + x_a sin; every step rounded by itself
-        const float a = __fmul_rn(x[k], c[k]), b = __fmul_rn(o[k], s[k]);
-        const float y = low ? __fsub_rn(a, b) : __fadd_rn(a, b);
-        x[k] = d < rotary ? y : x[k];
+        code[k] = fminf(fmaxf(code[k], 0.0f), 15.0f);
+        x[k] = __fadd_rn(__fmul_rn(code[k], scale), m);
     }
+    return static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(hm)) << 16);
 }
 
 // The page words [i] of this thread, and the nibbles of them that the rows
@@ -179,8 +236,8 @@ __device__ __forceinline__ uint32_t value_mask(int i, int lo, int hi)
 // number, then everything else at once.  So all that a block reads is asked
 // for before it is used: page words that are only partly written, the keys
 // that the page holds, the rows.
-template <int D, int kMode>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
+template <int D, int kMode, bool kBf16, int kAppendThreads>
+__global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3) kv_append_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
                                                                    gofann_kv_append_params p, bool q_wide,
                                                                    bool kv_wide)
 {
@@ -271,22 +328,32 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cac
         *reinterpret_cast<float4*>(&low_of[kVectors + part][d]) = make_float4(l[0], l[1], l[2], l[3]);
     }
 
-    // ---- rotate and quantise: a lane group takes a token and its vectors one
-    // after the other (query heads, key, value); where there are fewer tokens
-    // than groups, a token's vectors are dealt out to several groups
+    // ---- rotate and quantise: a group of lanes takes a token, its query
+    // heads, its key and its value; where there are fewer tokens than groups,
+    // several groups share a token's query heads
     const uint32_t group = p.n_heads / cache.n_kv_heads;
-    const int n_q = p.q ? static_cast<int>(group) : 0, kinds = n_q + 2, tokens = hi - lo;
+    const int n_q = p.q ? static_cast<int>(group) : 0, tokens = hi - lo;
     const int vec = threadIdx.x / kLanes, d0 = (threadIdx.x % kLanes) * 8;
     const int share = tokens < kVectors ? kVectors / tokens : 1;  // groups of a token
-    const int kind0 = share > 1 ? vec / tokens : 0;
-    const int step = share > 1 ? tokens : kVectors;
+    const int part = share > 1 ? vec / tokens : 0;
+    const int step = share > 1 ? tokens : kVectors, turns = (n_q + share - 1) / share;
     float high[8], low[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) high[k] = kNegInf, low[k] = -kNegInf;
     for (int t0 = 0; t0 < tokens; t0 += step) {
         const int token = lo + t0 + (share > 1 ? vec % tokens : vec);
-        const bool on = token < hi && kind0 < share;
+        const bool on = token < hi && part < share;
         const int row = first_row + base + (on ? token : lo) - start;
+        const uint4 raw_k = load8(p.k, static_cast<uint64_t>(row) * p.k_stride + head * D + d0, kv_wide);
+        const uint4 raw_v = load8(p.v, static_cast<uint64_t>(row) * p.v_stride + head * D + d0, kv_wide);
+        const uint64_t q_at = static_cast<uint64_t>(row) * p.q_stride + head * group * D + d0;
+        const auto fetch = [&](int kind) {
+            return kind < n_q ? load8(p.q, q_at + static_cast<uint64_t>(kind) * D, q_wide) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        constexpr int kAhead = 2;  // query vectors on their way
+        uint4 next[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) next[a] = fetch(part + a * share);
         float c[8], s[8];
         if (kMode != kRotateNone) {
             int pos = p.positions ? __ldg(p.positions + row) : base + (on ? token : lo);
@@ -296,102 +363,44 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cac
             }
             load_angles<kMode>(p, pos, d0, c, s);
         }
-        const uint64_t q_at = static_cast<uint64_t>(row) * p.q_stride + head * group * D + d0;
-        const uint64_t k_at = static_cast<uint64_t>(row) * p.k_stride + head * D + d0;
-        const uint64_t v_at = static_cast<uint64_t>(row) * p.v_stride + head * D + d0;
-        const auto fetch = [&](int kind) {
-            if (!on || kind >= kinds) return make_uint4(0u, 0u, 0u, 0u);
-            return kind < n_q ? load8(p.q, q_at + static_cast<uint64_t>(kind) * D, q_wide)
-                              : kind == n_q ? load8(p.k, k_at, kv_wide) : load8(p.v, v_at, kv_wide);
-        };
-        constexpr int kAhead = 3;  // vectors on their way
-        uint4 next[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) next[a] = fetch(kind0 + a * share);
-        // every lane of the warp makes the same turns (the shuffles need them)
-        for (int turn = 0; turn * share < kinds; ++turn) {
-            const int kind = kind0 + turn * share;
+        uint16_t* q_out = static_cast<uint16_t*>(p.q_out) + (static_cast<uint64_t>(row) * p.n_heads + head * group) * D + d0;
+        for (int turn = 0; turn < turns; ++turn) {
+            const int kind = part + turn * share;
             const uint4 raw = next[0];
 #pragma unroll
             for (int a = 0; a + 1 < kAhead; ++a) next[a] = next[a + 1];
             next[kAhead - 1] = fetch(kind + kAhead * share);
-            const bool is_q = kind < n_q, is_k = kind == n_q, live = on && kind < kinds;
             float x[8];
-            unpack8(raw, p.dtype, x);
-            if (kMode != kRotateNone) {
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = x[k];
-                // (low_of's row is free until the bounds are written)
-                rotate8<kMode>(p, raw, d0, c, s, low_of[vec], y);
-                if (kind <= n_q) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = y[k];
-                }
-            }
-            if (live && is_q)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.q_out) +
-                                          (static_cast<uint64_t>(row) * p.n_heads + head * group + kind) * D + d0) =
-                    pack8(x, p.dtype);
-            if (__all_sync(kFull, !live || is_q)) continue;
-            // minimum and maximum over the eight lanes of a group of 64
-            float mn, mx;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                x[k] = x[k] == x[k] ? fminf(fmaxf(x[k], -GOFANN_KV_CLAMP), GOFANN_KV_CLAMP) : 0.0f;
-                mn = k ? fminf(mn, x[k]) : x[k];
-                mx = k ? fmaxf(mx, x[k]) : x[k];
-            }
-#pragma unroll
-            for (int off = 1; off < 8; off <<= 1) {
-                mn = fminf(mn, __shfl_xor_sync(kFull, mn, off));
-                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
-            }
-            if (!live || is_q) continue;
-            const __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.0f)), hm = __float2half_rn(mn);
-            const float scale = __half2float(hs), m = __half2float(hm);
-            // rint of the quotient: by the reciprocal, unless that is so near
-            // a half that the rounded quotient might fall to the other side
-            const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-            float code[8];
-            bool near = false;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float t = (x[k] - m) * inv;
-                code[k] = rintf(t);
-                near |= fabsf(t - code[k]) > 0.4995f;
-            }
-            if (near) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) code[k] = scale > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x[k], m), scale)) : 0.0f;
-            }
+            unpack8<kBf16>(raw, x);
+            if (kMode != kRotateNone) rotate8<kMode, kBf16>(p, raw, d0, c, s, low_of[vec], x);
+            if (on && kind < n_q) *reinterpret_cast<uint4*>(q_out + kind * D) = pack8<kBf16>(x);
+        }
+        float x[8], code[8];
+        unpack8<kBf16>(raw_k, x);
+        // (low_of's row is free until the bounds are written)
+        if (kMode != kRotateNone) rotate8<kMode, kBf16>(p, raw_k, d0, c, s, low_of[vec], x);
+        const uint32_t kp_word = quantise8(x, code);
+        const uint64_t kv_out = (static_cast<uint64_t>(row) * cache.n_kv_heads + head) * D + d0;
+        const bool mine = on && part == 0;
+        if (mine) {
             uint32_t c8[2] = {0, 0};
-            float val[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                code[k] = fminf(fmaxf(code[k], 0.0f), 15.0f);
                 c8[k >> 2] |= static_cast<uint32_t>(code[k]) << (8 * (k & 3));
-                val[k] = __fadd_rn(__fmul_rn(code[k], scale), m);
+                high[k] = fmaxf(high[k], x[k]);
+                low[k] = fminf(low[k], x[k]);
             }
-            if (is_k) {
-                *reinterpret_cast<uint2*>(&key_codes[token * kKeyRow + d0]) = make_uint2(c8[0], c8[1]);
+            *reinterpret_cast<uint2*>(&key_codes[token * kKeyRow + d0]) = make_uint2(c8[0], c8[1]);
+            if ((d0 & (kKvGroup - 1)) == 0) params[0][token][d0 / kKvGroup] = kp_word;
+            if (p.k_out) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k_out) + kv_out) = pack8<kBf16>(x);
+        }
+        unpack8<kBf16>(raw_v, x);
+        const uint32_t vp_word = quantise8(x, code);
+        if (mine) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    high[k] = fmaxf(high[k], val[k]);
-                    low[k] = fminf(low[k], val[k]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) value_codes[(d0 + k) * kValueRow + token] = (c8[k >> 2] >> (8 * (k & 3))) & 0xff;
-            }
-            if ((d0 & (kKvGroup - 1)) == 0)
-                params[is_k ? 0 : 1][token][d0 / kKvGroup] = static_cast<uint32_t>(__half_as_ushort(hs)) |
-                                                            (static_cast<uint32_t>(__half_as_ushort(hm)) << 16);
-            void* out = is_k ? p.k_out : p.v_out;
-            if (out)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) +
-                                          (static_cast<uint64_t>(row) * cache.n_kv_heads + head) * D + d0) =
-                    pack8(val, p.dtype);
+            for (int k = 0; k < 8; ++k) value_codes[(d0 + k) * kValueRow + token] = static_cast<uint8_t>(code[k]);
+            if ((d0 & (kKvGroup - 1)) == 0) params[1][token][d0 / kKvGroup] = vp_word;
+            if (p.v_out) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v_out) + kv_out) = pack8<kBf16>(x);
         }
     }
     if (!page_ok) return;
@@ -471,18 +480,39 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(gofann_kv_cac
     if (threadIdx.x == 0) cache.bound_scale[entry] = scale;
 }
 
+template <int D, int kMode, bool kBf16>
+void launch_typed(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_append_params& p,
+                  bool q_wide, bool kv_wide, dim3 grid, cudaStream_t s)
+{
+    // Blocks with a few rows wait for memory most of their time: small ones, so
+    // that more of them fit an SM (96 sequences of one row, 4 heads: 11 us
+    // instead of 14; for 8 blocks there is no difference).
+    if (batch.max_rows <= 8)
+        kv_append_kernel<D, kMode, kBf16, 128><<<grid, 128, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+    else
+        kv_append_kernel<D, kMode, kBf16, 256><<<grid, 256, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+}
+template <int D, int kMode>
+void launch_mode(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_append_params& p,
+                 bool q_wide, bool kv_wide, dim3 grid, cudaStream_t s)
+{
+    if (p.dtype == GOFANN_DTYPE_BF16)
+        launch_typed<D, kMode, true>(cache, batch, p, q_wide, kv_wide, grid, s);
+    else
+        launch_typed<D, kMode, false>(cache, batch, p, q_wide, kv_wide, grid, s);
+}
 template <int D>
 void launch_append(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_append_params& p, int mode,
                    bool q_wide, bool kv_wide, dim3 grid, cudaStream_t s)
 {
     if (mode == kRotateNone)
-        kv_append_kernel<D, kRotateNone><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+        launch_mode<D, kRotateNone>(cache, batch, p, q_wide, kv_wide, grid, s);
     else if (mode == kRotateHalf)
-        kv_append_kernel<D, kRotateHalf><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+        launch_mode<D, kRotateHalf>(cache, batch, p, q_wide, kv_wide, grid, s);
     else if (mode == kRotatePairs)
-        kv_append_kernel<D, kRotatePairs><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+        launch_mode<D, kRotatePairs>(cache, batch, p, q_wide, kv_wide, grid, s);
     else
-        kv_append_kernel<D, kRotateAny><<<grid, kAppendThreads, 0, s>>>(cache, batch, p, q_wide, kv_wide);
+        launch_mode<D, kRotateAny>(cache, batch, p, q_wide, kv_wide, grid, s);
 }
 
 }  // namespace
@@ -532,12 +562,12 @@ int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
     const uint32_t units = static_cast<uint32_t>(bound < batch->n_rows ? bound : batch->n_rows);
     const bool q_wide = (bits(p.q) & 15) == 0 && (p.q_stride & 7) == 0;
     const bool kv_wide = ((bits(p.k) | bits(p.v)) & 15) == 0 && ((p.k_stride | p.v_stride) & 7) == 0;
-    // the two halves of a pair in lanes of their own need whole lanes and
-    // 16-byte table rows; adjacent pairs never cross a lane
+    // whole lanes of eight dimensions and 16-byte table rows, or the general form
+    const bool tables_wide = ((bits(p.cos) | bits(p.sin)) & 15) == 0;
     const int mode = p.rotary_dim == 0 ? kRotateNone
-                     : p.interleaved   ? kRotatePairs
-                     : p.rotary_dim % 16 == 0 && ((bits(p.cos) | bits(p.sin)) & 15) == 0 ? kRotateHalf
-                                                                                         : kRotateAny;
+                     : p.rotary_dim % (p.interleaved ? 8 : 16) || !tables_wide ? kRotateAny
+                     : p.interleaved                                           ? kRotatePairs
+                                                                               : kRotateHalf;
     const dim3 grid(units, cache->n_kv_heads);
     if (d == 64)
         launch_append<64>(*cache, *batch, p, mode, q_wide, kv_wide, grid, as_stream(stream));
