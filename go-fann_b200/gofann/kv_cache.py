@@ -78,22 +78,22 @@ def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, scalin
     return (angle.cos() * m).float(), (angle.sin() * m).float()
 
 
-def _rows(x: torch.Tensor, heads: int, dim: int, dtype, name: str) -> tuple[int, int]:
+def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str) -> tuple[int, int]:
     """Address and row stride of [rows][heads][dim] with contiguous heads."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim:
-        raise ValueError(f"{name} must be [rows][{heads}][{dim}], got {tuple(x.shape)}")
-    if x.dtype != dtype:
+    if x.shape != (rows, heads, dim):
+        raise ValueError(f"{name} must be [{rows} rows][{heads}][{dim}], got {tuple(x.shape)}")
+    if x.dtype is not dtype:
         raise TypeError(f"{name} is {x.dtype}, not {dtype}")
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim):
+    stride = x.stride()
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{name}: the heads of a row must be contiguous")
-    stride = x.stride(0) if x.shape[0] > 1 else heads * dim
-    return x.data_ptr(), stride
+    return x.data_ptr(), stride[0] if rows > 1 else heads * dim
 
 
 def _out(x: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, name: str) -> torch.Tensor:
     if x is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
-    if tuple(x.shape) != shape or x.dtype != dtype or not x.is_contiguous() or x.device != like.device:
+    if x.shape != shape or x.dtype is not dtype or not x.is_contiguous() or x.get_device() != like.get_device():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {like.device}")
     return x
 
@@ -120,19 +120,24 @@ class KVBatch:
         if n_rows < 0 or not 0 <= max_rows <= n_rows:
             raise ValueError(f"n_rows {n_rows} and max_rows {max_rows}")
         self.page_table, self.seq_len, self.row_offset = page_table, seq_len, row_offset
-        self.n_rows, self.max_rows = int(n_rows), int(max_rows)
+        self.n_seqs, self.n_rows, self.max_rows = n_seqs, int(n_rows), int(max_rows)
         self.status = status if status is not None else torch.zeros(1, dtype=torch.int32, device=page_table.device)
         self.struct = A.KvBatch(page_table=page_table.data_ptr(), seq_len=seq_len.data_ptr(),
                                 row_offset=row_offset.data_ptr(), status=self.status.data_ptr(), n_seqs=n_seqs,
                                 max_pages=int(page_table.shape[1]), n_rows=self.n_rows, max_rows=self.max_rows)
         self._ref = C.byref(self.struct)
         self._scratch = None
+        self._needs = {}
 
-    def scratch(self, n_bytes: int) -> int:
-        """Address of at least n_bytes of device scratch (kept, grown on demand)."""
+    def scratch(self, key: tuple, need) -> tuple[int, int]:
+        """Address and size of the device scratch of a call (kept, grown on
+        demand); `need` tells the bytes, once for each `key`, a call's sizes."""
+        n_bytes = self._needs.get(key)
+        if n_bytes is None:
+            n_bytes = self._needs[key] = max(int(need()), 256)
         if self._scratch is None or self._scratch.numel() < n_bytes:
-            self._scratch = torch.empty(max(n_bytes, 256), dtype=torch.uint8, device=self.page_table.device)
-        return self._scratch.data_ptr()
+            self._scratch = torch.empty(n_bytes, dtype=torch.uint8, device=self.page_table.device)
+        return self._scratch.data_ptr(), n_bytes
 
     def check(self) -> None:
         """Raises where a call found a page, position, length or row out of range (synchronises)."""
@@ -165,6 +170,7 @@ class KVCache:
         self.head_dim, self.n_kv_heads, self.n_pages = head_dim, n_kv, n_pages
         self.pages, self.bounds, self.bound_scale = pages, bounds, bound_scale
         self.device = first.device
+        self._index = first.get_device()
         self._lib = A.lib()
         self.struct = A.KvCache(pages=A.ptr(pages), bounds=A.ptr(bounds), bound_scale=A.ptr(bound_scale),
                                 n_pages=n_pages, n_kv_heads=n_kv, head_dim=head_dim)
@@ -179,14 +185,17 @@ class KVCache:
                    bound_scale=torch.zeros((n_pages, n_kv_heads), dtype=torch.float32, device=device))
 
     def _stream(self, stream) -> int:
-        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+        if stream is not None:
+            return stream.cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def _heads(self, q: torch.Tensor) -> int:
-        if q.dim() != 3 or q.shape[1] % self.n_kv_heads:
+        shape = q.shape
+        if len(shape) != 3 or shape[1] % self.n_kv_heads or not shape[1]:
             raise ValueError(f"queries must be [rows][heads][{self.head_dim}] with heads a multiple of {self.n_kv_heads}")
         if q.dtype not in DTYPES:
             raise TypeError(f"queries are {q.dtype}, not bfloat16 or float16")
-        return int(q.shape[1])
+        return shape[1]
 
     def append(self, batch: KVBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos=None, sin=None,
                rotary_dim: int = 0, interleaved: bool = False, positions=None, q_out=None, k_out=None, v_out=None,
@@ -199,36 +208,36 @@ class KVCache:
         dtype = k.dtype
         if dtype not in DTYPES:
             raise TypeError(f"keys are {dtype}, not bfloat16 or float16")
-        p = A.KvAppendParams()
-        p.k, p.k_stride = _rows(k, n_kv, d, dtype, "k")
-        p.v, p.v_stride = _rows(v, n_kv, d, dtype, "v")
-        heads = n_kv
+        k_at, k_stride = _rows(k, n, n_kv, d, dtype, "k")
+        v_at, v_stride = _rows(v, n, n_kv, d, dtype, "v")
+        heads, q_at, q_stride, q_to, k_to, v_to = n_kv, None, 0, None, None, None
         if q is not None:
             heads = self._heads(q)
-            p.q, p.q_stride = _rows(q, heads, d, dtype, "q")
+            q_at, q_stride = _rows(q, n, heads, d, dtype, "q")
             q_out = _out(q_out, (n, heads, d), dtype, k, "q_out")
-            p.q_out = q_out.data_ptr()
-        if any(x is not None and x.shape[0] != n for x in (q, k, v)):
-            raise ValueError(f"q, k and v must have the batch's {n} rows")
+            q_to = q_out.data_ptr()
         if held or k_out is not None:
             k_out = _out(k_out, (n, n_kv, d), dtype, k, "k_out")
-            p.k_out = k_out.data_ptr()
+            k_to = k_out.data_ptr()
         if held or v_out is not None:
             v_out = _out(v_out, (n, n_kv, d), dtype, k, "v_out")
-            p.v_out = v_out.data_ptr()
+            v_to = v_out.data_ptr()
+        cos_at, sin_at, n_positions, positions_at = None, None, 0, None
         if rotary_dim:
-            for t in (cos, sin):
-                if t is None or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
-                        t.shape[1] != rotary_dim // 2 or t.shape != cos.shape:
-                    raise ValueError(f"cos and sin must be contiguous float32 [positions][{rotary_dim // 2}]")
-            p.cos, p.sin, p.n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+            if cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
+                    cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or \
+                    not cos.is_contiguous() or not sin.is_contiguous():
+                raise ValueError(f"cos and sin must be contiguous float32 [positions][{rotary_dim // 2}]")
+            cos_at, sin_at, n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
         if positions is not None:
-            if positions.dtype != torch.int32 or tuple(positions.shape) != (n,) or not positions.is_contiguous():
+            if positions.dtype is not torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
                 raise ValueError("positions must be contiguous int32 [n_rows]")
-            p.positions = positions.data_ptr()
-        p.dtype, p.n_heads = DTYPES[dtype], heads
-        p.rotary_dim, p.interleaved = rotary_dim, int(interleaved)
-        A.check(self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), self._stream(stream)), "gofann_kv_append")
+            positions_at = positions.data_ptr()
+        p = A.KvAppendParams(q_at, k_at, v_at, q_stride, k_stride, v_stride, cos_at, sin_at, positions_at, q_to, k_to,
+                             v_to, DTYPES[dtype], heads, n_positions, rotary_dim, 1 if interleaved else 0)
+        status = self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), self._stream(stream))
+        if status:
+            A.check(status, "gofann_kv_append")
         return q_out if q is not None else None, k_out, v_out
 
     def select(self, batch: KVBatch, q: torch.Tensor, n_select: int, first: int = 1, recent: int = 1, ids=None,
@@ -236,19 +245,17 @@ class KVCache:
         """Blocks that each row and key/value head reads: ids int32 and scores
         f32 [n_rows][n_kv_heads][n_select], ascending blocks, -1 / -inf fill."""
         heads, n = self._heads(q), batch.n_rows
-        p = A.KvSelectParams()
-        p.q, p.q_stride = _rows(q, heads, self.head_dim, q.dtype, "q")
-        if q.shape[0] != n:
-            raise ValueError(f"q must have the batch's {n} rows")
+        at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q")
         shape = (n, self.n_kv_heads, n_select)
         ids = _out(ids, shape, torch.int32, q, "ids")
         scores = _out(scores, shape, torch.float32, q, "scores")
-        p.ids, p.scores = ids.data_ptr(), scores.data_ptr()
-        p.dtype, p.n_heads, p.n_select, p.n_first, p.n_recent = DTYPES[q.dtype], heads, n_select, first, recent
-        ref = C.byref(p)
-        need = self._lib.gofann_kv_select_scratch_bytes(self._ref, batch._ref, ref)
-        A.check(self._lib.gofann_kv_select(self._ref, batch._ref, ref, batch.scratch(need), need, self._stream(stream)),
-                "gofann_kv_select")
+        ref = C.byref(A.KvSelectParams(at, stride, ids.data_ptr(), scores.data_ptr(), DTYPES[q.dtype], heads, n_select,
+                                       first, recent))
+        scratch, size = batch.scratch((0, heads, self.n_kv_heads, self.head_dim, n_select),
+                                      lambda: self._lib.gofann_kv_select_scratch_bytes(self._ref, batch._ref, ref))
+        status = self._lib.gofann_kv_select(self._ref, batch._ref, ref, scratch, size, self._stream(stream))
+        if status:
+            A.check(status, "gofann_kv_select")
         return ids, scores
 
     def attend(self, batch: KVBatch, q: torch.Tensor, scale: float | None = None, causal: bool = True, window: int = 0,
@@ -260,27 +267,26 @@ class KVCache:
         0 hides it (filtered out or evicted).  scale defaults to
         head_dim^-0.5."""
         heads, n, d = self._heads(q), batch.n_rows, self.head_dim
-        p = A.KvAttentionParams()
-        p.q, p.q_stride = _rows(q, heads, d, q.dtype, "q")
-        if q.shape[0] != n:
-            raise ValueError(f"q must have the batch's {n} rows")
+        at, stride = _rows(q, n, heads, d, q.dtype, "q")
         out = _out(out, (n, heads, d), q.dtype, q, "out")
         lse = _out(lse, (n, heads), torch.float32, q, "lse")
-        p.out, p.lse = out.data_ptr(), lse.data_ptr()
+        selected_at, n_select, bits_at, words = None, 0, None, 0
         if selected is not None:
-            if selected.dtype != torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
-                    tuple(selected.shape[:2]) != (n, self.n_kv_heads):
+            if selected.dtype is not torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
+                    selected.shape[:2] != (n, self.n_kv_heads):
                 raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width]")
-            p.selected, p.n_select = selected.data_ptr(), selected.shape[2]
+            selected_at, n_select = selected.data_ptr(), selected.shape[2]
         if key_bits is not None:
-            if key_bits.dtype != torch.int32 or key_bits.dim() != 2 or not key_bits.is_contiguous() or \
-                    key_bits.shape[0] != batch.struct.n_seqs:
+            if key_bits.dtype is not torch.int32 or key_bits.dim() != 2 or not key_bits.is_contiguous() or \
+                    key_bits.shape[0] != batch.n_seqs:
                 raise ValueError("key_bits must be contiguous int32 [n_seqs][words]")
-            p.key_bits, p.key_words = key_bits.data_ptr(), key_bits.shape[1]
-        p.scale = d ** -0.5 if scale is None else scale
-        p.dtype, p.n_heads, p.causal, p.window = DTYPES[q.dtype], heads, int(causal), window
-        ref = C.byref(p)
-        need = self._lib.gofann_kv_attention_scratch_bytes(self._ref, batch._ref, ref)
-        A.check(self._lib.gofann_kv_attention(self._ref, batch._ref, ref, batch.scratch(need), need,
-                                              self._stream(stream)), "gofann_kv_attention")
+            bits_at, words = key_bits.data_ptr(), key_bits.shape[1]
+        ref = C.byref(A.KvAttentionParams(at, stride, selected_at, bits_at, out.data_ptr(), lse.data_ptr(),
+                                          d ** -0.5 if scale is None else scale, DTYPES[q.dtype], heads, n_select, words,
+                                          1 if causal else 0, window))
+        scratch, size = batch.scratch((1, heads, self.n_kv_heads, d, n_select),
+                                      lambda: self._lib.gofann_kv_attention_scratch_bytes(self._ref, batch._ref, ref))
+        status = self._lib.gofann_kv_attention(self._ref, batch._ref, ref, scratch, size, self._stream(stream))
+        if status:
+            A.check(status, "gofann_kv_attention")
         return out, lse
