@@ -32,14 +32,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// (a, b) = (a, b) * f + c, two f32 fmas in one instruction.
-__device__ __forceinline__ void fma_pair(float& a, float& b, const float* f, const float* c)
+// (a, b) += c, two f32 sums in one instruction.
+__device__ __forceinline__ void add_pair(float& a, float& b, const float* c)
 {
-    asm("{\n\t.reg .b64 x, y, z;\n\t"
-        "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 z, {%4, %5};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+    asm("{\n\t.reg .b64 x, y;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
         : "+f"(a), "+f"(b)
-        : "f"(f[0]), "f"(f[1]), "f"(c[0]), "f"(c[1]));
+        : "f"(c[0]), "f"(c[1]));
 }
 // The A operand of 16 rows x 16 steps from one word of eight codes.
 __device__ __forceinline__ void code_operand(uint32_t w, uint32_t (&a)[4])
@@ -74,6 +74,12 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A call's parameters, and the units that every tile counts where that is the
+// same number for all of them (0 = each sequence has its own).
+struct Call : gofann_kv_attention_params {
+    int fixed;
+};
+
 // The query columns that a warp works on at a time: rows of a sequence x
 // query heads of one key/value head.
 struct Tile {
@@ -90,7 +96,7 @@ struct SeqWork {
     int tiles, lo, span;
 };
 template <bool kSelected>
-__device__ __forceinline__ SeqWork seq_work(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group,
+__device__ __forceinline__ SeqWork seq_work(const gofann_kv_batch& b, const Call& p, int group,
                                             int width, uint32_t s)
 {
     int first, n, lo = 0, hi = static_cast<int>(p.n_select);
@@ -104,7 +110,7 @@ __device__ __forceinline__ SeqWork seq_work(const gofann_kv_batch& b, const gofa
         dense_blocks(p, group, kv_len(b, s), n, 0, n * group, lo, hi);
     }
     w.lo = lo;
-    w.span = hi > lo ? hi - lo : 1;
+    w.span = p.fixed ? p.fixed : hi > lo ? hi - lo : 1;
     return w;
 }
 
@@ -123,7 +129,7 @@ struct SeqCursor {
 };
 
 template <bool kSelected>
-__device__ __forceinline__ void make_tile(const gofann_kv_batch& b, const gofann_kv_attention_params& p, int group,
+__device__ __forceinline__ void make_tile(const gofann_kv_batch& b, const Call& p, int group,
                                           int width, uint32_t seq, int at, Tile& tile)
 {
     tile.seq = seq;
@@ -143,7 +149,7 @@ __device__ __forceinline__ void make_tile(const gofann_kv_batch& b, const gofann
 }
 
 template <bool kSelected>
-__device__ __forceinline__ uint64_t total_units(const gofann_kv_batch& b, const gofann_kv_attention_params& p,
+__device__ __forceinline__ uint64_t total_units(const gofann_kv_batch& b, const Call& p,
                                                 uint32_t n_kv, int group, int width)
 {
     return kv_total<uint64_t>(b.n_seqs, [&](uint32_t s) {
@@ -153,7 +159,7 @@ __device__ __forceinline__ uint64_t total_units(const gofann_kv_batch& b, const 
 }
 // The sequence of unit `flat`; false past the end.
 template <bool kSelected>
-__device__ __forceinline__ bool seek(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+__device__ __forceinline__ bool seek(const gofann_kv_batch& b, const Call& p, uint32_t n_kv,
                                      int group, int width, uint64_t flat, SeqCursor& c)
 {
     uint64_t at;
@@ -169,9 +175,41 @@ __device__ __forceinline__ bool seek(const gofann_kv_batch& b, const gofann_kv_a
     c.span = w.span;
     return true;
 }
+// The sequence of the unit that `place` names once it knows the number of all
+// units; false where it names one past the end.
+template <bool kSelected, class F>
+__device__ __forceinline__ bool seek_by_total(const gofann_kv_batch& b, const Call& p, uint32_t n_kv, int group, int width,
+                                              F place, SeqCursor& c)
+{
+    if (b.n_seqs > 32) {
+        const uint64_t flat = place(total_units<kSelected>(b, p, n_kv, group, width));
+        return seek<kSelected>(b, p, n_kv, group, width, flat, c);
+    }
+    // one look at the sequences is enough
+    const int lane = threadIdx.x & 31;
+    SeqWork w{0, 0, 1};
+    if (lane < static_cast<int>(b.n_seqs)) w = seq_work<kSelected>(b, p, group, width, lane);
+    const uint64_t units = static_cast<uint64_t>(w.tiles) * n_kv * w.span;
+    uint64_t upto = units;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t v = __shfl_up_sync(kFull, upto, off);
+        if (lane >= off) upto += v;
+    }
+    const uint64_t flat = place(__shfl_sync(kFull, upto, 31));
+    const unsigned past = __ballot_sync(kFull, flat < upto);
+    if (!past) return false;
+    const int l = __ffs(past) - 1;
+    c.seq = l;
+    c.end = __shfl_sync(kFull, upto, l);
+    c.begin = c.end - __shfl_sync(kFull, units, l);
+    c.lo = __shfl_sync(kFull, w.lo, l);
+    c.span = __shfl_sync(kFull, w.span, l);
+    return true;
+}
 // The next sequence that has units (the caller knows that there is one).
 template <bool kSelected>
-__device__ __forceinline__ void next_sequence(const gofann_kv_batch& b, const gofann_kv_attention_params& p,
+__device__ __forceinline__ void next_sequence(const gofann_kv_batch& b, const Call& p,
                                               uint32_t n_kv, int group, int width, SeqCursor& c)
 {
     while (c.seq + 1 < b.n_seqs) {
@@ -185,7 +223,7 @@ __device__ __forceinline__ void next_sequence(const gofann_kv_batch& b, const go
     }
 }
 template <bool kSelected>
-__device__ __forceinline__ void make_item(const gofann_kv_batch& b, const gofann_kv_attention_params& p, uint32_t n_kv,
+__device__ __forceinline__ void make_item(const gofann_kv_batch& b, const Call& p, uint32_t n_kv,
                                           int group, int width, uint64_t flat, const SeqCursor& c, Item& item)
 {
     const uint64_t i = (flat - c.begin) / c.span;
@@ -197,12 +235,15 @@ __device__ __forceinline__ void make_item(const gofann_kv_batch& b, const gofann
 
 // Running softmax state of one warp for columns 2t, 2t + 1 of each 8-column
 // tile and dimensions 16 dt + g, + 8.  All sums are in units of the weights
-// 2^(logit - base), base = max - (26 - e) in log2 units: e is the largest
-// exponent of a value scale so far, so the products weight * scale stay below
-// 2^12 and f16 holds them down to 2^-24 whatever the values' magnitude.
+// 2^(logit - base), base = reference - (kUp - e) in log2 units: e is the
+// largest exponent of a value scale so far, so the products weight * scale are
+// below 2^8 at the reference, below 2^15 where a logit is kLag above it, and
+// f16 holds them down to 2^-24 whatever the values' magnitude.
+constexpr int kUp = 22;
+constexpr float kLag = 7.0f;
 template <int D, int NT>
 struct State {
-    float m[NT][2];                      // largest logit, in the query column's own unit
+    float m[NT][2];                      // reference, in the query column's own unit
     float l[NT][2];                      // this lane's part of the sum of weights
     float z[NT][2][KvChunk<D>::kGroups]; // this lane's part of sum w * (minimum + 8 scale)
     float o[D / 16][NT][4];              // sum (w * scale) * (code - 8) * 2^-24
@@ -235,7 +276,7 @@ __device__ __forceinline__ void clear(State<D, NT>& st)
 template <int D, int NT>
 struct Query {
     uint32_t b[D / 16][NT][2];
-    float unit[NT][2];
+    float unit[NT][2], lag[NT][2];          // lag: kLag in the column's unit
     float sum[NT][2][KvChunk<D>::kGroups];  // sum of the column over a group
     int limit[NT][2], low[NT][2];           // keys seen: low < key <= limit
 };
@@ -328,27 +369,53 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
             top = __hmax2(top, *reinterpret_cast<const __half2*>(&w[k]));
         }
     }
-    const uint32_t top_bits = *reinterpret_cast<const uint32_t*>(&top) & 0x7c00u;
-    const int e = max(st.e, static_cast<int>(__reduce_max_sync(kFull, top_bits) >> 10));
-    const float shift = static_cast<float>(e - st.e), up = static_cast<float>(26 - e);
-    st.e = e;
-    float rescale[NT][2];
+    const int e_here = static_cast<int>((*reinterpret_cast<const uint32_t*>(&top) & 0x7c00u) >> 10);
+
+    // ---- the reference of the weights: it moves only where a score is kLag
+    // above it, there is none yet, or a value scale has a larger exponent
+    float local[NT][2];
+    bool far = e_here > st.e;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            float mx = st.m[n][c];
+            float mx = fmaxf(s[0][n][c], s[0][n][2 + c]);
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(s[kt][n][c], s[kt][n][2 + c]));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-            const float use = mx == kNegInf ? 0.0f : mx, unit = q.unit[n][c];
-            const float f = exp2_fast(fmaf(st.m[n][c] - use, unit, -shift));
-            const float base = fmaf(use, unit, -up);
-            st.m[n][c] = mx;
-            rescale[n][c] = f;
-            float l = st.l[n][c] * f;
+            for (int kt = 1; kt < 4; ++kt) mx = fmaxf(mx, fmaxf(s[kt][n][c], s[kt][n][2 + c]));
+            local[n][c] = mx;
+            far |= mx > st.m[n][c] + q.lag[n][c];
+        }
+    if (__any_sync(kFull, far)) {
+        const int e = max(st.e, static_cast<int>(__reduce_max_sync(kFull, static_cast<unsigned>(e_here))));
+        const float shift = static_cast<float>(e - st.e);
+        st.e = e;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float mx = fmaxf(local[n][c], st.m[n][c]);
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+                const float use = mx == kNegInf ? 0.0f : mx;
+                const float f = exp2_fast(fmaf(st.m[n][c] - use, q.unit[n][c], -shift));
+                st.m[n][c] = mx;
+                st.l[n][c] *= f;
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] *= f;
+#pragma unroll
+                for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) st.o[dt][n][2 * r + c] *= f;
+            }
+    }
+    const float up = static_cast<float>(kUp - st.e);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float unit = q.unit[n][c], base = fmaf(st.m[n][c] == kNegInf ? 0.0f : st.m[n][c], unit, -up);
+            float l = st.l[n][c];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -358,15 +425,13 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
                     l += x;
                 }
             st.l[n][c] = l;
-#pragma unroll
-            for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] *= f;
         }
 
     // ---- weighted values.  The matrix instruction truncates its sums, so a
     // long chain of the codes' one-sided products would drift: codes are
     // centred (8 times the sum of the weights is taken off by the same
     // instruction on a constant operand) and a page's sum joins the running
-    // one by an f32 fma that also rescales it.
+    // one by an f32 addition.
     const uint32_t eight[4] = {0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u};  // -8 * 2^-24, -8 * 2^-20
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -408,13 +473,13 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 4; k += 2) fma_pair(st.o[dt][n][k], st.o[dt][n][k + 1], rescale[n], acc[n] + k);
+                for (int k = 0; k < 4; k += 2) add_pair(st.o[dt][n][k], st.o[dt][n][k + 1], acc[n] + k);
         }
     }
 }
 
 template <int D, int NT>
-__device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head,
+__device__ __forceinline__ void load_query(const Call& p, const Tile& tile, uint32_t head,
                                            int group, bool selected, bool wide, Query<D, NT>& q)
 {
     constexpr int G = KvChunk<D>::kGroups;
@@ -478,6 +543,7 @@ __device__ __forceinline__ void load_query(const gofann_kv_attention_params& p, 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             q.unit[n][e] = __shfl_sync(kFull, undo, 4 * (2 * t + e));
+            q.lag[n][e] = fminf(kLag / q.unit[n][e], FLT_MAX);
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) q.sum[n][e][grp] = __shfl_sync(kFull, sum[grp], 4 * (2 * t + e));
             const int cc = n * 8 + 2 * t + e;
@@ -533,9 +599,11 @@ struct Attend {
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
 };
 
-// Units of one block: a share of the total, at least one per warp.
-__device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks, int warps)
+// Units of one block: a share of the total, at least one per warp, and whole
+// items where all count the same (then no item has to be joined).
+__device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks, int warps, int fixed)
 {
+    if (fixed) return (total / fixed + blocks - 1) / blocks * fixed;
     const uint64_t c = (total + blocks - 1) / blocks;
     return c > warps ? c : warps;
 }
@@ -546,7 +614,7 @@ template <int D, int NT>
 constexpr size_t kPartFloats = 8 * NT * (D + 2);
 
 template <int D>
-__device__ __forceinline__ void store_row(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head, int group,
+__device__ __forceinline__ void store_row(const Call& p, const Tile& tile, uint32_t head, int group,
                                           bool selected, int c, int d, float m, float l, const float (&o)[4])
 {
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -562,7 +630,7 @@ __device__ __forceinline__ void store_row(const gofann_kv_attention_params& p, c
 // The rows of a whole item from the lanes that hold them: pairs of columns
 // become pairs of dimensions by the transposition that P takes.
 template <int D, int NT, bool kSelected>
-__device__ __forceinline__ void store_item(const gofann_kv_attention_params& p, const Tile& tile, uint32_t head, int group,
+__device__ __forceinline__ void store_item(const Call& p, const Tile& tile, uint32_t head, int group,
                                            const State<D, NT>& st)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -605,7 +673,7 @@ struct Batch32 {
 
 template <int D, int NT, bool kSelected>
 __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofann_kv_batch& b,
-                                        const gofann_kv_attention_params& p, int group, uint64_t flat0, uint64_t end,
+                                        const Call& p, int group, uint64_t flat0, uint64_t end,
                                         SeqCursor& c, Batch32& got)
 {
     constexpr int kCols = 8 * NT;
@@ -654,7 +722,7 @@ __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofa
 template <int D, int NT, bool kSelected>
 __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(gofann_kv_cache cache,
                                                                                gofann_kv_batch batch,
-                                                                               gofann_kv_attention_params p, bool wide,
+                                                                               Call p, bool wide,
                                                                                float* __restrict__ parts)
 {
     using Cfg = Attend<D, NT>;
@@ -676,19 +744,28 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     launch_next();
     if (lane < 2) mine.part[lane].end = 0;
     __syncwarp();
-    const uint64_t total = total_units<kSelected>(batch, p, n_kv, group, kCols);
-    const uint64_t share = units_per_block(total, gridDim.x, kWarps);
-    const uint64_t u0 = share * blockIdx.x, u1 = u0 + share < total ? u0 + share : total;
+    uint64_t u0 = 0, u1 = 0, w0 = 0, w1 = 0;  // units of the block, of the warp
+    SeqCursor from;
+    seek_by_total<kSelected>(
+        batch, p, n_kv, group, kCols,
+        [&](uint64_t total) {
+            const uint64_t share = units_per_block(total, gridDim.x, kWarps, p.fixed);
+            u0 = share * blockIdx.x;
+            u1 = u0 + share < total ? u0 + share : total;
+            if (u0 >= u1) return ~0ull;
+            const uint64_t per_warp = (u1 - u0 + kWarps - 1) / kWarps;
+            w0 = u0 + warp * per_warp;
+            w1 = w0 + per_warp < u1 ? w0 + per_warp : u1;
+            return static_cast<unsigned long long>(w0 < w1 ? w0 : ~0ull);
+        },
+        from);
     if (u0 >= u1) return;
-    const uint64_t per_warp = (u1 - u0 + kWarps - 1) / kWarps;
-    const uint64_t w0 = u0 + warp * per_warp, w1 = w0 + per_warp < u1 ? w0 + per_warp : u1;
 
     bool alive = true;  // false once a wait has run out
     if (w0 < w1) {
         Batch32 now, then;
         {
-            SeqCursor c;
-            seek<kSelected>(batch, p, n_kv, group, kCols, w0, c);
+            SeqCursor c = from;
             if (lane == 0) mine.here = c;
             look_up<D, NT, kSelected>(cache, batch, p, group, w0, w1, c, now);
             if (lane == 0) mine.ahead = c;
@@ -823,7 +900,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
                         for (int grp = 0; grp < G; ++grp) st.z[n][c][grp] += __shfl_xor_sync(kFull, st.z[n][c][grp], off);
                     }
                     // the maximum becomes the base of the weights, in log2 units
-                    st.m[n][c] = st.l[n][c] > 0.0f ? fmaf(st.m[n][c], q.unit[n][c], static_cast<float>(st.e - 26)) : kNegInf;
+                    st.m[n][c] = st.l[n][c] > 0.0f ? fmaf(st.m[n][c], q.unit[n][c], static_cast<float>(st.e - kUp)) : kNegInf;
 #pragma unroll
                     for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
@@ -909,44 +986,76 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     }
 }
 
-// Items that several blocks share: their partial results in block order, so
-// that the sum does not depend on which block was done first.
+// Items that several blocks share.  The factors of the partial results first,
+// then their weighted sum in block order, all loads side by side; the sum does
+// not depend on which block was done first.
+constexpr int kMaxBlocks = 192, kJoinThreads = 256;
 template <int D, int NT, bool kSelected>
-__global__ void __launch_bounds__(128) kv_join_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
-                                                      gofann_kv_attention_params p, uint32_t blocks,
-                                                      const float* __restrict__ parts)
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(gofann_kv_cache cache, gofann_kv_batch batch, Call p,
+                                                               uint32_t blocks, const float* __restrict__ parts)
 {
     constexpr int kCols = 8 * NT;
+    __shared__ float factor[kMaxBlocks][kCols], total_of[kCols], base_of[kCols];
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
     const uint32_t n_kv = cache.n_kv_heads;
-    const uint64_t total = total_units<kSelected>(batch, p, n_kv, group, kCols);
-    const uint64_t share = units_per_block(total, blocks, Attend<D, NT>::kWarps);
     // block i joins the item that the end of share i cuts, if that is the item's first cut
-    const uint64_t cut = share * (blockIdx.x + 1);
+    uint64_t share = 0, cut = 0;
     SeqCursor c;
+    const bool any = seek_by_total<kSelected>(
+        batch, p, n_kv, group, kCols,
+        [&](uint64_t total) {
+            share = units_per_block(total, blocks, Attend<D, NT>::kWarps, 0);
+            cut = share * (blockIdx.x + 1);
+            return static_cast<unsigned long long>(cut < total ? cut : ~0ull);
+        },
+        c);
+    if (!any) return;
     Item item;
-    if (cut >= total || !seek<kSelected>(batch, p, n_kv, group, kCols, cut, c)) return;
     make_item<kSelected>(batch, p, n_kv, group, kCols, cut, c, item);
     if (item.begin >= cut || item.begin < share * blockIdx.x) return;
+    const uint64_t first = blockIdx.x;
+    const int count = static_cast<int>((item.end - 1) / share - first) + 1;
+    const auto part_at = [&](int b) {
+        return parts + (2 * (first + b) + (item.begin <= share * (first + b) ? 0 : 1)) * kPartFloats<D, NT>;
+    };
     wait_previous();
-    const uint64_t first = blockIdx.x, last = (item.end - 1) / share;
-    for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += 128) {
-        const int col = i / (D / 4), d = i % (D / 4) * 4;
-        float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint64_t b = first; b <= last; ++b) {
-            const float* part = parts + (2 * b + (item.begin <= share * b ? 0 : 1)) * kPartFloats<D, NT>;
-            const float pm = __ldcg(part + col), pl = __ldcg(part + kCols + col);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * kCols + col * D + d));
-            const float top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
-            const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
-            l = l * f + pl * h;
-            o[0] = o[0] * f + v.x * h;
-            o[1] = o[1] * f + v.y * h;
-            o[2] = o[2] * f + v.z * h;
-            o[3] = o[3] * f + v.w * h;
-            m = top;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int col = warp; col < item.tile.cols; col += kJoinThreads / 32) {
+        float m = kNegInf, l = 0.0f;
+        for (int b = lane; b < count; b += 32) {
+            const float x = __ldcg(part_at(b) + col);
+            factor[b][col] = x;
+            m = fmaxf(m, x);
         }
-        store_row<D>(p, item.tile, item.head, group, kSelected, col, d, m, l, o);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, off));
+        const float base = m == kNegInf ? 0.0f : m;
+        for (int b = lane; b < count; b += 32) {
+            const float f = exp2_fast(factor[b][col] - base);
+            factor[b][col] = f;
+            l = fmaf(__ldcg(part_at(b) + kCols + col), f, l);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(kFull, l, off);
+        if (lane == 0) {
+            base_of[col] = base;
+            total_of[col] = l;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += kJoinThreads) {
+        const int col = i / (D / 4), d = i % (D / 4) * 4;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int b = 0; b < count; ++b) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(b) + 2 * kCols + col * D + d));
+            const float f = factor[b][col];
+            o[0] = fmaf(v.x, f, o[0]);
+            o[1] = fmaf(v.y, f, o[1]);
+            o[2] = fmaf(v.z, f, o[2]);
+            o[3] = fmaf(v.w, f, o[3]);
+        }
+        store_row<D>(p, item.tile, item.head, group, kSelected, col, d, base_of[col], total_of[col], o);
     }
 }
 
@@ -959,22 +1068,31 @@ bool many_columns(const gofann_kv_cache& cache, const gofann_kv_batch& batch, co
            static_cast<uint64_t>(batch.max_rows) * (p.n_heads / cache.n_kv_heads) >= kManyColumns;
 }
 
-// Thread blocks of the attention kernel: one per SM (the ring takes most of
-// its shared memory), no more than there can be units.
-uint32_t attend_blocks(const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
+// Cache blocks that an item can have at most.
+uint64_t most_blocks(const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
 {
     const uint64_t span = p.selected ? p.n_select : batch.max_pages;
-    const uint64_t most = static_cast<uint64_t>(batch.n_rows) * p.n_heads * (span ? span : 1);
-    const int sms = sm_count();
+    return span ? span : 1;
+}
+
+// Thread blocks of the attention kernel: one per SM (the ring takes most of
+// its shared memory), no more than there can be units (items, where each is
+// done by one block).
+uint32_t attend_blocks(const gofann_kv_batch& batch, const Call& p)
+{
+    const uint64_t most = static_cast<uint64_t>(batch.n_rows) * p.n_heads * (p.fixed ? 1 : most_blocks(batch, p));
+    const int sms = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
     const uint64_t want = sms > 0 ? sms : 1;
     return static_cast<uint32_t>(most < want ? most : want);
 }
 
 template <int D, int NT, bool kSelected>
-int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
-                  float* parts, cudaStream_t s)
+int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, Call p, float* parts, cudaStream_t s)
 {
     using Cfg = Attend<D, NT>;
+    // Items of at most two pages a warp stay in one block: what a split would
+    // gain, the joining kernel would cost.
+    p.fixed = most_blocks(batch, p) <= 2 * Cfg::kWarps ? static_cast<int>(most_blocks(batch, p)) : 0;
     auto* kernel = kv_attend_kernel<D, NT, kSelected>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kBytes));
     if (e != cudaSuccess) return cuda_status(e, "kv_attention: shared memory attribute");
@@ -983,10 +1101,10 @@ int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, co
     const uint32_t blocks = attend_blocks(batch, p);
     kernel<<<blocks, Cfg::kThreads, Cfg::kBytes, s>>>(cache, batch, p, wide, parts);
     GOFANN_CHECK_LAUNCH("kv_attend_kernel");
-    if (blocks == 1) return GOFANN_OK;
+    if (blocks == 1 || p.fixed) return GOFANN_OK;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks - 1);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1019,7 +1137,9 @@ int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* bat
                         const gofann_kv_attention_params* params, void* scratch, size_t scratch_bytes, void* stream)
 {
     if (!params) return fail(GOFANN_ERR_INVALID, "kv_attention: null descriptor");
-    const gofann_kv_attention_params& p = *params;
+    Call p;
+    static_cast<gofann_kv_attention_params&>(p) = *params;
+    p.fixed = 0;
     int st = kv_check("kv_attention", cache, batch, p.dtype, p.n_heads);
     if (st != GOFANN_OK) return st;
     const uint32_t d = cache->head_dim;
