@@ -222,15 +222,21 @@ __device__ __forceinline__ void next_sequence(const gofann_kv_batch& b, const Ca
         return;
     }
 }
+// a / b: 64-bit numbers take a routine, most are short.
+__device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b)
+{
+    return a >> 32 ? a / b : static_cast<uint32_t>(a) / b;
+}
+
 template <bool kSelected>
 __device__ __forceinline__ void make_item(const gofann_kv_batch& b, const Call& p, uint32_t n_kv,
                                           int group, int width, uint64_t flat, const SeqCursor& c, Item& item)
 {
-    const uint64_t i = (flat - c.begin) / c.span;
+    const uint64_t i = divide(flat - c.begin, c.span), tile = divide(i, n_kv);
     item.begin = c.begin + i * c.span;
     item.end = item.begin + c.span;
-    item.head = static_cast<uint32_t>(i % n_kv);
-    make_tile<kSelected>(b, p, group, width, c.seq, static_cast<int>(i / n_kv), item.tile);
+    item.head = static_cast<uint32_t>(i - tile * n_kv);
+    make_tile<kSelected>(b, p, group, width, c.seq, static_cast<int>(tile), item.tile);
 }
 
 // Running softmax state of one warp for columns 2t, 2t + 1 of each 8-column
@@ -282,9 +288,10 @@ struct Query {
 };
 
 // Scores of a page's 64 tokens x 8 NT columns from the key half of a chunk.
-// This lane's tokens are first + 2 i, i = 0 .. 7.  kMasked: some token of
-// the page is hidden from some column; `shown` has a bit per token.
-template <int D, int NT, bool kMasked>
+// This lane's tokens are first + 2 i, i = 0 .. 7.  kMask: 0 = every column
+// sees every token, 1 = every column sees the tokens whose bit `shown` has,
+// 2 = each column has limits of its own too.
+template <int D, int NT, int kMask>
 __device__ __forceinline__ void page_scores(const unsigned char* keys, const Query<D, NT>& q, int key0, uint64_t shown,
                                             float (&s)[4][NT][4])
 {
@@ -329,31 +336,32 @@ __device__ __forceinline__ void page_scores(const unsigned char* keys, const Que
                 }
         }
     }
-    if constexpr (kMasked) {
+    if constexpr (kMask > 0) {
         const int first = 16 * (g >> 1) + (g & 1);
+        const uint32_t mine = static_cast<uint32_t>(shown >> first);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int token = first + 4 * kt + 2 * r, key = key0 + token;
-                const bool on = (shown >> token) & 1;
+                const bool on = (mine >> (4 * kt + 2 * r)) & 1;
+                const int key = key0 + first + 4 * kt + 2 * r;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
-                        if (!on || key > q.limit[n][c] || key <= q.low[n][c]) s[kt][n][2 * r + c] = kNegInf;
+                        if (!on || (kMask == 2 && (key > q.limit[n][c] || key <= q.low[n][c]))) s[kt][n][2 * r + c] = kNegInf;
             }
     }
 }
 
 // Softmax update and weighted values from the value half of a chunk.
-template <int D, int NT, bool kMasked>
+template <int D, int NT, int kMask>
 __device__ __forceinline__ void page_values(const unsigned char* values, const Query<D, NT>& q, uint64_t shown,
                                             float (&s)[4][NT][4], State<D, NT>& st)
 {
     constexpr int G = KvChunk<D>::kGroups, kAt = KvChunk<D>::kCodes;
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    const int first = 16 * (g >> 1) + (g & 1);
+    const uint32_t mine = static_cast<uint32_t>(shown >> (16 * (g >> 1) + (g & 1)));
 
     // ---- the largest value scale; a hidden token's params may be anything,
     // so they count as 0 here and below
@@ -365,7 +373,7 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
         load_words<4>(reinterpret_cast<const unsigned char*>(params + 4 * i), w);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (kMasked && !((shown >> (first + 2 * ((4 * i + k) / G))) & 1)) w[k] = 0;
+            if (kMask > 0 && !((mine >> (2 * ((4 * i + k) / G))) & 1)) w[k] = 0;
             top = __hmax2(top, *reinterpret_cast<const __half2*>(&w[k]));
         }
     }
@@ -443,7 +451,7 @@ __device__ __forceinline__ void page_values(const unsigned char* values, const Q
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 uint32_t w = params[(2 * kt + r) * G + grp];
-                if (kMasked && !((shown >> (first + 4 * kt + 2 * r)) & 1)) w = 0;
+                if (kMask > 0 && !((mine >> (4 * kt + 2 * r)) & 1)) w = 0;
                 const float2 sm = both_halves(w);
                 const float vs = r ? sm.x * 0.0625f : sm.x, vm = fmaf(8.0f, sm.x, sm.y);
 #pragma unroll
@@ -603,8 +611,8 @@ struct Attend {
 // items where all count the same (then no item has to be joined).
 __device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blocks, int warps, int fixed)
 {
-    if (fixed) return (total / fixed + blocks - 1) / blocks * fixed;
-    const uint64_t c = (total + blocks - 1) / blocks;
+    if (fixed) return divide(divide(total, fixed) + blocks - 1, blocks) * fixed;
+    const uint64_t c = divide(total + blocks - 1, blocks);
     return c > warps ? c : warps;
 }
 
@@ -685,11 +693,11 @@ __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofa
     while (true) {
         if (todo && flat < c.end) {
             todo = false;
-            const uint64_t at = flat - c.begin, i = at / c.span;
-            const uint32_t head = static_cast<uint32_t>(i % n_kv);
+            const uint64_t at = flat - c.begin, i = divide(at, c.span), tile_at = divide(i, n_kv);
+            const uint32_t head = static_cast<uint32_t>(i - tile_at * n_kv);
             int block = c.lo + static_cast<int>(at - i * c.span);
             Tile tile;
-            make_tile<kSelected>(b, p, group, kCols, c.seq, static_cast<int>(i / n_kv), tile);
+            make_tile<kSelected>(b, p, group, kCols, c.seq, static_cast<int>(tile_at), tile);
             bool on = true;
             if (kSelected) {
                 block = __ldg(p.selected +
@@ -753,7 +761,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
             u0 = share * blockIdx.x;
             u1 = u0 + share < total ? u0 + share : total;
             if (u0 >= u1) return ~0ull;
-            const uint64_t per_warp = (u1 - u0 + kWarps - 1) / kWarps;
+            const uint64_t per_warp = divide(u1 - u0 + kWarps - 1, kWarps);
             w0 = u0 + warp * per_warp;
             w1 = w0 + per_warp < u1 ? w0 + per_warp : u1;
             return static_cast<unsigned long long>(w0 < w1 ? w0 : ~0ull);
@@ -832,16 +840,23 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
             const uint64_t start = flat, stop = item.end < w1 ? item.end : w1;
             Query<D, NT> q;
             load_query<D, NT>(p, tile, item.head, group, kSelected, wide, q);
-            int limit = 0x7fffffff, low = -1;  // keys in (low, limit] are seen by every column
+            // keys in (low, limit] are seen by every column; `alike`: by the
+            // same token, no column sees another key
+            int limit = 0x7fffffff, low = -1, limit_most = -1, low_least = 0x7fffffff;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     limit = min(limit, q.limit[n][e]);
                     low = max(low, q.low[n][e]);
+                    if (n * 8 + 2 * t + e < tile.cols) {
+                        limit_most = max(limit_most, q.limit[n][e]);
+                        low_least = min(low_least, q.low[n][e]);
+                    }
                 }
             limit = __reduce_min_sync(kFull, limit);
             low = __reduce_max_sync(kFull, low);
+            const bool alike = limit == __reduce_max_sync(kFull, limit_most) && low == __reduce_min_sync(kFull, low_least);
             State<D, NT> st;
             clear(st);
             const uint32_t seq = tile.seq;
@@ -867,23 +882,35 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
                 }
                 if (!((now.valid >> l) & 1) || !alive) continue;
                 const int block = __shfl_sync(kFull, now.block, l), key0 = block * kKvPage;
-                const uint64_t shown = shown_tokens(p, seq, len, block);
-                const bool masked = shown != ~0ull || key0 + kKvPage - 1 > limit || key0 <= low;
+                uint64_t shown = shown_tokens(p, seq, len, block);
+                const bool edge = key0 + kKvPage - 1 > limit || key0 <= low;
+                if (edge && alike) {
+                    const int a = limit - key0, b = low - key0;
+                    shown &= a < 0 ? 0ull : a >= 63 ? ~0ull : (2ull << a) - 1;
+                    shown &= b < 0 ? ~0ull : b >= 63 ? 0ull : ~((2ull << b) - 1);
+                }
+                const int mask = edge && !alike ? 2 : shown != ~0ull ? 1 : 0;
                 float s[4][NT][4];
                 alive = take();
                 if (!alive) continue;
-                if (masked)
-                    page_scores<D, NT, true>(ring + out.slot * kHalf, q, key0, shown, s);
-                else
-                    page_scores<D, NT, false>(ring + out.slot * kHalf, q, key0, shown, s);
+                if (shown != 0) {
+                    if (mask == 0)
+                        page_scores<D, NT, 0>(ring + out.slot * kHalf, q, key0, shown, s);
+                    else if (mask == 1)
+                        page_scores<D, NT, 1>(ring + out.slot * kHalf, q, key0, shown, s);
+                    else
+                        page_scores<D, NT, 2>(ring + out.slot * kHalf, q, key0, shown, s);
+                }
                 release();
                 fill();
                 alive = take();
                 if (!alive) continue;
-                if (masked)
-                    page_values<D, NT, true>(ring + out.slot * kHalf, q, shown, s, st);
-                else
-                    page_values<D, NT, false>(ring + out.slot * kHalf, q, shown, s, st);
+                if (shown != 0) {
+                    if (mask == 0)
+                        page_values<D, NT, 0>(ring + out.slot * kHalf, q, shown, s, st);
+                    else
+                        page_values<D, NT, 1>(ring + out.slot * kHalf, q, shown, s, st);
+                }
                 release();
                 fill();
             }
