@@ -602,8 +602,9 @@ struct Attend {
     static constexpr size_t kRing = static_cast<size_t>(kWarps) * kSlots * kHalf;
     static constexpr size_t kFirst = sizeof(float) * kWarps * kPart;
     static constexpr size_t kItems = sizeof(WarpItems) * kWarps;
-    static constexpr size_t kBytes = kRing + kFirst + kItems + sizeof(uint64_t) * kWarps * kSlots;
-    static_assert(sizeof(float) * kPart <= kSlots * kHalf, "a warp's last partial result takes its ring's place");
+    static constexpr size_t kFactors = sizeof(float) * kCols * 34;
+    static constexpr size_t kBytes = kRing + kFirst + kItems + kFactors + sizeof(uint64_t) * kWarps * kSlots;
+    static_assert(2 * kWarps <= 32 && sizeof(float) * kPart <= kSlots * kHalf, "a warp's last partial result takes its ring's place");
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
 };
 
@@ -743,7 +744,8 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
     const auto last_part = [&](int w) { return reinterpret_cast<float*>(smem + static_cast<size_t>(w) * kSlots * kHalf); };
     WarpItems* warp_items = reinterpret_cast<WarpItems*>(smem + Cfg::kRing + Cfg::kFirst);
     WarpItems& mine = warp_items[warp];
-    const uint32_t bars = shared_addr(smem + Cfg::kRing + Cfg::kFirst + Cfg::kItems) + warp * kSlots * 8;
+    float* factors = reinterpret_cast<float*>(smem + Cfg::kRing + Cfg::kFirst + Cfg::kItems);  // [cols][32], max, sum
+    const uint32_t bars = shared_addr(smem + Cfg::kRing + Cfg::kFirst + Cfg::kItems + Cfg::kFactors) + warp * kSlots * 8;
     const int group = static_cast<int>(p.n_heads / cache.n_kv_heads);
     const uint32_t n_kv = cache.n_kv_heads;
 
@@ -775,6 +777,15 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
         {
             SeqCursor c = from;
             if (lane == 0) mine.here = c;
+            // the first item's queries come while the pages are looked up
+            Item item;
+            make_item<kSelected>(batch, p, n_kv, group, kCols, w0, c, item);
+            if (lane < item.tile.cols * 2) {
+                const int col = item.tile.col0 + lane / 2;
+                const int row = item.tile.first_row + (kSelected ? item.tile.row : col / group);
+                prefetch_l1(static_cast<const uint16_t*>(p.q) + static_cast<uint64_t>(row) * p.q_stride +
+                            static_cast<uint64_t>(item.head * group + (kSelected ? col : col % group)) * D + (lane & 1) * (D / 2));
+            }
             look_up<D, NT, kSelected>(cache, batch, p, group, w0, w1, c, now);
             if (lane == 0) mine.ahead = c;
             __syncwarp();
@@ -971,45 +982,64 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
 
     // ---- join the warps' partial results of each item, in unit order: the
     // rows where the block has the whole item, else a partial result for the
-    // joining kernel
-    const auto part_item = [&](int e) -> const Item& { return warp_items[e >> 1].part[e & 1]; };
-    for (int e0 = 0; e0 < 2 * kWarps;) {
-        if (part_item(e0).end == 0) {
-            ++e0;
-            continue;
-        }
-        const Item item = part_item(e0);
-        int e1 = e0 + 1;
-        while (e1 < 2 * kWarps && (part_item(e1).end == 0 || part_item(e1).begin == item.begin)) ++e1;
-        const bool whole = item.begin >= u0 && item.end <= u1;
-        float* out = parts + (2ull * blockIdx.x + (item.begin <= u0 ? 0 : 1)) * kPartFloats<D, NT>;
-        for (int i = threadIdx.x; i < item.tile.cols * (D / 4); i += Cfg::kThreads) {
-            const int c = i / (D / 4), d = i % (D / 4) * 4;
-            float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int e = e0; e < e1; ++e) {
-                if (part_item(e).end == 0) continue;
-                const float* part = e & 1 ? last_part(e >> 1) : first_part(e >> 1);
-                const float pm = part[kCols * (D + 4) + c], top = fmaxf(m, pm), base = top == kNegInf ? 0.0f : top;
-                const float f = exp2_fast(m - base), h = exp2_fast(pm - base);
-                const float4 v = *reinterpret_cast<const float4*>(part + c * (D + 4) + d);
-                l = l * f + part[kCols * (D + 5) + c] * h;
-                o[0] = o[0] * f + v.x * h;
-                o[1] = o[1] * f + v.y * h;
-                o[2] = o[2] * f + v.z * h;
-                o[3] = o[3] * f + v.w * h;
-                m = top;
+    // joining kernel.  First the factors (a warp a column, a lane a partial
+    // result), then the weighted sums.
+    const auto part_of = [&](int e) -> const float* { return e & 1 ? last_part(e >> 1) : first_part(e >> 1); };
+    const bool there = lane < 2 * kWarps && warp_items[lane >> 1].part[lane & 1].end != 0;
+    const uint64_t begin = there ? warp_items[lane >> 1].part[lane & 1].begin : 0;
+    unsigned left = __ballot_sync(kFull, there);  // entries still to be joined; the same in every warp
+    while (left) {
+        const int e0 = __ffs(left) - 1;
+        const uint64_t first_begin = __shfl_sync(kFull, begin, e0);
+        const unsigned mine_of = __ballot_sync(kFull, there && begin == first_begin) & left;
+        left &= ~mine_of;
+        const Item& item = warp_items[e0 >> 1].part[e0 & 1];
+        const int cols = item.tile.cols;
+        for (int c = warp; c < cols; c += kWarps) {
+            const bool on = (mine_of >> lane) & 1;
+            const float* part = part_of(on ? lane : e0);
+            const float pm = on ? part[kCols * (D + 4) + c] : kNegInf;
+            float m = pm;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, off));
+            const float base = m == kNegInf ? 0.0f : m;
+            const float f = on ? exp2_fast(pm - base) : 0.0f;
+            float l = on ? part[kCols * (D + 5) + c] * f : 0.0f;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(kFull, l, off);
+            factors[c * 32 + lane] = f;
+            if (lane == 0) {
+                factors[kCols * 32 + c] = m;
+                factors[kCols * 33 + c] = l;
             }
+        }
+        __syncthreads();
+        const bool whole = item.begin >= u0 && item.end <= u1;
+        float* out_part = parts + (2ull * blockIdx.x + (item.begin <= u0 ? 0 : 1)) * kPartFloats<D, NT>;
+        for (int i = threadIdx.x; i < cols * (D / 4); i += Cfg::kThreads) {
+            const int c = i / (D / 4), d = i % (D / 4) * 4;
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (unsigned rest = mine_of; rest; rest &= rest - 1) {
+                const int e = __ffs(rest) - 1;
+                const float4 v = *reinterpret_cast<const float4*>(part_of(e) + c * (D + 4) + d);
+                const float f = factors[c * 32 + e];
+                o[0] = fmaf(v.x, f, o[0]);
+                o[1] = fmaf(v.y, f, o[1]);
+                o[2] = fmaf(v.z, f, o[2]);
+                o[3] = fmaf(v.w, f, o[3]);
+            }
+            const float m = factors[kCols * 32 + c], l = factors[kCols * 33 + c];
             if (whole) {
-                store_row<D>(p, item.tile, item.head, group, kSelected, c, d, m, l, o);
+                store_row<D>(p, item.tile, item.head, group, kSelected, c, d, m == kNegInf ? 0.0f : m, l, o);
             } else {
                 if (d == 0) {
-                    out[c] = m;
-                    out[kCols + c] = l;
+                    out_part[c] = m;
+                    out_part[kCols + c] = l;
                 }
-                *reinterpret_cast<float4*>(out + 2 * kCols + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<float4*>(out_part + 2 * kCols + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
             }
         }
-        e0 = e1;
+        __syncthreads();
     }
 }
 
