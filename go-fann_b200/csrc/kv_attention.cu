@@ -594,7 +594,7 @@ struct WarpItems {
 template <int D, int NT>
 struct Attend {
     static constexpr int kCols = 8 * NT;
-    static constexpr int kWarps = D * NT <= 128 ? 12 : 8;  // 168 or 255 registers a thread
+    static constexpr int kWarps = D * NT == 64 ? 16 : D * NT == 128 ? 12 : 8;  // 128, 168 or 255 registers a thread
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kHalf = KvChunk<D>::kBytes / 2;
     static constexpr int kSlots = D == 64 || NT == 2 ? 4 : 3;
