@@ -47,33 +47,6 @@ __device__ __forceinline__ uint32_t touched_pages(const gofann_kv_batch& b, uint
     return static_cast<uint32_t>((len + kKvPage - 1) / kKvPage - start / kKvPage);
 }
 
-// Eight consecutive elements as they lie; `wide`: the address is a multiple
-// of 16 bytes.
-__device__ __forceinline__ uint4 load8(const void* p, uint64_t i, bool wide)
-{
-    const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    if (wide) return *reinterpret_cast<const uint4*>(q);
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = q[2 * k] | (static_cast<uint32_t>(q[2 * k + 1]) << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <bool kBf16>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8])
-{
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (kBf16) {
-            x[2 * k] = __uint_as_float(w[k] << 16);
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-            x[2 * k] = f.x;
-            x[2 * k + 1] = f.y;
-        }
-    }
-}
 template <bool kBf16>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8])
 {

@@ -1,19 +1,17 @@
 // kv_select.cu — the blocks of the 4-bit cache that a query reads, by an int8
 // upper bound of q.k over each block.
 //
-// Two launches: scores of every (row, key/value head, block) by int8 matrix
-// instructions (m16n8k32: 16 blocks x 8 query columns x 32 bytes), then one
-// block per (row, head) picks the n_select largest by a radix select over the
-// scores' ordered bits.
-#include "kv_common.cuh"
+// Two launches, the second programmatic: scores of every (row, key/value head,
+// block) by int8 matrix instructions (m16n8k32: 16 blocks x 8 query columns x
+// 32 bytes), then a warp or a thread block per (row, head) finds the n_select-th
+// largest score by bisection over the scores' ordered bits, its keys in
+// registers.
+#include "kv_async.cuh"
 
 namespace gofann {
 namespace {
 
 constexpr int kScoreThreads = 256;
-constexpr int kScoreWarps = kScoreThreads / 32;
-constexpr int kScoreBlocks = 16 * kScoreWarps;  // cache blocks of one thread block
-constexpr int kScoreCols = 64;                  // query columns of one thread block
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -33,145 +31,233 @@ __device__ __forceinline__ int row_blocks(int len, int n, int i)
 // Columns of a row: the group's query heads, padded to a power of two (or a
 // multiple of 8), so that an 8-column tile holds whole rows or part of one.
 struct SelectShape {
-    int group, cols_per_row, rows_per_block;
-    uint32_t block_tiles, stride;  // kScoreBlocks tiles of max_pages; floats of a score row
+    int group, cols_per_row;
+    int tiles;                    // 8-column tiles of a warp
+    int rows;                     // rows of a warp
+    uint32_t splits, split_tiles; // parts of a row's blocks, their 16-block tiles
+    uint32_t stride;              // floats of a score row
 };
 
+// The bounds of 16 blocks as A fragments: lane t takes the 16-byte pieces t of
+// each 64 bytes of rows g and g + 8 (the order of the k axis is free as long
+// as the queries follow it).
 template <int D>
-__global__ void __launch_bounds__(kScoreThreads) kv_score_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
-                                                                 gofann_kv_select_params p, SelectShape sh,
-                                                                 float* __restrict__ scores)
+struct BlockTile {
+    static constexpr int kPieces = 2 * D / 64;
+    uint4 low[kPieces], high[kPieces];
+    float scale[2];  // negative where there is no page
+};
+// Pages of a lane's two blocks; -1 = past the sequence or not a page.
+__device__ __forceinline__ void tile_pages(const gofann_kv_cache& cache, const gofann_kv_batch& b, uint32_t seq, int len,
+                                           int block, int (&page)[2])
 {
-    extern __shared__ __align__(16) unsigned char smem[];
-    int8_t* q8 = reinterpret_cast<int8_t*>(smem);               // [cols][2 D + 16]: positive parts, negative parts
-    constexpr int kStride = 2 * D + 16;
-    float* qs = reinterpret_cast<float*>(smem + static_cast<size_t>(sh.rows_per_block) * sh.cols_per_row * kStride);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t head = blockIdx.y;
-    uint32_t seq, tile;
-    const uint32_t row_tile = blockIdx.x / sh.block_tiles, block_tile = blockIdx.x % sh.block_tiles;
-    const auto tiles = [&](uint32_t s) {
-        int first, n;
-        kv_rows(batch, s, first, n);
-        return static_cast<uint32_t>((n + sh.rows_per_block - 1) / sh.rows_per_block);
-    };
-    if (!kv_find(batch.n_seqs, row_tile, tiles, seq, tile)) return;
-    int first, n;
-    kv_rows(batch, seq, first, n);
-    const int len = kv_len(batch, seq);
-    const int r0 = static_cast<int>(tile) * sh.rows_per_block;
-    const int r1 = r0 + sh.rows_per_block < n ? r0 + sh.rows_per_block : n;
-    const int b0 = static_cast<int>(block_tile) * kScoreBlocks;
-    if (b0 >= row_blocks(len, n, r1 - 1)) return;
-
-    // ---- this warp's 16 blocks as A fragments: lane t takes the 16-byte
-    // pieces t of each 64 bytes of rows g and g + 8 (the order of the k axis
-    // is free as long as q8 follows it)
-    constexpr int kPieces = 2 * D / 64;
-    uint4 lo4[kPieces], hi4[kPieces];
-    float scale[2];
-    int page[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int b = b0 + warp * 16 + g + 8 * r;
+        const int at = block + 8 * r;
         page[r] = -1;
-        if (b * kKvPage < len) {
-            page[r] = __ldg(batch.page_table + static_cast<size_t>(seq) * batch.max_pages + b);
+        if (at * kKvPage < len) {
+            page[r] = __ldg(b.page_table + static_cast<size_t>(seq) * b.max_pages + at);
             if (page[r] < 0 || static_cast<uint32_t>(page[r]) >= cache.n_pages) {
                 page[r] = -1;
-                kv_invalid(batch);
+                kv_invalid(b);
             }
         }
+    }
+}
+template <int D>
+__device__ __forceinline__ void tile_bounds(const gofann_kv_cache& cache, uint32_t head, const int (&page)[2], BlockTile<D>& tile)
+{
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
         const size_t entry = page[r] < 0 ? 0 : static_cast<size_t>(page[r]) * cache.n_kv_heads + head;
         const uint4* src = reinterpret_cast<const uint4*>(cache.bounds + entry * 2 * D) + t;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
+        for (int i = 0; i < BlockTile<D>::kPieces; ++i) {
             const uint4 w = page[r] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(src + 4 * i);
-            if (r == 0) lo4[i] = w; else hi4[i] = w;
+            if (r == 0) tile.low[i] = w; else tile.high[i] = w;
         }
-        scale[r] = page[r] < 0 ? 0.0f : __ldg(cache.bound_scale + entry);
+        tile.scale[r] = page[r] < 0 ? -1.0f : __ldg(cache.bound_scale + entry);
     }
+}
 
-    // ---- int8 queries of the rows, one warp per column
-    const int cols = (r1 - r0) * sh.cols_per_row;
-    for (int c = warp; c < (cols + 7) / 8 * 8; c += kScoreWarps) {
-        const int r = c / sh.cols_per_row, h = c % sh.cols_per_row;
-        float x[D / 32];
-        const bool on = c < cols && h < sh.group;
-        const uint64_t at = static_cast<uint64_t>(first + r0 + r) * p.q_stride + (head * sh.group + h) * D;
-        float a = 0.0f;
-        bool fine = true;
+// One query column in 8 bits as this lane's part of a B fragment: dimensions
+// 64 i + 16 t .. + 15, positive parts in the first pieces, negative ones in the
+// others.  The four lanes of a column call it together; returns the scale, 0
+// for a column that is zero or not finite.
+template <int D, bool kBf16>
+__device__ __forceinline__ float query_column(const gofann_kv_select_params& p, uint64_t at, bool on, bool wide,
+                                              uint4 (&b)[2 * D / 64])
+{
+    uint4 raw[D / 32];
+    float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            x[i] = on ? kv_load(p.q, at + lane + 32 * i, p.dtype) : 0.0f;
-            fine &= fabsf(x[i]) < __int_as_float(0x7f800000);
-            a = fmaxf(a, fabsf(x[i]));
-        }
+    for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(kFull, a, off));
-        fine = __all_sync(kFull, fine) && a > 0.0f;
-        const float s = fine ? __fdiv_rn(a, 127.0f) : 0.0f;
+        for (int k = 0; k < 2; ++k) {
+            uint4& w = raw[2 * i + k];
+            w = on ? load8(p.q, at + 64 * i + 8 * k, wide) : make_uint4(0u, 0u, 0u, 0u);
+            float x[8];
+            unpack8<kBf16>(w, x);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int v = fine ? static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.0f), 127.0f)) : 0;
-            q8[c * kStride + lane + 32 * i] = static_cast<int8_t>(v > 0 ? v : 0);
-            q8[c * kStride + D + lane + 32 * i] = static_cast<int8_t>(v < 0 ? v : 0);
-        }
-        if (lane == 0) qs[c] = on ? s : -1.0f;  // -1 marks a padding column
-    }
-    __syncthreads();
-
-    const int rows_per_tile = sh.cols_per_row < 8 ? 8 / sh.cols_per_row : 1;  // rows in an 8-column tile
-    float best[2] = {kNegInf, kNegInf};
-    for (int c0 = 0; c0 < cols; c0 += 8) {
-        int acc[4] = {0, 0, 0, 0};
-        const uint4* bq = reinterpret_cast<const uint4*>(q8 + (c0 + g) * kStride) + t;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const uint4 w = bq[4 * i];
-            const uint32_t a0[4] = {lo4[i].x, hi4[i].x, lo4[i].y, hi4[i].y};
-            const uint32_t a1[4] = {lo4[i].z, hi4[i].z, lo4[i].w, hi4[i].w};
-            mma_s8(acc, a0, w.x, w.y);
-            mma_s8(acc, a1, w.z, w.w);
-        }
-        // acc: blocks g, g + 8 x columns 2t, 2t + 1
-        float v[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float s = qs[c0 + 2 * t + e];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-                v[r][e] = s < 0.0f ? kNegInf : __fmul_rn(static_cast<float>(acc[2 * r + e]), s);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (sh.cols_per_row >= 2) v[r][0] = v[r][1] = fmaxf(v[r][0], v[r][1]);
-            if (sh.cols_per_row >= 4) v[r][0] = v[r][1] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 1));
-            if (sh.cols_per_row >= 8) v[r][0] = v[r][1] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 2));
-        }
-        bool last = true;
-        if (sh.cols_per_row > 8) {  // a row of several tiles
-            const int part = (c0 / 8) % (sh.cols_per_row / 8);
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                best[r] = part == 0 ? v[r][0] : fmaxf(best[r], v[r][0]);
-                v[r][0] = best[r];
+            for (int e = 0; e < 8; ++e) {
+                // a NaN counts as an infinity
+                const float m = fabsf(x[e]);
+                top = fmaxf(top, m == m ? m : __int_as_float(0x7f800000));
             }
-            last = part == sh.cols_per_row / 8 - 1;
         }
-        if (!last) continue;
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+    const bool fine = top > 0.0f && top < __int_as_float(0x7f800000);
+    const float s = fine ? __fdiv_rn(top, 127.0f) : 0.0f, inv = fine ? __fdiv_rn(1.0f, s) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int col = 2 * t + e;
-            // one writer per row of the tile: its first column
-            if (sh.cols_per_row >= 8 ? col != 0 : col % sh.cols_per_row != 0) continue;
-            const int r = sh.cols_per_row >= 8 ? c0 / sh.cols_per_row : c0 / 8 * rows_per_tile + col / sh.cols_per_row;
-            if (r0 + r >= r1) continue;
-            float* out = scores + (static_cast<size_t>(first + r0 + r) * cache.n_kv_heads + head) * sh.stride;
+    for (int i = 0; i < D / 64; ++i) {
+        uint32_t up[4] = {0, 0, 0, 0}, down[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int b = b0 + warp * 16 + g + 8 * k;
-                if (b < row_blocks(len, n, r0 + r)) out[b] = page[k] < 0 ? kNegInf : __fmul_rn(v[k][e], scale[k]);
+        for (int k = 0; k < 2; ++k) {
+            float x[8];
+            unpack8<kBf16>(raw[2 * i + k], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // rint of the quotient: by the reciprocal (off by less than
+                // 3e-5), unless that is so near a half that the rounded
+                // quotient might fall to the other side
+                const float t = x[e] * inv;
+                float r = rintf(t);
+                if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(x[e], s));
+                const int v = fine ? static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f)) : 0;
+                up[2 * k + e / 4] |= static_cast<uint32_t>(max(v, 0)) << (8 * (e & 3));
+                down[2 * k + e / 4] |= (static_cast<uint32_t>(min(v, 0)) & 0xffu) << (8 * (e & 3));
+            }
+        }
+        b[i] = make_uint4(up[0], up[1], up[2], up[3]);
+        b[D / 64 + i] = make_uint4(down[0], down[1], down[2], down[3]);
+    }
+    return s;
+}
+
+// Scores of one warp: NT tiles of 8 query columns, kept as B fragments, against
+// a part of the cache blocks, 16 at a time, the next ones' pages on their way.  kCols columns a row; 16 stands for a row of
+// several tiles (any multiple of 8), which is done NT tiles at a time with the
+// maximum so far in the score row.
+// What bounds it: for a decode step the bounds' bytes (2 D + 4 a block) and how
+// many of them are on their way, for a chunk the instructions around the
+// products (eight products of 16 x 8 x 32 a tile at head_dim 128).
+template <int D, bool kBf16, int kCols, int NT>
+__global__ void __launch_bounds__(kScoreThreads, NT == 1 ? 3 : 2) kv_score_kernel(gofann_kv_cache cache,
+                                                                                  gofann_kv_batch batch,
+                                                                                  gofann_kv_select_params p,
+                                                                                  SelectShape sh, bool wide,
+                                                                                  float* __restrict__ scores)
+{
+    constexpr int kPieces = BlockTile<D>::kPieces;
+    constexpr int kPerTile = kCols >= 8 ? 1 : 8 / kCols;   // rows of an 8-column tile
+    constexpr int kOut = kCols == 1 ? 2 : 1;               // rows of a tile that a lane writes
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    launch_next();
+    // Few rows: a block's warps take the heads of a page, whose bounds lie side
+    // by side in memory. Many: rows of one head, which share its bounds.
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kScoreThreads / 32) + (threadIdx.x >> 5);
+    const uint64_t per_head = static_cast<uint64_t>(gridDim.x) * (kScoreThreads / 32) / cache.n_kv_heads;
+    const uint64_t unit = NT == 1 ? item / cache.n_kv_heads : item % per_head;
+    const uint32_t head = static_cast<uint32_t>(NT == 1 ? item - unit * cache.n_kv_heads : item / per_head);
+    if (head >= cache.n_kv_heads) return;
+    uint32_t seq, tile;
+    const auto tiles = [&](uint32_t s) {
+        int first, n;
+        kv_rows(batch, s, first, n);
+        return static_cast<uint32_t>((n + sh.rows - 1) / sh.rows);
+    };
+    if (!kv_find<uint32_t>(batch.n_seqs, static_cast<uint32_t>(unit / sh.splits), tiles, seq, tile)) return;
+    int first, n;
+    kv_rows(batch, seq, first, n);
+    const int len = kv_len(batch, seq);
+    const int r0 = static_cast<int>(tile) * sh.rows, r1 = min(r0 + sh.rows, n);
+    const int b0 = static_cast<int>(unit % sh.splits * sh.split_tiles) * 16;
+    const int b1 = min(row_blocks(len, n, r1 - 1), b0 + static_cast<int>(sh.split_tiles) * 16);
+    if (b0 >= b1) return;
+    const int chunks = kCols == 16 ? (sh.cols_per_row / 8 + NT - 1) / NT : 1;
+
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        int page[2];
+        tile_pages(cache, batch, seq, len, b0 + g, page);
+        // ---- the queries
+        uint4 b[NT][kPieces];
+        float qs[NT][2];               // scales of columns 2t, 2t + 1; negative for a padding column
+        float* out[NT][kOut];
+        int blocks[NT][kOut];          // blocks of the rows that this lane writes
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+            const int row = kCols == 16 ? r0 : r0 + k * kPerTile + g / (kCols < 8 ? kCols : 8);
+            const int h = kCols == 16 ? (chunk * NT + k) * 8 + g : g % (kCols < 8 ? kCols : 8);
+            const bool on = row < r1 && h < sh.group;
+            const uint64_t at = static_cast<uint64_t>(first + (on ? row : r0)) * p.q_stride +
+                                static_cast<uint64_t>(head * sh.group + (on ? h : 0)) * D + 16 * t;
+            const float s = query_column<D, kBf16>(p, at, on, wide, b[k]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qs[k][e] = __shfl_sync(kFull, on ? s : -1.0f, 4 * (2 * t + e));
+#pragma unroll
+            for (int e = 0; e < kOut; ++e) {
+                const int mine = kCols >= 8 ? 0 : kCols == 4 ? t >> 1 : kCols == 2 ? t : 2 * t + e;
+                const int r = kCols == 16 ? r0 : r0 + k * kPerTile + mine;
+                blocks[k][e] = r < r1 ? row_blocks(len, n, r) : 0;
+                out[k][e] = scores + (static_cast<size_t>(first + min(r, r1 - 1)) * cache.n_kv_heads + head) * sh.stride + g;
+            }
+        }
+        for (int at = b0; at < b1; at += 16) {
+            BlockTile<D> now;
+            tile_bounds<D>(cache, head, page, now);
+            if (at + 16 < b1) tile_pages(cache, batch, seq, len, at + 16 + g, page);
+            float best[2] = {kNegInf, kNegInf};
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const uint32_t a0[4] = {now.low[i].x, now.high[i].x, now.low[i].y, now.high[i].y};
+                    const uint32_t a1[4] = {now.low[i].z, now.high[i].z, now.low[i].w, now.high[i].w};
+                    mma_s8(acc, a0, b[k][i].x, b[k][i].y);
+                    mma_s8(acc, a1, b[k][i].z, b[k][i].w);
+                }
+                // acc: blocks g, g + 8 x columns 2t, 2t + 1
+                float v[2][2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        v[r][e] = qs[k][e] < 0.0f ? kNegInf : __fmul_rn(static_cast<float>(acc[2 * r + e]), qs[k][e]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if (kCols >= 2) v[r][0] = fmaxf(v[r][0], v[r][1]);
+                    if (kCols >= 4) v[r][0] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 1));
+                    if (kCols >= 8) v[r][0] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 2));
+                }
+                if (kCols == 16) {
+                    best[0] = fmaxf(best[0], v[0][0]);
+                    best[1] = fmaxf(best[1], v[1][0]);
+                    if (k < NT - 1) continue;
+                    v[0][0] = best[0];
+                    v[1][0] = best[1];
+                }
+                if (kCols >= 4) {
+                    // two lanes that hold the same: one a block
+                    const int r = t & 1;
+                    if (t < (kCols >= 8 ? 2 : 4) && at + g + 8 * r < blocks[k][0]) {
+                        float* o = out[k][0] + at + 8 * r;
+                        float x = r ? v[1][0] : v[0][0];
+                        const float scale = r ? now.scale[1] : now.scale[0];
+                        if (kCols == 16 && chunk > 0) x = fmaxf(x, *o);
+                        if (chunk == chunks - 1) x = scale < 0.0f ? kNegInf : __fmul_rn(x, scale);
+                        *o = x;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kOut; ++e)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            if (at + g + 8 * r < blocks[k][e])
+                                out[k][e][at + 8 * r] = now.scale[r] < 0.0f ? kNegInf : __fmul_rn(v[r][e], now.scale[r]);
+                }
             }
         }
     }
@@ -187,9 +273,152 @@ __device__ __forceinline__ uint32_t order_key(float x)
 
 constexpr int kPickThreads = 256;
 
+// The largest n_select of a row's scores, kWarps warps a row, up to kKeys keys
+// a lane in registers (block kWarps 32 i + place): bisection, bit by bit from
+// the top, for the largest key that at least n_select keys reach; all above it
+// and the first ones at it are taken, in block order.
+template <int kWarps, int kKeys>
 __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
                                                                gofann_kv_select_params p, uint32_t stride,
                                                                const float* __restrict__ scores)
+{
+    constexpr int kRows = kPickThreads / 32 / kWarps;  // rows of a thread block
+    __shared__ uint32_t sums[2][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, place = threadIdx.x % (32 * kWarps);
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * kRows + warp / kWarps;
+    if (item >= static_cast<uint64_t>(batch.n_rows) * cache.n_kv_heads) return;  // whole warps (kWarps 8: whole blocks)
+    const uint32_t row = static_cast<uint32_t>(item / cache.n_kv_heads);
+    uint32_t seq = 0, at = 0;
+    const auto rows = [&](uint32_t s) {
+        int first, n;
+        kv_rows(batch, s, first, n);
+        return static_cast<uint32_t>(n);
+    };
+    int blocks = 0;
+    if (kv_find<uint32_t>(batch.n_seqs, row, rows, seq, at)) {
+        int first, n;
+        kv_rows(batch, seq, first, n);
+        blocks = row_blocks(kv_len(batch, seq), n, static_cast<int>(at));
+    }
+    wait_previous();
+    const float* sc = scores + item * stride;
+    int32_t* ids = p.ids + item * p.n_select;
+    float* out = p.scores ? p.scores + item * p.n_select : nullptr;
+    const uint32_t want = p.n_select;
+    uint32_t key[kKeys];
+    uint32_t valid = 0;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+        const int b = 32 * kWarps * i + place;
+        key[i] = 0;
+        if (b < blocks) {
+            const float x = __ldcg(sc + b);
+            if (x != kNegInf) {
+                key[i] = b < static_cast<int>(p.n_first) || b >= blocks - static_cast<int>(p.n_recent) ? 0xffffffffu
+                                                                                                        : order_key(x);
+                ++valid;
+            }
+        }
+    }
+    int turn = 0;
+    // the sum of a count over the row's warps, and over those before this one
+    const auto row_sum = [&](uint32_t c, uint32_t& before) {
+        if (kWarps == 1) {
+            before = 0;
+            return c;
+        }
+        turn ^= 1;
+        if (lane == 0) sums[turn][warp] = c;
+        __syncthreads();
+        uint32_t all = 0;
+        before = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const uint32_t v = sums[turn][w];
+            all += v;
+            if (w < warp) before += v;
+        }
+        return all;
+    };
+    const auto row_max = [&](uint32_t c) {
+        if (kWarps == 1) return c;
+        turn ^= 1;
+        if (lane == 0) sums[turn][warp] = c;
+        __syncthreads();
+        uint32_t m = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = max(m, sums[turn][w]);
+        return m;
+    };
+    uint32_t before;
+    const uint32_t present = row_sum(__reduce_add_sync(kFull, valid), before);
+    uint32_t limit = 1, ties = 0xffffffffu;  // keys from `limit` on, of those at it the first `ties`
+    if (present > want) {
+        // the bits that all but the forced keys share need no bisection
+        uint32_t most = 0, least = ~0u;
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) {
+            if (key[i] != 0xffffffffu) most = max(most, key[i]);
+            if (key[i] != 0) least = min(least, key[i]);
+        }
+        most = row_max(__reduce_max_sync(kFull, most));
+        least = ~row_max(~__reduce_min_sync(kFull, least));
+        const uint32_t differ = most ^ least;
+        const int high = differ ? 31 - __clz(differ) : -1;
+        limit = high < 31 ? least & ~((2u << (high < 0 ? 0 : high)) - 1u) : 0u;
+        if (high < 0) limit = least;
+        uint32_t above = present;  // keys that reach `limit`
+        for (int bit = high; bit >= 0 && above != want; --bit) {
+            const uint32_t try_at = limit | (1u << bit);
+            uint32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) c += key[i] >= try_at;
+            c = row_sum(__reduce_add_sync(kFull, c), before);
+            if (c >= want) {
+                limit = try_at;
+                above = c;
+            }
+        }
+        if (above != want) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) c += key[i] > limit;
+            ties = want - row_sum(__reduce_add_sync(kFull, c), before);
+        }
+    }
+    uint32_t taken = 0, tied = 0;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+        if (32 * kWarps * i >= blocks) break;
+        const bool tie = key[i] == limit, more = key[i] > limit;
+        const unsigned tb = __ballot_sync(kFull, tie), ab = __ballot_sync(kFull, more);
+        // counts of both, packed
+        uint32_t earlier;
+        const uint32_t all = row_sum(__popc(ab) | (__popc(tb) << 16), earlier);
+        const unsigned below = (1u << lane) - 1u;
+        const uint32_t a0 = taken + (earlier & 0xffff) + __popc(ab & below);
+        const uint32_t t0 = tied + (earlier >> 16) + __popc(tb & below);
+        if (more || (tie && t0 < ties)) {
+            const uint32_t slot = a0 + (t0 < ties ? t0 : ties);
+            const int b = 32 * kWarps * i + place;
+            ids[slot] = b;
+            if (out) out[slot] = __ldcg(sc + b);
+        }
+        taken += all & 0xffff;
+        tied += all >> 16;
+    }
+    const uint32_t filled = taken + (tied < ties ? tied : ties);
+    for (uint32_t i = filled + place; i < want; i += 32 * kWarps) {
+        ids[i] = -1;
+        if (out) out[i] = kNegInf;
+    }
+}
+
+// The same for rows of any length, a thread block a row: the limit by four
+// passes of a histogram over the scores in memory.
+__global__ void __launch_bounds__(kPickThreads) kv_pick_long_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
+                                                                    gofann_kv_select_params p, uint32_t stride,
+                                                                    const float* __restrict__ scores)
 {
     __shared__ uint32_t hist[256];
     __shared__ uint32_t warp_sum[kPickThreads / 32][2];
@@ -203,11 +432,12 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache c
         return static_cast<uint32_t>(n);
     };
     int blocks = 0;
-    if (kv_find(batch.n_seqs, row, rows, seq, at)) {
+    if (kv_find<uint32_t>(batch.n_seqs, row, rows, seq, at)) {
         int first, n;
         kv_rows(batch, seq, first, n);
         blocks = row_blocks(kv_len(batch, seq), n, static_cast<int>(at));
     }
+    wait_previous();
     const float* sc = scores + (static_cast<size_t>(row) * cache.n_kv_heads + head) * stride;
     int32_t* ids = p.ids + (static_cast<size_t>(row) * cache.n_kv_heads + head) * p.n_select;
     float* out = p.scores ? p.scores + (static_cast<size_t>(row) * cache.n_kv_heads + head) * p.n_select : nullptr;
@@ -295,6 +525,14 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache c
     }
 }
 
+// Row tiles of a call: a sequence of n rows has at most n / rows + 1, and at
+// most n.
+uint64_t row_tiles(const gofann_kv_batch& b, const SelectShape& s)
+{
+    const uint64_t bound = static_cast<uint64_t>(b.n_rows) / s.rows + b.n_seqs;
+    return bound < b.n_rows ? bound : b.n_rows;
+}
+
 SelectShape select_shape(const gofann_kv_cache& c, const gofann_kv_batch& b, const gofann_kv_select_params& p)
 {
     SelectShape s;
@@ -302,10 +540,37 @@ SelectShape select_shape(const gofann_kv_cache& c, const gofann_kv_batch& b, con
     int cols = 1;
     while (cols < 8 && cols < s.group) cols *= 2;
     s.cols_per_row = s.group > 8 ? (s.group + 7) / 8 * 8 : cols;
-    s.rows_per_block = s.cols_per_row >= kScoreCols ? 1 : kScoreCols / s.cols_per_row;
-    s.block_tiles = (b.max_pages + kScoreBlocks - 1) / kScoreBlocks;
+    // two 8-column tiles a warp where rows fill them
+    s.tiles = s.cols_per_row > 8 || static_cast<uint64_t>(b.max_rows) * s.cols_per_row > 8 ? 2 : 1;
+    s.rows = s.cols_per_row >= 8 ? (s.cols_per_row > 8 ? 1 : s.tiles) : s.tiles * 8 / s.cols_per_row;
+    // enough parts of a row's blocks for 16 warps an SM, no more
+    const uint32_t tiles = (b.max_pages + 15) / 16;
+    const uint64_t units = row_tiles(b, s) * c.n_kv_heads, want = 16ull * (sm_count() > 0 ? sm_count() : 1);
+    uint64_t splits = units ? (want + units - 1) / units : 1;
+    if (splits > tiles) splits = tiles;
+    if (splits < 1) splits = 1;
+    s.split_tiles = static_cast<uint32_t>((tiles + splits - 1) / splits);
+    s.splits = s.split_tiles ? (tiles + s.split_tiles - 1) / s.split_tiles : 1;
     s.stride = (b.max_pages + 3) / 4 * 4;
     return s;
+}
+
+template <int D, bool kBf16>
+void launch_score(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_select_params& p,
+                  const SelectShape& s, bool wide, float* scores, dim3 grid, cudaStream_t cs)
+{
+    const auto go = [&](auto* kernel) { kernel<<<grid, kScoreThreads, 0, cs>>>(cache, batch, p, s, wide, scores); };
+    switch (s.cols_per_row * 4 + s.tiles) {
+        case 4 + 1: return go(kv_score_kernel<D, kBf16, 1, 1>);
+        case 4 + 2: return go(kv_score_kernel<D, kBf16, 1, 2>);
+        case 8 + 1: return go(kv_score_kernel<D, kBf16, 2, 1>);
+        case 8 + 2: return go(kv_score_kernel<D, kBf16, 2, 2>);
+        case 16 + 1: return go(kv_score_kernel<D, kBf16, 4, 1>);
+        case 16 + 2: return go(kv_score_kernel<D, kBf16, 4, 2>);
+        case 32 + 1: return go(kv_score_kernel<D, kBf16, 8, 1>);
+        case 32 + 2: return go(kv_score_kernel<D, kBf16, 8, 2>);
+        default: return go(kv_score_kernel<D, kBf16, 16, 2>);
+    }
 }
 
 }  // namespace
@@ -350,31 +615,44 @@ int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
     if (scratch_bytes < need)
         return fail(GOFANN_ERR_CAPACITY, "kv_select: scratch of %zu bytes, %zu needed", scratch_bytes, need);
     const SelectShape s = select_shape(*cache, *batch, p);
-    // a sequence of n rows has at most n / rows_per_block + 1 tiles, and at most n
-    const uint64_t bound = static_cast<uint64_t>(batch->n_rows) / s.rows_per_block + batch->n_seqs;
-    const uint64_t tiles = (bound < batch->n_rows ? bound : batch->n_rows) * s.block_tiles;
-    if (tiles > 0x7fffffffull)
-        return fail(GOFANN_ERR_UNSUPPORTED, "kv_select: %llu tiles (at most 2^31 - 1)", static_cast<unsigned long long>(tiles));
+    // whole blocks of each head's warps
+    const uint64_t units = (row_tiles(*batch, s) * s.splits + kScoreThreads / 32 - 1) / (kScoreThreads / 32) * cache->n_kv_heads;
+    const uint64_t items = static_cast<uint64_t>(batch->n_rows) * cache->n_kv_heads;
+    if (units > 0x7fffffffull || items > 0x7fffffffull)
+        return fail(GOFANN_ERR_UNSUPPORTED, "kv_select: %u rows of %u heads (2^31 - 1 at most)", batch->n_rows,
+                    cache->n_kv_heads);
     float* scores = static_cast<float*>(scratch);
     cudaStream_t cs = as_stream(stream);
-    const dim3 grid(static_cast<uint32_t>(tiles), cache->n_kv_heads);
-    const size_t cols = static_cast<size_t>(s.rows_per_block) * s.cols_per_row;
-    const size_t smem = cols * (2 * d + 16 + 4);
-    if (smem > 200 * 1024)
-        return fail(GOFANN_ERR_UNSUPPORTED, "kv_select: %d query heads per key/value head", s.group);
-    const void* fn = d == 64 ? reinterpret_cast<const void*>(kv_score_kernel<64>)
-                             : reinterpret_cast<const void*>(kv_score_kernel<128>);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return cuda_status(e, "kv_select: shared memory attribute");
-    }
+    const dim3 grid(static_cast<uint32_t>(units));
+    const bool wide = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && (p.q_stride & 7) == 0;
     if (d == 64)
-        kv_score_kernel<64><<<grid, kScoreThreads, smem, cs>>>(*cache, *batch, p, s, scores);
+        p.dtype == GOFANN_DTYPE_BF16 ? launch_score<64, true>(*cache, *batch, p, s, wide, scores, grid, cs)
+                                     : launch_score<64, false>(*cache, *batch, p, s, wide, scores, grid, cs);
     else
-        kv_score_kernel<128><<<grid, kScoreThreads, smem, cs>>>(*cache, *batch, p, s, scores);
+        p.dtype == GOFANN_DTYPE_BF16 ? launch_score<128, true>(*cache, *batch, p, s, wide, scores, grid, cs)
+                                     : launch_score<128, false>(*cache, *batch, p, s, wide, scores, grid, cs);
     GOFANN_CHECK_LAUNCH("kv_score_kernel");
-    kv_pick_kernel<<<dim3(batch->n_rows, cache->n_kv_heads), kPickThreads, 0, cs>>>(*cache, *batch, p, s.stride, scores);
-    GOFANN_CHECK_LAUNCH("kv_pick_kernel");
+    // A row's keys stay in registers up to 16384 blocks; a warp is enough for
+    // 1024 where there are rows for every SM.
+    const bool single = items >= 8ull * sm_count() && batch->max_pages <= 1024;
+    const auto pick = batch->max_pages > 16384  ? kv_pick_long_kernel
+                      : single                  ? (batch->max_pages <= 256   ? kv_pick_kernel<1, 8>
+                                                   : batch->max_pages <= 640 ? kv_pick_kernel<1, 20>
+                                                                             : kv_pick_kernel<1, 32>)
+                      : batch->max_pages <= 2048 ? kv_pick_kernel<8, 8>
+                                                 : kv_pick_kernel<8, 64>;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = batch->max_pages > 16384 ? dim3(batch->n_rows, cache->n_kv_heads)
+                                           : dim3(static_cast<uint32_t>(single ? (items + 7) / 8 : items));
+    cfg.blockDim = dim3(kPickThreads);
+    cfg.stream = cs;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pick, *cache, *batch, p, s.stride, static_cast<const float*>(scores));
+    if (e != cudaSuccess) return cuda_status(e, "kv_pick_kernel");
     return GOFANN_OK;
 }
 

@@ -297,6 +297,20 @@ def test_select_long_sequence():
     check_select(R.Case([64 * 5003 - 11], [1], 2, 1, 64, BF16), 64)
 
 
+def test_select_longest_rows():
+    """More blocks than a thread block's registers hold."""
+    check_select(R.Case([64 * 16390 + 1, 200], [1, 2], 2, 1, 64, F16), 100)
+
+
+def test_select_many_rows():
+    """Rows for every SM: a warp a row."""
+    check_select(R.Case([64 * 30 + 7, 700], [610, 20], 2, 2, 64, BF16), 9)
+    case = R.Case([64 * 19], [600], 2, 2, 64, BF16)
+    bounds, unit = random_bounds(case, levels=1)
+    unit[:] = 1.0
+    check_select(case, 6, 0, 0, q=torch.ones(600, 2, 64, dtype=BF16, device="cuda"), bounds=bounds, unit=unit)
+
+
 def test_select_ties_go_to_the_lowest_block():
     case = R.Case([64 * 300], [2], 4, 2, 64, F16)
     bounds, unit = random_bounds(case, levels=1)
