@@ -74,10 +74,12 @@ __device__ __forceinline__ void tile_bounds(const gofann_kv_cache& cache, uint32
         const uint4* src = reinterpret_cast<const uint4*>(cache.bounds + entry * 2 * D) + t;
 #pragma unroll
         for (int i = 0; i < BlockTile<D>::kPieces; ++i) {
-            const uint4 w = page[r] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(src + 4 * i);
+            // (those of page 0 where there is none: the scale says so)
+            const uint4 w = __ldg(src + 4 * i);
             if (r == 0) tile.low[i] = w; else tile.high[i] = w;
         }
-        tile.scale[r] = page[r] < 0 ? -1.0f : __ldg(cache.bound_scale + entry);
+        const float scale = __ldg(cache.bound_scale + entry);
+        tile.scale[r] = page[r] < 0 ? -1.0f : scale;
     }
 }
 
@@ -91,6 +93,7 @@ __device__ __forceinline__ float query_column(const gofann_kv_select_params& p, 
 {
     uint4 raw[D / 32];
     float top = 0.0f;
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
 #pragma unroll
@@ -101,38 +104,52 @@ __device__ __forceinline__ float query_column(const gofann_kv_select_params& p, 
             unpack8<kBf16>(w, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                // a NaN counts as an infinity
-                const float m = fabsf(x[e]);
-                top = fmaxf(top, m == m ? m : __int_as_float(0x7f800000));
+                top = fmaxf(top, fabsf(x[e]));
+                nan |= x[e] != x[e];
             }
         }
+    if (nan) top = __int_as_float(0x7f800000);  // fmaxf passes over it
     top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
     top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
     const bool fine = top > 0.0f && top < __int_as_float(0x7f800000);
     const float s = fine ? __fdiv_rn(top, 127.0f) : 0.0f, inv = fine ? __fdiv_rn(1.0f, s) : 0.0f;
+    // rint of the quotients: by the reciprocal (off by less than 3e-5), unless
+    // one is so near a half that the rounded quotient might fall to the other
+    // side
+    bool near = false;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-        uint32_t up[4] = {0, 0, 0, 0}, down[4] = {0, 0, 0, 0};
+    for (int i = 0; i < D / 32; ++i) {
+        float x[8];
+        unpack8<kBf16>(raw[i], x);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float x[8];
-            unpack8<kBf16>(raw[2 * i + k], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // rint of the quotient: by the reciprocal (off by less than
-                // 3e-5), unless that is so near a half that the rounded
-                // quotient might fall to the other side
-                const float t = x[e] * inv;
-                float r = rintf(t);
-                if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(x[e], s));
-                const int v = fine ? static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f)) : 0;
-                up[2 * k + e / 4] |= static_cast<uint32_t>(max(v, 0)) << (8 * (e & 3));
-                down[2 * k + e / 4] |= (static_cast<uint32_t>(min(v, 0)) & 0xffu) << (8 * (e & 3));
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float t = x[e] * inv;
+            near |= fabsf(t - rintf(t)) > 0.4999f;
         }
-        b[i] = make_uint4(up[0], up[1], up[2], up[3]);
-        b[D / 64 + i] = make_uint4(down[0], down[1], down[2], down[3]);
     }
+    const auto split = [&](auto quotient) {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            uint32_t up[4] = {0, 0, 0, 0}, down[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float x[8];
+                unpack8<kBf16>(raw[2 * i + k], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int v = __float2int_rn(fminf(fmaxf(quotient(x[e]), -127.0f), 127.0f));
+                    up[2 * k + e / 4] |= static_cast<uint32_t>(max(v, 0)) << (8 * (e & 3));
+                    down[2 * k + e / 4] |= (static_cast<uint32_t>(min(v, 0)) & 0xffu) << (8 * (e & 3));
+                }
+            }
+            b[i] = make_uint4(up[0], up[1], up[2], up[3]);
+            b[D / 64 + i] = make_uint4(down[0], down[1], down[2], down[3]);
+        }
+    };
+    if (near && fine)
+        split([&](float x) { return __fdiv_rn(x, s); });
+    else
+        split([&](float x) { return fine ? x * inv : 0.0f; });
     return s;
 }
 
@@ -608,7 +625,7 @@ int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
         return fail(GOFANN_ERR_INVALID, "kv_select: bounds must be 16-byte, queries 2-byte aligned");
     if (p.q_stride < static_cast<uint64_t>(p.n_heads) * d)
         return fail(GOFANN_ERR_INVALID, "kv_select: a row stride is shorter than its row");
-    if (batch->max_pages == 0) return fail(GOFANN_ERR_INVALID, "kv_select: rows without pages");
+    if (batch->max_pages == 0 || cache->n_pages == 0) return fail(GOFANN_ERR_INVALID, "kv_select: rows without pages");
     const size_t need = gofann_kv_select_scratch_bytes(cache, batch, params);
     if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255))
         return fail(GOFANN_ERR_INVALID, "kv_select: scratch must be 256-byte aligned");
