@@ -39,19 +39,6 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity)
         : "memory");
     return done != 0;
 }
-// Whether the phase of `parity` has completed; does not wait.
-__device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity)
-{
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0;
-}
 // Waits for the phase of `parity`; false when the limit of some 2 s ran out.
 constexpr long long kWaitCycles = 4ll << 30;
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity)

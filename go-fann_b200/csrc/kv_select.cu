@@ -2,7 +2,7 @@
 // upper bound of q.k over each block.
 //
 // Two launches, the second programmatic: scores of every (row, key/value head,
-// block) by int8 matrix instructions (m16n8k32: 16 blocks x 8 query columns x
+// block) by int8 matrix instructions (m16n8k32: 16 query columns x 8 blocks x
 // 32 bytes), then a warp or a thread block per (row, head) finds the n_select-th
 // largest score by bisection over the scores' ordered bits, its keys in
 // registers.
@@ -29,23 +29,24 @@ __device__ __forceinline__ int row_blocks(int len, int n, int i)
 }
 
 // Columns of a row: the group's query heads, padded to a power of two (or a
-// multiple of 8), so that an 8-column tile holds whole rows or part of one.
+// multiple of 16), so that the 16 columns of a warp hold whole rows or part of
+// one.
 struct SelectShape {
     int group, cols_per_row;
-    int tiles;                    // 8-column tiles of a warp
+    int columns;                  // columns of a warp: 8 or 16
     int rows;                     // rows of a warp
     uint32_t splits, split_tiles; // parts of a row's blocks, their 16-block tiles
     uint32_t stride;              // floats of a score row
 };
 
-// The bounds of 16 blocks as A fragments: lane t takes the 16-byte pieces t of
-// each 64 bytes of rows g and g + 8 (the order of the k axis is free as long
-// as the queries follow it).
+// The bounds of two times 8 blocks as B fragments: lane t takes the 16-byte
+// pieces t of each 64 bytes of blocks g and g + 8 (the order of the k axis is
+// free as long as the queries follow it), so that a load fills two fragments.
 template <int D>
 struct BlockTile {
     static constexpr int kPieces = 2 * D / 64;
-    uint4 low[kPieces], high[kPieces];
-    float scale[2];  // negative where there is no page
+    uint4 piece[2][kPieces];
+    float scale[2];  // of blocks g, g + 8; negative where there is no page
 };
 // Pages of a lane's two blocks; -1 = past the sequence or not a page.
 __device__ __forceinline__ void tile_pages(const gofann_kv_cache& cache, const gofann_kv_batch& b, uint32_t seq, int len,
@@ -76,14 +77,14 @@ __device__ __forceinline__ void tile_bounds(const gofann_kv_cache& cache, uint32
         for (int i = 0; i < BlockTile<D>::kPieces; ++i) {
             // (those of page 0 where there is none: the scale says so)
             const uint4 w = __ldg(src + 4 * i);
-            if (r == 0) tile.low[i] = w; else tile.high[i] = w;
+            tile.piece[r][i] = w;
         }
         const float scale = __ldg(cache.bound_scale + entry);
         tile.scale[r] = page[r] < 0 ? -1.0f : scale;
     }
 }
 
-// One query column in 8 bits as this lane's part of a B fragment: dimensions
+// One query column in 8 bits as this lane's part of A fragments: dimensions
 // 64 i + 16 t .. + 15, positive parts in the first pieces, negative ones in the
 // others.  The four lanes of a column call it together; returns the scale, 0
 // for a column that is zero or not finite.
@@ -153,31 +154,35 @@ __device__ __forceinline__ float query_column(const gofann_kv_select_params& p, 
     return s;
 }
 
-// Scores of one warp: NT tiles of 8 query columns, kept as B fragments, against
-// a part of the cache blocks, 16 at a time, the next ones' pages on their way.  kCols columns a row; 16 stands for a row of
-// several tiles (any multiple of 8), which is done NT tiles at a time with the
-// maximum so far in the score row.
+// Scores of one warp: 16 query columns, kept as A fragments, against a part of
+// the cache blocks, 16 at a time, the next ones' pages on their way.  kCols
+// columns a row; 16 stands for rows of 16 columns and more (any multiple),
+// which are done 16 at a time with the maximum so far in the score row.
+// The maximum over a row's columns, which lanes 4 apart hold, is found by
+// halves: at each step a lane keeps half of its values and sends the others.
 // What bounds it: for a decode step the bounds' bytes (2 D + 4 a block) and how
 // many of them are on their way, for a chunk the instructions around the
-// products (eight products of 16 x 8 x 32 a tile at head_dim 128).
-template <int D, bool kBf16, int kCols, int NT>
-__global__ void __launch_bounds__(kScoreThreads, NT == 1 ? 3 : 2) kv_score_kernel(gofann_kv_cache cache,
+// products (16 products of 16 x 8 x 32 for 16 blocks at head_dim 128).
+// kGroups: 2, or 1 where a sequence's rows have 8 columns at most: the other
+// half of the fragments is zero then and takes no registers (64 rows: 44 us
+// against 47).
+template <int D, bool kBf16, int kCols, int kGroups>
+__global__ void __launch_bounds__(kScoreThreads, (D == 64 ? 3 : 2) + (kGroups == 1)) kv_score_kernel(gofann_kv_cache cache,
                                                                                   gofann_kv_batch batch,
                                                                                   gofann_kv_select_params p,
                                                                                   SelectShape sh, bool wide,
                                                                                   float* __restrict__ scores)
 {
     constexpr int kPieces = BlockTile<D>::kPieces;
-    constexpr int kPerTile = kCols >= 8 ? 1 : 8 / kCols;   // rows of an 8-column tile
-    constexpr int kOut = kCols == 1 ? 2 : 1;               // rows of a tile that a lane writes
+    constexpr int kOut = kCols == 1 ? kGroups : 1;  // rows that a lane writes
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     launch_next();
     // Few rows: a block's warps take the heads of a page, whose bounds lie side
     // by side in memory. Many: rows of one head, which share its bounds.
     const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kScoreThreads / 32) + (threadIdx.x >> 5);
     const uint64_t per_head = static_cast<uint64_t>(gridDim.x) * (kScoreThreads / 32) / cache.n_kv_heads;
-    const uint64_t unit = NT == 1 ? item / cache.n_kv_heads : item % per_head;
-    const uint32_t head = static_cast<uint32_t>(NT == 1 ? item - unit * cache.n_kv_heads : item / per_head);
+    const uint64_t unit = kGroups == 2 ? item % per_head : item / cache.n_kv_heads;
+    const uint32_t head = static_cast<uint32_t>(kGroups == 2 ? item / per_head : item - unit * cache.n_kv_heads);
     if (head >= cache.n_kv_heads) return;
     uint32_t seq, tile;
     const auto tiles = [&](uint32_t s) {
@@ -193,87 +198,104 @@ __global__ void __launch_bounds__(kScoreThreads, NT == 1 ? 3 : 2) kv_score_kerne
     const int b0 = static_cast<int>(unit % sh.splits * sh.split_tiles) * 16;
     const int b1 = min(row_blocks(len, n, r1 - 1), b0 + static_cast<int>(sh.split_tiles) * 16);
     if (b0 >= b1) return;
-    const int chunks = kCols == 16 ? (sh.cols_per_row / 8 + NT - 1) / NT : 1;
+    const int chunks = kCols == 16 ? sh.cols_per_row / 16 : 1;
 
     for (int chunk = 0; chunk < chunks; ++chunk) {
         int page[2];
         tile_pages(cache, batch, seq, len, b0 + g, page);
-        // ---- the queries
-        uint4 b[NT][kPieces];
-        float qs[NT][2];               // scales of columns 2t, 2t + 1; negative for a padding column
-        float* out[NT][kOut];
-        int blocks[NT][kOut];          // blocks of the rows that this lane writes
+        // ---- the queries: columns g and g + 8
+        uint32_t a[2 * kPieces][4] = {};
+        float qs[kGroups];  // their scales; negative for a padding column
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {
-            const int row = kCols == 16 ? r0 : r0 + k * kPerTile + g / (kCols < 8 ? kCols : 8);
-            const int h = kCols == 16 ? (chunk * NT + k) * 8 + g : g % (kCols < 8 ? kCols : 8);
+        for (int k = 0; k < kGroups; ++k) {
+            const int c = g + 8 * k;
+            const int row = kCols == 16 ? r0 : r0 + c / kCols, h = kCols == 16 ? chunk * 16 + c : c % kCols;
             const bool on = row < r1 && h < sh.group;
             const uint64_t at = static_cast<uint64_t>(first + (on ? row : r0)) * p.q_stride +
                                 static_cast<uint64_t>(head * sh.group + (on ? h : 0)) * D + 16 * t;
-            const float s = query_column<D, kBf16>(p, at, on, wide, b[k]);
+            uint4 q[kPieces];
+            const float s = query_column<D, kBf16>(p, at, on, wide, q);
+            qs[k] = on ? s : -1.0f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) qs[k][e] = __shfl_sync(kFull, on ? s : -1.0f, 4 * (2 * t + e));
-#pragma unroll
-            for (int e = 0; e < kOut; ++e) {
-                const int mine = kCols >= 8 ? 0 : kCols == 4 ? t >> 1 : kCols == 2 ? t : 2 * t + e;
-                const int r = kCols == 16 ? r0 : r0 + k * kPerTile + mine;
-                blocks[k][e] = r < r1 ? row_blocks(len, n, r) : 0;
-                out[k][e] = scores + (static_cast<size_t>(first + min(r, r1 - 1)) * cache.n_kv_heads + head) * sh.stride + g;
+            for (int i = 0; i < kPieces; ++i) {
+                a[2 * i][k] = q[i].x, a[2 * i][2 + k] = q[i].y;
+                a[2 * i + 1][k] = q[i].z, a[2 * i + 1][2 + k] = q[i].w;
             }
         }
+        // ---- what this lane writes: of rows `mine`, blocks `off` (and off + 1)
+        constexpr bool kTwo = kGroups == 2;
+        int mine, off = 2 * t;
+        if (kCols == 16) mine = 0, off += g >> 2;
+        if (kCols == 8) mine = kTwo ? g >> 2 : 0, off += kTwo ? (g >> 1) & 1 : g >> 2;
+        if (kCols == 4) mine = kTwo ? (g & 2) + (g >> 2) : g >> 2, off += kTwo ? g & 1 : (g >> 1) & 1;
+        if (kCols == 2) mine = kTwo ? 4 * (g & 1) + (g >> 1) : g >> 1, off += kTwo ? 0 : g & 1;
+        if (kCols == 1) mine = g;
+        float* out[kOut];
+        int blocks[kOut];
+#pragma unroll
+        for (int e = 0; e < kOut; ++e) {
+            const int r = r0 + mine + 8 * e;
+            blocks[e] = r < r1 ? row_blocks(len, n, r) : 0;
+            out[e] = scores + (static_cast<size_t>(first + min(r, r1 - 1)) * cache.n_kv_heads + head) * sh.stride + off;
+        }
+        constexpr int kHeld = kCols == 16 ? 4 : kCols >= (kTwo ? 8 : 4) ? kCols / (kTwo ? 4 : 2) : 1;
+        const bool writes = g % kHeld == 0;  // lanes that hold the same values
         for (int at = b0; at < b1; at += 16) {
             BlockTile<D> now;
             tile_bounds<D>(cache, head, page, now);
             if (at + 16 < b1) tile_pages(cache, batch, seq, len, at + 16 + g, page);
-            float best[2] = {kNegInf, kNegInf};
 #pragma unroll
-            for (int k = 0; k < NT; ++k) {
+            for (int u = 0; u < 2; ++u) {
                 int acc[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    const uint32_t a0[4] = {now.low[i].x, now.high[i].x, now.low[i].y, now.high[i].y};
-                    const uint32_t a1[4] = {now.low[i].z, now.high[i].z, now.low[i].w, now.high[i].w};
-                    mma_s8(acc, a0, b[k][i].x, b[k][i].y);
-                    mma_s8(acc, a1, b[k][i].z, b[k][i].w);
+                    mma_s8(acc, a[2 * i], now.piece[u][i].x, now.piece[u][i].y);
+                    mma_s8(acc, a[2 * i + 1], now.piece[u][i].z, now.piece[u][i].w);
                 }
-                // acc: blocks g, g + 8 x columns 2t, 2t + 1
-                float v[2][2];
+                // acc: columns g, g + 8 x blocks 2t, 2t + 1 of the eight
+                float v[kGroups][2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int k = 0; k < kGroups; ++k)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        v[r][e] = qs[k][e] < 0.0f ? kNegInf : __fmul_rn(static_cast<float>(acc[2 * r + e]), qs[k][e]);
+                    for (int e = 0; e < 2; ++e)
+                        v[k][e] = qs[k] < 0.0f ? kNegInf : __fmul_rn(static_cast<float>(acc[2 * k + e]), qs[k]);
+                // halves that go: the other column group's, then the other block's
+                const auto keep_group = [&](bool second, int lanes) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    if (kCols >= 2) v[r][0] = fmaxf(v[r][0], v[r][1]);
-                    if (kCols >= 4) v[r][0] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 1));
-                    if (kCols >= 8) v[r][0] = fmaxf(v[r][0], __shfl_xor_sync(kFull, v[r][0], 2));
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        const float got = __shfl_xor_sync(kFull, second ? v[0][e] : v[kGroups - 1][e], lanes);
+                        v[0][e] = fmaxf(second ? v[kGroups - 1][e] : v[0][e], got);
+                    }
+                };
+                const auto keep_block = [&](bool second, int lanes) {
+                    const float got = __shfl_xor_sync(kFull, second ? v[0][0] : v[0][1], lanes);
+                    v[0][0] = fmaxf(second ? v[0][1] : v[0][0], got);
+                };
+                const auto same = [&](int lanes) { v[0][0] = fmaxf(v[0][0], __shfl_xor_sync(kFull, v[0][0], lanes)); };
                 if (kCols == 16) {
-                    best[0] = fmaxf(best[0], v[0][0]);
-                    best[1] = fmaxf(best[1], v[1][0]);
-                    if (k < NT - 1) continue;
-                    v[0][0] = best[0];
-                    v[1][0] = best[1];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) v[0][e] = fmaxf(v[0][e], v[kGroups - 1][e]);
+                    keep_block(g & 4, 16), same(8), same(4);
                 }
-                if (kCols >= 4) {
-                    // two lanes that hold the same: one a block
-                    const int r = t & 1;
-                    if (t < (kCols >= 8 ? 2 : 4) && at + g + 8 * r < blocks[k][0]) {
-                        float* o = out[k][0] + at + 8 * r;
-                        float x = r ? v[1][0] : v[0][0];
-                        const float scale = r ? now.scale[1] : now.scale[0];
+                if (kCols == 8 && kTwo) keep_group(g & 4, 16), keep_block(g & 2, 8), same(4);
+                if (kCols == 8 && !kTwo) keep_block(g & 4, 16), same(8), same(4);
+                if (kCols == 4 && kTwo) keep_group(g & 2, 8), keep_block(g & 1, 4);
+                if (kCols == 4 && !kTwo) keep_block(g & 2, 8), same(4);
+                if (kCols == 2 && kTwo) keep_group(g & 1, 4);
+                if (kCols == 2 && !kTwo) keep_block(g & 1, 4);
+                constexpr int kBlocks = kCols >= (kTwo ? 4 : 2) ? 1 : 2;  // blocks that a lane writes
+#pragma unroll
+                for (int w = 0; w < kBlocks; ++w) {
+                    const float scale = __shfl_sync(kFull, now.scale[u], 4 * (off + w));
+#pragma unroll
+                    for (int e = 0; e < kOut; ++e) {
+                        if (!writes || at + 8 * u + off + w >= blocks[e]) continue;
+                        float* o = out[e] + at + 8 * u + w;
+                        float x = v[e][w];
                         if (kCols == 16 && chunk > 0) x = fmaxf(x, *o);
                         if (chunk == chunks - 1) x = scale < 0.0f ? kNegInf : __fmul_rn(x, scale);
                         *o = x;
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kOut; ++e)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                            if (at + g + 8 * r < blocks[k][e])
-                                out[k][e][at + 8 * r] = now.scale[r] < 0.0f ? kNegInf : __fmul_rn(v[r][e], now.scale[r]);
                 }
             }
         }
@@ -556,13 +578,16 @@ SelectShape select_shape(const gofann_kv_cache& c, const gofann_kv_batch& b, con
     s.group = static_cast<int>(p.n_heads / c.n_kv_heads);
     int cols = 1;
     while (cols < 8 && cols < s.group) cols *= 2;
-    s.cols_per_row = s.group > 8 ? (s.group + 7) / 8 * 8 : cols;
-    // two 8-column tiles a warp where rows fill them
-    s.tiles = s.cols_per_row > 8 || static_cast<uint64_t>(b.max_rows) * s.cols_per_row > 8 ? 2 : 1;
-    s.rows = s.cols_per_row >= 8 ? (s.cols_per_row > 8 ? 1 : s.tiles) : s.tiles * 8 / s.cols_per_row;
-    // enough parts of a row's blocks for 16 warps an SM, no more
+    s.cols_per_row = s.group > 8 ? (s.group + 15) / 16 * 16 : cols;
+    // columns of a warp: 8, if no sequence has more
+    s.columns = s.cols_per_row <= 8 && static_cast<uint64_t>(b.max_rows) * s.cols_per_row <= 8 ? 8 : 16;
+    s.rows = s.cols_per_row > 8 ? 1 : s.columns / s.cols_per_row;
+    // Enough parts of a row's blocks for 16 (8 columns) or 12 warps an SM: each
+    // part finds its sequence and rounds its queries anew. Both kernels at 64
+    // rows over 131072 tokens: 8 an SM 55 us, 12 48 us, 16 44 us, 32 51 us; at
+    // 2043 rows over 40003: 8 and 12 71 us, 16 74 us, 32 78 us.
     const uint32_t tiles = (b.max_pages + 15) / 16;
-    const uint64_t units = row_tiles(b, s) * c.n_kv_heads, want = 16ull * (sm_count() > 0 ? sm_count() : 1);
+    const uint64_t units = row_tiles(b, s) * c.n_kv_heads, want = (s.columns == 8 ? 16ull : 12ull) * (sm_count() > 0 ? sm_count() : 1);
     uint64_t splits = units ? (want + units - 1) / units : 1;
     if (splits > tiles) splits = tiles;
     if (splits < 1) splits = 1;
@@ -577,15 +602,12 @@ void launch_score(const gofann_kv_cache& cache, const gofann_kv_batch& batch, co
                   const SelectShape& s, bool wide, float* scores, dim3 grid, cudaStream_t cs)
 {
     const auto go = [&](auto* kernel) { kernel<<<grid, kScoreThreads, 0, cs>>>(cache, batch, p, s, wide, scores); };
-    switch (s.cols_per_row * 4 + s.tiles) {
-        case 4 + 1: return go(kv_score_kernel<D, kBf16, 1, 1>);
-        case 4 + 2: return go(kv_score_kernel<D, kBf16, 1, 2>);
-        case 8 + 1: return go(kv_score_kernel<D, kBf16, 2, 1>);
-        case 8 + 2: return go(kv_score_kernel<D, kBf16, 2, 2>);
-        case 16 + 1: return go(kv_score_kernel<D, kBf16, 4, 1>);
-        case 16 + 2: return go(kv_score_kernel<D, kBf16, 4, 2>);
-        case 32 + 1: return go(kv_score_kernel<D, kBf16, 8, 1>);
-        case 32 + 2: return go(kv_score_kernel<D, kBf16, 8, 2>);
+    const bool one = s.columns == 8;
+    switch (s.cols_per_row) {
+        case 1: return one ? go(kv_score_kernel<D, kBf16, 1, 1>) : go(kv_score_kernel<D, kBf16, 1, 2>);
+        case 2: return one ? go(kv_score_kernel<D, kBf16, 2, 1>) : go(kv_score_kernel<D, kBf16, 2, 2>);
+        case 4: return one ? go(kv_score_kernel<D, kBf16, 4, 1>) : go(kv_score_kernel<D, kBf16, 4, 2>);
+        case 8: return one ? go(kv_score_kernel<D, kBf16, 8, 1>) : go(kv_score_kernel<D, kBf16, 8, 2>);
         default: return go(kv_score_kernel<D, kBf16, 16, 2>);
     }
 }
