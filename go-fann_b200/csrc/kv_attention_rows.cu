@@ -51,12 +51,15 @@ struct Rows {
     static constexpr int kValues = kStepKeys * D * 2;               // [page][D dims][64 tokens]
     static constexpr int kHalf = KvChunk<D>::kBytes / 2;            // keys or values of a page
     static constexpr int kRaw = D == 64 ? 12 : 6;
+    // Stages of the keys' lower parts and of the values: what shared memory holds.
+    static constexpr int kLate = D == 64 ? 2 : 1;
     static constexpr int kOffK = kTiles * kQTile;
-    static constexpr int kOffV = kOffK + 2 * kKeys;
-    static constexpr int kOffRaw = kOffV + 2 * kValues;
+    static constexpr int kOffLow = kOffK + 2 * kKeys;
+    static constexpr int kOffV = kOffLow + kLate * kKeys;
+    static constexpr int kOffRaw = kOffV + kLate * kValues;
     static constexpr int kOffShown = kOffRaw + kRaw * kHalf;        // u64 [8 steps][2 pages]
     static constexpr int kOffBars = kOffShown + 8 * 16;
-    static constexpr int kBars = 2 * kRaw + 8 + 5 * kTiles + 2;
+    static constexpr int kBars = 2 * kRaw + 4 + 6 * kLate + 5 * kTiles + 2;
     static constexpr int kBytes = 1024 + kOffBars + 8 * kBars + 16;
     static_assert(kBytes <= 227 * 1024, "shared memory of a block");
     // tensor memory columns
@@ -202,13 +205,44 @@ __device__ __forceinline__ void code_pairs(uint32_t w, __half2& low, __half2& hi
     high = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, back);  // / 16 - 64
 }
 
-// Keys of one page from the key half of its chunk: this warp's quarter (16 tokens) as rows of 64 dimensions.
+// Two f32 numbers as f16, and what the rounding left of them.
+__device__ __forceinline__ void split_two(uint64_t x, uint32_t& high, uint32_t& low)
+{
+    const __half2 h = __floats2half2_rn(first_of(x), second_of(x));
+    const float2 back = __half22float2(h);
+    const uint64_t rest = add_two(x, pair(-back.x, -back.y));
+    high = as_word(h);
+    low = as_word(__floats2half2_rn(first_of(rest), second_of(rest)));
+}
+
+// 16 bytes of every row of one page's keys: this warp's quarter (16 tokens) as
+// rows of 64 dimensions.
 template <int D>
-__device__ __forceinline__ void decode_keys(const unsigned char* chunk, unsigned char* keys, int page, int warp)
+__device__ __forceinline__ void store_keys(const uint32_t (&k)[KvChunk<D>::kGroups][2][8], unsigned char* keys, int page,
+                                           int kt)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int token0 = 16 * (g >> 1) + 4 * kt + (g & 1);
+#pragma unroll
+    for (int grp = 0; grp < KvChunk<D>::kGroups; ++grp)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t(&w)[8] = k[grp][r];
+            const int row = page * kKvPage + token0 + 2 * r;
+            unsigned char* dst = keys + grp * (kStepKeys * 128) + row * 128;
+            *reinterpret_cast<uint4*>(dst + (((2 * t) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + (((2 * t + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+}
+
+// Keys of one page from the key half of its chunk, this warp's quarter, as
+// sums of two f16 numbers: c * s + m takes up to 22 bits.
+template <int D>
+__device__ __forceinline__ void decode_keys(const unsigned char* chunk, int kt, uint32_t (&high)[KvChunk<D>::kGroups][2][8],
+                                            uint32_t (&low)[KvChunk<D>::kGroups][2][8])
 {
     constexpr int G = KvChunk<D>::kGroups;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, kt = warp;
-    const int token0 = 16 * (g >> 1) + 4 * kt + (g & 1);
+    const int lane = threadIdx.x & 31, g = lane >> 2;
     const uint32_t* params = reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kCodes) + (g * 4 + kt) * 2 * G;
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
@@ -216,20 +250,16 @@ __device__ __forceinline__ void decode_keys(const unsigned char* chunk, unsigned
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const __half2 sm = as_half2(params[r * G + grp]);
-            const __half2 s = __low2half2(sm), m = __high2half2(sm);
-            uint32_t out[8];
+            const float2 sm = __half22float2(as_half2(params[r * G + grp]));
+            const uint64_t s2 = pair(sm.x, sm.x), m2 = pair(sm.y, sm.y);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 __half2 a, b;
                 code_pairs(r ? w[j] >> 8 : w[j], a, b);
-                out[2 * j] = as_word(__hfma2(a, s, m));
-                out[2 * j + 1] = as_word(__hfma2(b, s, m));
+                const float2 x = __half22float2(a), y = __half22float2(b);
+                split_two(fma_two(pair(x.x, x.y), s2, m2), high[grp][r][2 * j], low[grp][r][2 * j]);
+                split_two(fma_two(pair(y.x, y.y), s2, m2), high[grp][r][2 * j + 1], low[grp][r][2 * j + 1]);
             }
-            const int row = page * kKvPage + token0 + 2 * r;
-            unsigned char* dst = keys + grp * (kStepKeys * 128) + row * 128;
-            *reinterpret_cast<uint4*>(dst + (((2 * t) ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-            *reinterpret_cast<uint4*>(dst + (((2 * t + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
         }
     }
 }
@@ -482,9 +512,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     uint64_t* step_shown = reinterpret_cast<uint64_t*>(smem + Cfg::kOffShown);  // [step & 7][page]
     const uint32_t bars = shared_addr(smem + Cfg::kOffBars);
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * kRaw;
-    const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
+    constexpr uint32_t kLate = Cfg::kLate;
+    const uint32_t k_full = raw_empty + 8 * kRaw, k_empty = k_full + 16;
+    const uint32_t low_full = k_empty + 16, low_empty = low_full + 8 * kLate;
+    const uint32_t v_full = low_empty + 8 * kLate, v_empty = v_full + 16 * kLate;  // [stage][page]
     // [tile][half] of S and P
-    const uint32_t s_full = v_empty + 16, p_full = s_full + 16 * kTiles, q_full = p_full + 16 * kTiles;
+    const uint32_t s_full = v_empty + 16 * kLate, p_full = s_full + 16 * kTiles, q_full = p_full + 16 * kTiles;
     const uint32_t all_done = q_full + 8, o_half = all_done + 8;  // o_half: [tile] the first page's product
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffBars + 8 * Cfg::kBars);
     volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a wait has run out
@@ -516,7 +549,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         for (int i = 0; i < 2; ++i) {
             barrier_init(k_full + 8 * i, kDecodeWarps);
             barrier_init(k_empty + 8 * i, 1);
-            barrier_init(v_full + 8 * i, kDecodeWarps);
+        }
+        for (uint32_t i = 0; i < kLate; ++i) {
+            barrier_init(low_full + 8 * i, kDecodeWarps);
+            barrier_init(low_empty + 8 * i, 1);
+        }
+        for (uint32_t i = 0; i < 2 * kLate; ++i) {
+            barrier_init(v_full + 8 * i, kDecodeWarps / 2);
             barrier_init(v_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2 * kTiles; ++i) {
@@ -608,59 +647,72 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         Item it = start;
         const uint32_t base = shared_addr(smem);
         const uint64_t q_desc = operand_desc(base);
-        const auto scores = [&](int tile, uint32_t stage) {
+        const auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(kFull, wait(bar, parity)) != 0; };
+        // S of a tile at step g: the keys' upper parts, then the lower ones
+        const auto scores = [&](int tile, uint32_t g) {
+            const uint32_t late = g % kLate;
             const uint64_t q = q_desc + tile * (Cfg::kQTile >> 4);
-            const uint64_t k = q_desc + (Cfg::kOffK >> 4) + stage * (Cfg::kKeys >> 4);
-            if (elect_one()) {
+            const uint64_t k = q_desc + (Cfg::kOffK >> 4) + (g & 1) * (Cfg::kKeys >> 4);
+            const uint64_t low = q_desc + (Cfg::kOffLow >> 4) + late * (Cfg::kKeys >> 4);
+            const auto products = [&](uint64_t keys, bool add) {
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
                     mma_shared(tmem + Cfg::kScores + tile * kStepKeys, q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4),
-                               k + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kStepKeys), i > 0);
+                               keys + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kStepKeys),
+                               add || i > 0);
+            };
+            if (tile == 0) {
+                if (!all_wait(k_full + 8 * (g & 1), g >> 1)) return false;
+                fence_after();
+            }
+            if (elect_one()) products(k, false);
+            if (tile == 0) {
+                if (!all_wait(low_full + 8 * late, g / kLate)) return false;
+                fence_after();
+            }
+            if (elect_one()) {
+                products(low, true);
                 mma_commit(s_full + 16 * tile);
                 mma_commit(s_full + 16 * tile + 8);
-                if (tile == kTiles - 1) mma_commit(k_empty + 8 * stage);
+                if (tile == kTiles - 1) {
+                    mma_commit(k_empty + 8 * (g & 1));
+                    mma_commit(low_empty + 8 * late);
+                }
             }
+            return true;
         };
-        const auto output = [&](int tile, int h, uint32_t stage, uint32_t add) {
-            const uint64_t v = q_desc + ((Cfg::kOffV + h * (D * 128)) >> 4) + stage * (Cfg::kValues >> 4);
+        const auto output = [&](int tile, int h, uint32_t g, uint32_t add) {
+            const uint32_t late = g % kLate;
+            const uint64_t v = q_desc + ((Cfg::kOffV + h * (D * 128)) >> 4) + late * (Cfg::kValues >> 4);
+            if (tile == 0 && !all_wait(v_full + 16 * late + 8 * h, g / kLate)) return false;
+            fence_after();
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < kKvPage / 16; ++k)
                     mma_tensor(tmem + Cfg::kOut + tile * D, tmem + Cfg::kScores + tile * kStepKeys + h * kKvPage + 8 * k,
                                v + (k * 32 >> 4), mma_shape(kTileRows, D), k > 0 ? 1u : add);
                 if (h == 0) mma_commit(o_half + 8 * tile);
-                if (tile == kTiles - 1 && h == 1) mma_commit(v_empty + 8 * stage);
+                if (tile == kTiles - 1) mma_commit(v_empty + 16 * late + 8 * h);
             }
+            return true;
         };
-        const auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(kFull, wait(bar, parity)) != 0; };
         uint32_t g = 0, items = 0;  // steps and items so far
         bool ok = true;
         do {
             const int steps = __shfl_sync(kFull, it.to - it.from, 0);
-            ok = all_wait(q_full, items) && all_wait(k_full + 8 * (g & 1), g >> 1);
-            if (!ok) break;
+            ok = all_wait(q_full, items);
             fence_after();
-#pragma unroll
-            for (int tile = 0; tile < kTiles; ++tile) scores(tile, g & 1);
+            for (int tile = 0; tile < kTiles; ++tile) ok = ok && scores(tile, g);
             for (int j = 0; j < steps && ok; ++j, ++g) {
-                const uint32_t st = g & 1, next = st ^ 1;
                 const bool more = j + 1 < steps;
-                ok = all_wait(v_full + 8 * st, g >> 1);
 #pragma unroll
                 for (int i = 0; i < 2 * kTiles; ++i) {
                     const int tile = i % kTiles, h = i / kTiles;
-                    ok = ok && all_wait(p_full + 16 * tile + 8 * h, g);
+                    ok = ok && all_wait(p_full + 16 * tile + 8 * h, g) && output(tile, h, g, j > 0 || h > 0);
                     if (!ok) break;
-                    fence_after();
-                    output(tile, h, st, j > 0 || h > 0);
                     if (h == 0) continue;
                     if (more) {
-                        if (tile == 0) {
-                            ok = all_wait(k_full + 8 * next, (g + 1) >> 1);
-                            if (!ok) break;
-                            fence_after();
-                        }
-                        scores(tile, next);
+                        ok = scores(tile, g + 1);
                     } else if (elect_one()) {
                         mma_commit(s_full + 16 * tile);
                         mma_commit(s_full + 16 * tile + 8);
@@ -686,21 +738,31 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                 const uint32_t st = g & 1, i = 4 * g + page, slot = i % kRaw, slot2 = (i + 2) % kRaw;
                 ok = wait(raw_full + 8 * slot, i / kRaw) && (g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1));
                 if (!ok) break;
-                decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
+                uint32_t high[KvChunk<D>::kGroups][2][8], low[KvChunk<D>::kGroups][2][8];
+                decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf, quarter, high, low);
+                store_keys<D>(high, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
                 fence_shared();
                 __syncwarp();
                 if (lane == 0) {
                     barrier_arrive(k_full + 8 * st);
                     barrier_arrive(raw_empty + 8 * slot);
                 }
-                ok = wait(raw_full + 8 * slot2, (i + 2) / kRaw) && (g < 2 || wait(v_empty + 8 * st, (g >> 1) - 1));
+                const uint32_t late = g % kLate, turn = g / kLate - 1;  // turn: of the buffer's last use
+                ok = g < kLate || wait(low_empty + 8 * late, turn);
+                if (!ok) break;
+                store_keys<D>(low, smem + Cfg::kOffLow + late * Cfg::kKeys, page, quarter);
+                fence_shared();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(low_full + 8 * late);
+                ok = wait(raw_full + 8 * slot2, (i + 2) / kRaw) && (g < kLate || wait(v_empty + 16 * late + 8 * page, turn));
                 if (!ok) break;
                 decode_values<D>(smem + Cfg::kOffRaw + slot2 * Cfg::kHalf,
-                                 smem + Cfg::kOffV + st * Cfg::kValues + page * (D * 128), quarter, step_shown[(g & 7) * 2 + page]);
+                                 smem + Cfg::kOffV + late * Cfg::kValues + page * (D * 128), quarter,
+                                 step_shown[(g & 7) * 2 + page]);
                 fence_shared();
                 __syncwarp();
                 if (lane == 0) {
-                    barrier_arrive(v_full + 8 * st);
+                    barrier_arrive(v_full + 16 * late + 8 * page);
                     barrier_arrive(raw_empty + 8 * slot2);
                 }
             }
