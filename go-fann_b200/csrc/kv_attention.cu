@@ -1116,13 +1116,17 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(gofann_kv_cache c
     }
 }
 
-// Query columns (rows x query heads) of a key/value head from which the
-// tensor memory kernel runs.
-constexpr uint64_t kManyColumns = 128;
+// The tensor memory kernel takes 256 query columns (rows x query heads of a
+// key/value head) at a time, whatever there is of them; the other one's time
+// grows with the columns.  8 sequences of 16384 tokens, 8 key/value heads, us
+// (the other kernel / tensor memory): head_dim 128 at 64 columns 190 / 260, at
+// 128 326 / 272, at 256 601 / 292; head_dim 64 at 128 columns 190 / 202, at 256
+// 352 / 215.
+constexpr uint64_t kManyColumnDims = 128 * 128;
 bool many_columns(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p)
 {
     return !p.selected && cache.n_kv_heads &&
-           static_cast<uint64_t>(batch.max_rows) * (p.n_heads / cache.n_kv_heads) >= kManyColumns;
+           static_cast<uint64_t>(batch.max_rows) * (p.n_heads / cache.n_kv_heads) * cache.head_dim >= kManyColumnDims;
 }
 
 // Cache blocks that an item can have at most.

@@ -6,11 +6,12 @@
 // one key/value head) at a time and walks their blocks of the cache, two pages
 // (128 tokens) a step:
 // * a loader copies packed chunks to a shared ring (bulk copies);
-// * eight warps turn codes into f16 keys [token][dim] and transposed values
-//   [dim][token], both 128-byte swizzled and K-major, each page once for all
-//   256 columns;
-// * one thread issues S = Q K^T (tcgen05.mma, M = 128, N = 128) and
-//   O += P V (M = 128, N = head_dim, P from tensor memory);
+// * eight warps turn codes into keys [token][dim], each a sum of two f16
+//   numbers, and four into f16 values [dim][token], all 128-byte swizzled and
+//   K-major, each page once for all 256 columns;
+// * one thread issues S = Q K^T (tcgen05.mma, M = 128, N = 128, twice: the
+//   keys' upper and lower parts) and O += P V (M = 128, N = head_dim, P from
+//   tensor memory);
 // * two warpgroups, one thread a query column, turn S into P: mask and
 //   exponential; P takes the place of S in tensor memory as f16.
 // While one tile is in the exponentials the other has the tensor cores.
@@ -19,10 +20,11 @@
 // per SM: a block does a run of them, and an item that a share's end cuts is
 // joined from partial results by a second, programmatic launch.
 //
-// Precision: keys and values c * s + m are rounded to f16 (at most 2^-11 of
-// the value; a quantisation step is at least 2^-4 of the group's range, so
-// this is below 2^-7 of what the cache has already rounded), weights to f16;
-// logits, sums and the output are f32.  A column's weights are relative to a
+// Precision: a key c * s + m is held as its f16 rounding and the f16 rounding
+// of what that left, 22 bits in all: a logit that one f16 number a key gives
+// is off by some 2e-4, which lse shows (up to 5e-5 of it where a row sees few
+// tokens).  Values and weights are rounded to f16 once (2^-11; the output is
+// of 16 bits anyway); logits, sums and the output are f32.  A column's weights are relative to a
 // reference, its first maximum, times 2^7; the reference moves up to the
 // maximum only where 32 weights sum to more than 2^15 (f16 ends at 2^16), so
 // the maximum is rarely looked for and the output rarely rescaled.
@@ -33,14 +35,14 @@ namespace {
 
 constexpr int kTileRows = 128, kTiles = 2;
 constexpr int kStepKeys = 2 * kKvPage;
-// Eight warps decode: a quarter of the keys and of the values of one of a
-// step's two pages each.
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
+// Eight warps decode keys, a quarter of one of a step's two pages each; four
+// decode values, a quarter of both.
+constexpr int kSoftmaxWarps = 8, kKeyWarps = 8, kDecodeWarps = kKeyWarps + 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kRowThreads = 32 * (kLoadWarp + 3);  // whole warpgroups
-// Registers a thread: 96 at launch for 640 threads, 61440 in all; the split
-// below takes 256 x 112 + 256 x 88 + 128 x 72 = 60416.
-constexpr int kSoftmaxRegs = 112, kDecodeRegs = 88, kOtherRegs = 72;
+// Registers a thread: 80 at launch for 768 threads, 61440 in all, which is
+// what 256 x 104 + 384 x 72 + 128 x 56 takes.
+constexpr int kSoftmaxRegs = 104, kDecodeRegs = 72, kOtherRegs = 56;
 constexpr float kHead = 7.0f;      // log2 of a weight at the reference
 constexpr float kMost = 32768.0f;  // sum of 32 weights from which the reference moves up
 
@@ -83,11 +85,15 @@ __host__ __device__ constexpr uint32_t mma_shape(int m, int n)
 {
     return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add)
+// d (+)= a b + a c: the second product takes a from the buffer that the first
+// one left it in.
+__device__ __forceinline__ void mma_shared_two(uint32_t d, uint64_t a, uint64_t b, uint64_t c, uint32_t shape, uint32_t add)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"(add)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], %1, %2, %4, p;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], %1, %3, %4, q;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "l"(c), "r"(shape), "r"(add)
         : "memory");
 }
 __device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, uint32_t add)
@@ -544,18 +550,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     if (warp == 1 && lane == 0) {
         for (int i = 0; i < kRaw; ++i) {
             barrier_init(raw_full + 8 * i, 1);
-            barrier_init(raw_empty + 8 * i, kDecodeWarps / 2);
+            barrier_init(raw_empty + 8 * i, 4);
         }
         for (int i = 0; i < 2; ++i) {
-            barrier_init(k_full + 8 * i, kDecodeWarps);
+            barrier_init(k_full + 8 * i, kKeyWarps);
             barrier_init(k_empty + 8 * i, 1);
         }
         for (uint32_t i = 0; i < kLate; ++i) {
-            barrier_init(low_full + 8 * i, kDecodeWarps);
+            barrier_init(low_full + 8 * i, kKeyWarps);
             barrier_init(low_empty + 8 * i, 1);
         }
         for (uint32_t i = 0; i < 2 * kLate; ++i) {
-            barrier_init(v_full + 8 * i, kDecodeWarps / 2);
+            barrier_init(v_full + 8 * i, 4);
             barrier_init(v_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2 * kTiles; ++i) {
@@ -654,24 +660,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             const uint64_t q = q_desc + tile * (Cfg::kQTile >> 4);
             const uint64_t k = q_desc + (Cfg::kOffK >> 4) + (g & 1) * (Cfg::kKeys >> 4);
             const uint64_t low = q_desc + (Cfg::kOffLow >> 4) + late * (Cfg::kKeys >> 4);
-            const auto products = [&](uint64_t keys, bool add) {
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma_shared(tmem + Cfg::kScores + tile * kStepKeys, q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4),
-                               keys + (((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4), mma_shape(kTileRows, kStepKeys),
-                               add || i > 0);
-            };
             if (tile == 0) {
-                if (!all_wait(k_full + 8 * (g & 1), g >> 1)) return false;
-                fence_after();
-            }
-            if (elect_one()) products(k, false);
-            if (tile == 0) {
-                if (!all_wait(low_full + 8 * late, g / kLate)) return false;
+                if (!all_wait(k_full + 8 * (g & 1), g >> 1) || !all_wait(low_full + 8 * late, g / kLate)) return false;
                 fence_after();
             }
             if (elect_one()) {
-                products(low, true);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint64_t at = ((i / 4) * (kStepKeys * 128) + (i % 4) * 32) >> 4;
+                    mma_shared_two(tmem + Cfg::kScores + tile * kStepKeys,
+                                   q + (((i / 4) * (kTileRows * 128) + (i % 4) * 32) >> 4), k + at, low + at,
+                                   mma_shape(kTileRows, kStepKeys), i > 0);
+                }
                 mma_commit(s_full + 16 * tile);
                 mma_commit(s_full + 16 * tile + 8);
                 if (tile == kTiles - 1) {
@@ -729,44 +729,56 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
     } else if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
         // ---- codes to f16 operands
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegs));
-        const int page = (warp - kSoftmaxWarps) >> 2, quarter = warp & 3;
+        const int quarter = warp & 3;
         Item it = start;
         uint32_t g = 0;
         bool ok = true;
-        do {
-            for (int j = it.from; j < it.to; ++j, ++g) {
-                const uint32_t st = g & 1, i = 4 * g + page, slot = i % kRaw, slot2 = (i + 2) % kRaw;
-                ok = wait(raw_full + 8 * slot, i / kRaw) && (g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1));
-                if (!ok) break;
-                uint32_t high[KvChunk<D>::kGroups][2][8], low[KvChunk<D>::kGroups][2][8];
-                decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf, quarter, high, low);
-                store_keys<D>(high, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
-                fence_shared();
-                __syncwarp();
-                if (lane == 0) {
-                    barrier_arrive(k_full + 8 * st);
-                    barrier_arrive(raw_empty + 8 * slot);
+        if (warp < kSoftmaxWarps + kKeyWarps) {
+            const int page = (warp - kSoftmaxWarps) >> 2;
+            do {
+                for (int j = it.from; j < it.to && ok; ++j, ++g) {
+                    const uint32_t st = g & 1, late = g % kLate, turn = g / kLate - 1;  // turn: of the buffer's last use
+                    const uint32_t i = 4 * g + page, slot = i % kRaw;
+                    ok = wait(raw_full + 8 * slot, i / kRaw) && (g < 2 || wait(k_empty + 8 * st, (g >> 1) - 1));
+                    if (!ok) break;
+                    uint32_t high[KvChunk<D>::kGroups][2][8], low[KvChunk<D>::kGroups][2][8];
+                    decode_keys<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf, quarter, high, low);
+                    store_keys<D>(high, smem + Cfg::kOffK + st * Cfg::kKeys, page, quarter);
+                    fence_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        barrier_arrive(k_full + 8 * st);
+                        barrier_arrive(raw_empty + 8 * slot);
+                    }
+                    ok = g < kLate || wait(low_empty + 8 * late, turn);
+                    if (!ok) break;
+                    store_keys<D>(low, smem + Cfg::kOffLow + late * Cfg::kKeys, page, quarter);
+                    fence_shared();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(low_full + 8 * late);
                 }
-                const uint32_t late = g % kLate, turn = g / kLate - 1;  // turn: of the buffer's last use
-                ok = g < kLate || wait(low_empty + 8 * late, turn);
-                if (!ok) break;
-                store_keys<D>(low, smem + Cfg::kOffLow + late * Cfg::kKeys, page, quarter);
-                fence_shared();
-                __syncwarp();
-                if (lane == 0) barrier_arrive(low_full + 8 * late);
-                ok = wait(raw_full + 8 * slot2, (i + 2) / kRaw) && (g < kLate || wait(v_empty + 16 * late + 8 * page, turn));
-                if (!ok) break;
-                decode_values<D>(smem + Cfg::kOffRaw + slot2 * Cfg::kHalf,
-                                 smem + Cfg::kOffV + late * Cfg::kValues + page * (D * 128), quarter,
-                                 step_shown[(g & 7) * 2 + page]);
-                fence_shared();
-                __syncwarp();
-                if (lane == 0) {
-                    barrier_arrive(v_full + 16 * late + 8 * page);
-                    barrier_arrive(raw_empty + 8 * slot2);
+            } while (ok && next_item(batch, p, n_kv, group, it));
+        } else {
+            do {
+                for (int j = it.from; j < it.to && ok; ++j, ++g) {
+                    const uint32_t late = g % kLate, turn = g / kLate - 1;
+                    for (int page = 0; page < 2; ++page) {
+                        const uint32_t i = 4 * g + 2 + page, slot = i % kRaw;
+                        ok = wait(raw_full + 8 * slot, i / kRaw) && (g < kLate || wait(v_empty + 16 * late + 8 * page, turn));
+                        if (!ok) break;
+                        decode_values<D>(smem + Cfg::kOffRaw + slot * Cfg::kHalf,
+                                         smem + Cfg::kOffV + late * Cfg::kValues + page * (D * 128), quarter,
+                                         step_shown[(g & 7) * 2 + page]);
+                        fence_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            barrier_arrive(v_full + 16 * late + 8 * page);
+                            barrier_arrive(raw_empty + 8 * slot);
+                        }
+                    }
                 }
-            }
-        } while (ok && next_item(batch, p, n_kv, group, it));
+            } while (ok && next_item(batch, p, n_kv, group, it));
+        }
     } else if (warp < kSoftmaxWarps) {
         // ---- softmax: one thread a query column
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));

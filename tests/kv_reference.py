@@ -152,20 +152,12 @@ class Case:
         return k, v, (float(scale.abs().max()) if n else 0.0), (float(v.abs().max()) if n else 0.0)
 
 
-MANY_COLUMNS = 128  # query columns of a key/value head from which keys and values are rounded to f16
-
-
 def attention(case, pages, q, scale, causal=True, window=0, selected=None, bits=None):
-    """out, lse in 64 bits and the bounds of the error that f16 weights, f32 sums and the output's rounding allow.
-
-    Keys rounded to f16 (dense calls of MANY_COLUMNS columns) move a logit by a sum of independent roundings, each
-    at most 2^-11 |q_d k_d| and uniform: six standard deviations of it, and what they do to the weights."""
+    """out, lse in 64 bits and the bounds of the error that f16 weights, f32 sums and the output's rounding allow."""
     group = case.heads // case.kv
     out = torch.zeros(case.n_rows, case.heads, case.d, dtype=torch.float64, device="cuda")
     lse = torch.full((case.n_rows, case.heads), -math.inf, dtype=torch.float64, device="cuda")
     slack = torch.zeros(case.n_rows, case.heads, 1, dtype=torch.float64, device="cuda")
-    lse_slack = torch.zeros(case.n_rows, case.heads, dtype=torch.float64, device="cuda")
-    many = selected is None and max(case.rows) * group >= MANY_COLUMNS
     row = 0
     for s, n in enumerate(case.lens):
         if case.rows[s] == 0:
@@ -201,17 +193,12 @@ def attention(case, pages, q, scale, causal=True, window=0, selected=None, bits=
             score = torch.where(mine, q[lo:hi, h].double() @ k[:, kv].T * scale, -math.inf)
             if n == 0:
                 continue
-            if many:
-                off = (q[lo:hi, h].double().square() @ k[:, kv].square().T).sqrt() * abs(scale) * 2.0 ** -11 / 3 ** 0.5
-                off = 6 * torch.where(mine, off, 0.0).amax(-1)
-                lse_slack[lo:hi, h] = off
-                slack[lo:hi, h] += torch.expm1(2 * off)[:, None] * top_value
             lse[lo:hi, h] = torch.logsumexp(score, -1)
             some = mine.any(-1, keepdim=True)
             w = torch.where(some, torch.softmax(torch.where(some, score, 0.0), -1), 0.0)
             out[lo:hi, h] = w @ v[:, kv]
     unit = 2.0 ** -8 if case.dtype == torch.bfloat16 else 2.0 ** -11
-    return out, lse, unit * out.abs() + slack, 2.0 ** -16 + 2.0 ** -18 * lse.abs() + lse_slack
+    return out, lse, unit * out.abs() + slack, 2.0 ** -16 + 2.0 ** -18 * lse.abs()
 
 
 def check_attention(got, lse, want, want_lse, slack, lse_slack):
