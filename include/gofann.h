@@ -696,7 +696,8 @@ typedef struct gofann_kv_cache {
 /* Sequences of one call and their query rows.  Row i of sequence s (rows
  * row_offset[s] .. row_offset[s+1] - 1 of the call) is the token at position
  * seq_len[s] - rows + i: a sequence's rows are its newest tokens.  seq_len
- * counts the tokens in the cache with this call's rows among them. */
+ * counts the tokens in the cache with this call's rows among them.  Sequences
+ * may share pages that hold none of a call's rows (a common beginning). */
 typedef struct gofann_kv_batch {
     const int32_t* page_table;   /* device [n_seqs][max_pages]: pages of a sequence in token order */
     const uint32_t* seq_len;     /* device [n_seqs], at most max_pages * GOFANN_KV_PAGE */
@@ -706,7 +707,8 @@ typedef struct gofann_kv_batch {
     uint32_t n_seqs;
     uint32_t max_pages;
     uint32_t n_rows;
-    uint32_t max_rows;           /* largest number of rows of a sequence; chooses kernels, not results */
+    uint32_t max_rows;           /* largest number of rows of a sequence; chooses kernels, whose results differ
+                                    by roundings */
 } gofann_kv_batch;
 
 /* Rows of q, k and v are [heads][head_dim] contiguous, consecutive rows
@@ -774,7 +776,8 @@ GOFANN_API size_t gofann_kv_chunk_bytes(uint32_t head_dim);
  * f16((max - min) / 15), code = clamp(rint((x - m) / s), 0, 15), or 0 where s
  * is 0) and renews the bounds of the touched pages from all tokens that they
  * hold.  Tokens of the touched pages other than the rows keep their codes.
- * One launch, no scratch; q_out may be q where q's rows are contiguous. */
+ * One launch, no scratch; q_out may be q where q's rows are contiguous.
+ * Outputs are 16-byte aligned; inputs need no more than their type's. */
 GOFANN_API int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                                 const gofann_kv_append_params* params, void* stream);
 
@@ -796,8 +799,9 @@ GOFANN_API int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_ba
 /* out = softmax(scale * q.K^T) V over the cached tokens that each row sees:
  * those of the selected blocks (or of all blocks), up to the row's own token
  * (causal), inside the window and shown by key_bits.  Query head h reads
- * key/value head h / (n_heads / n_kv_heads).  Logits, maxima, sums and the
- * output are accumulated in f32.  scratch: gofann_kv_attention_scratch_bytes,
+ * key/value head h / (n_heads / n_kv_heads).  Logits, sums and the output are
+ * accumulated in f32; weights are rounded to f16, and so are values where the
+ * query rows of all sequences are many.  Every sum has a fixed order.  scratch: gofann_kv_attention_scratch_bytes,
  * 256-byte aligned. */
 GOFANN_API size_t gofann_kv_attention_scratch_bytes(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                                                     const gofann_kv_attention_params* params);
