@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
         const auto fetch = [&](int kind) {
             return kind < n_q ? load8(p.q, q_at + static_cast<uint64_t>(kind) * D, q_wide) : make_uint4(0u, 0u, 0u, 0u);
         };
-        constexpr int kAhead = 2;  // query vectors on their way
+        // query vectors on their way: chunks of 2043 rows 51 us with 2, 45 with 4, 47 with 6
+        constexpr int kAhead = 4;
         uint4 next[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) next[a] = fetch(part + a * share);
