@@ -206,7 +206,10 @@ __device__ __forceinline__ uint32_t value_mask(int i, int lo, int hi)
 
 // What bounds it: a full page is a stream (q, k, v in, q, k, v out, codes),
 // a decode step's single rows are the chain of dependent loads: sequence, page
-// number, then everything else at once.  So all that a block reads is asked
+// number, then everything else at once (one row 8.5 us, 96 rows 10.7 us).  Five
+// chunks of 2043 rows (32 query and 8 key/value heads of 64, in pairs) take 45
+// us, 2.9 TB/s: 28 M instructions of a warp, 56 % of the issue slots, half of
+// them rounding and rotating; the rest is the wait for a page's first rows.  So all that a block reads is asked
 // for before it is used: page words that are only partly written, the keys
 // that the page holds, the rows.
 template <int D, int kMode, bool kBf16, int kAppendThreads>

@@ -594,7 +594,10 @@ struct WarpItems {
 template <int D, int NT>
 struct Attend {
     static constexpr int kCols = 8 * NT;
-    static constexpr int kWarps = D * NT == 64 ? 16 : D * NT == 128 ? 12 : 8;  // 128, 168 or 255 registers a thread
+    // 128, 168 or 255 registers a thread.  Instead with 8 warps: 32 rows over
+    // 32768 tokens, head_dim 128, 8 columns, 183 us (12 warps: 170); 509 rows of
+    // 32 selected blocks, head_dim 64, 107 us (16 warps: 86).
+    static constexpr int kWarps = D * NT == 64 ? 16 : D * NT == 128 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kHalf = KvChunk<D>::kBytes / 2;
     static constexpr int kSlots = D == 64 || NT == 2 ? 4 : 3;
@@ -728,6 +731,14 @@ __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofa
 // Each thread block takes an equal share of all units, each warp an equal,
 // consecutive part of the share; a warp that has a whole item writes its rows
 // itself.
+//
+// What bounds it: the instructions that turn codes into operands and join a
+// page's sums (a warp issues 94 M of them for 0.81 GB), whose fixed latencies
+// 12 to 16 warps hide in part; 54 % of the issue slots are taken.  32 rows over
+// 32768 tokens (64 query, 8 key/value heads of 128) take 170 us, 4.8 TB/s, 0.73
+// of the measured copy; one row over 131072 tokens 51 us, of which the
+// partial results' join is 8; 48 rows of 64 selected blocks 70 us, 3.2 TB/s:
+// each (row, head) has its own list of pages to look up and its own join.
 template <int D, int NT, bool kSelected>
 __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(gofann_kv_cache cache,
                                                                                gofann_kv_batch batch,
@@ -1045,7 +1056,9 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
 
 // Items that several blocks share.  The factors of the partial results first,
 // then their weighted sum in block order, all loads side by side; the sum does
-// not depend on which block was done first.
+// not depend on which block was done first.  Two dependent loads from L2 and a
+// launch: 8 us under a profiler, about 5 behind the main kernel, which it is
+// launched beside.
 constexpr int kMaxBlocks = 192, kJoinThreads = 256;
 template <int D, int NT, bool kSelected>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(gofann_kv_cache cache, gofann_kv_batch batch, Call p,
@@ -1152,7 +1165,8 @@ int launch_attend(const gofann_kv_cache& cache, const gofann_kv_batch& batch, Ca
 {
     using Cfg = Attend<D, NT>;
     // Items of at most two pages a warp stay in one block: what a split would
-    // gain, the joining kernel would cost.
+    // gain, the joining kernel would cost (one row over 777 tokens 12.6 us, split
+    // 16.5; 509 rows of 32 selected blocks 86 us, split 90).
     p.fixed = most_blocks(batch, p) <= 2 * Cfg::kWarps ? static_cast<int>(most_blocks(batch, p)) : 0;
     auto* kernel = kv_attend_kernel<D, NT, kSelected>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kBytes));

@@ -161,8 +161,11 @@ __device__ __forceinline__ float query_column(const gofann_kv_select_params& p, 
 // The maximum over a row's columns, which lanes 4 apart hold, is found by
 // halves: at each step a lane keeps half of its values and sends the others.
 // What bounds it: for a decode step the bounds' bytes (2 D + 4 a block) and how
-// many of them are on their way, for a chunk the instructions around the
-// products (16 products of 16 x 8 x 32 for 16 blocks at head_dim 128).
+// many of them are on their way (64 rows over 131072 tokens, 4 heads of 128:
+// 104 MB in 31 us, 3.4 TB/s; fetching a tile ahead changes nothing), for a
+// chunk the instructions around the products (16 products of 16 x 8 x 32 for
+// 16 blocks at head_dim 128; 2043 rows over 40003 tokens, 2 heads: 52 us, 18 M
+// instructions of a warp, 35 % of the issue slots).
 // kGroups: 2, or 1 where a sequence's rows have 8 columns at most: the other
 // half of the fragments is zero then and takes no registers (64 rows: 44 us
 // against 47).
@@ -315,7 +318,9 @@ constexpr int kPickThreads = 256;
 // The largest n_select of a row's scores, kWarps warps a row, up to kKeys keys
 // a lane in registers (block kWarps 32 i + place): bisection, bit by bit from
 // the top, for the largest key that at least n_select keys reach; all above it
-// and the first ones at it are taken, in block order.
+// and the first ones at it are taken, in block order.  The scores come from L2:
+// what bounds it is the chain of loads, up to 32 counts and the ranks (256 rows
+// of 2048 blocks 15 us, 4086 rows of 626 blocks 26 us).
 template <int kWarps, int kKeys>
 __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache cache, gofann_kv_batch batch,
                                                                gofann_kv_select_params p, uint32_t stride,
@@ -671,17 +676,21 @@ int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
         p.dtype == GOFANN_DTYPE_BF16 ? launch_score<128, true>(*cache, *batch, p, s, wide, scores, grid, cs)
                                      : launch_score<128, false>(*cache, *batch, p, s, wide, scores, grid, cs);
     GOFANN_CHECK_LAUNCH("kv_score_kernel");
-    // A row's keys stay in registers up to 16384 blocks; a warp is enough for
-    // 1024 where there are rows for every SM.
+    // A row's keys stay in registers up to 2048 blocks; a warp is enough for
+    // 1024 where there are rows for every SM.  Both launches, us: 2043 rows x 2
+    // heads of 626 blocks, a warp with 20 keys a lane 70, with 32 keys 84, eight
+    // warps 88, keys in memory 83; 64 rows x 4 heads of 2048 blocks, eight warps
+    // with 8 keys a lane 44, keys in memory 45; 4 rows x 4 heads of 2500
+    // blocks, 64 keys a lane 23, keys in memory 16.
     const bool single = items >= 8ull * sm_count() && batch->max_pages <= 1024;
-    const auto pick = batch->max_pages > 16384  ? kv_pick_long_kernel
-                      : single                  ? (batch->max_pages <= 256   ? kv_pick_kernel<1, 8>
-                                                   : batch->max_pages <= 640 ? kv_pick_kernel<1, 20>
-                                                                             : kv_pick_kernel<1, 32>)
-                      : batch->max_pages <= 2048 ? kv_pick_kernel<8, 8>
-                                                 : kv_pick_kernel<8, 64>;
+    const bool in_memory = batch->max_pages > 2048;
+    const auto pick = in_memory ? kv_pick_long_kernel
+                      : !single ? kv_pick_kernel<8, 8>
+                      : batch->max_pages <= 256 ? kv_pick_kernel<1, 8>
+                      : batch->max_pages <= 640 ? kv_pick_kernel<1, 20>
+                                                : kv_pick_kernel<1, 32>;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = batch->max_pages > 16384 ? dim3(batch->n_rows, cache->n_kv_heads)
+    cfg.gridDim = in_memory ? dim3(batch->n_rows, cache->n_kv_heads)
                                            : dim3(static_cast<uint32_t>(single ? (items + 7) / 8 : items));
     cfg.blockDim = dim3(kPickThreads);
     cfg.stream = cs;
