@@ -311,6 +311,13 @@ def test_select_many_rows():
     check_select(case, 6, 0, 0, q=torch.ones(600, 2, 64, dtype=BF16, device="cuda"), bounds=bounds, unit=unit)
 
 
+@pytest.mark.parametrize("blocks", [256, 257, 640, 641, 1024, 1025, 2048, 2049])
+@pytest.mark.parametrize("rows", [1, 620])
+def test_select_blocks_around_the_kernels_limits(blocks, rows):
+    """Where a row's scores change from a warp's registers to a block's, and to memory."""
+    check_select(R.Case([64 * blocks - 5], [rows], 2, 2, 64, BF16), 33, first=1, recent=1)
+
+
 def test_select_ties_go_to_the_lowest_block():
     case = R.Case([64 * 300], [2], 4, 2, 64, F16)
     bounds, unit = random_bounds(case, levels=1)
