@@ -57,7 +57,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 // Programmatic launches: the next kernel of the stream may start, and wait
-// for the work of the one before.
+// for the work of the one before.  Every thread of a kernel launched that way
+// waits before it returns, one with nothing to do too: what follows in the
+// stream is ordered behind that kernel only, so it must not end first.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -1079,10 +1079,16 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(gofann_kv_cache c
             return static_cast<unsigned long long>(cut < total ? cut : ~0ull);
         },
         c);
-    if (!any) return;
+    if (!any) {
+        wait_previous();
+        return;
+    }
     Item item;
     make_item<kSelected>(batch, p, n_kv, group, kCols, cut, c, item);
-    if (item.begin >= cut || item.begin < share * blockIdx.x) return;
+    if (item.begin >= cut || item.begin < share * blockIdx.x) {
+        wait_previous();
+        return;
+    }
     const uint64_t first = blockIdx.x;
     const int count = static_cast<int>((item.end - 1) / share - first) + 1;
     const auto part_at = [&](int b) {

@@ -994,16 +994,18 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_rows_kernel(gofann_kv_ca
     const uint64_t share = steps_per_block(total, blocks);
     // block i joins the item that the end of share i cuts, if that is the item's first cut
     const uint64_t cut = share * (blockIdx.y + 1);
-    if (cut >= total) return;
+    if (cut >= total) {
+        wait_previous();
+        return;
+    }
     const Place at = locate(batch, p, n_kv, group, cut);
     Item it{};
     it.seq = at.seq, it.head = at.head, it.tile = at.tile, it.flat = cut, it.limit = ~0ull;
     open_item(batch, p, group, at.step, it);
     const uint64_t begin = cut - at.step, end = begin + it.steps;
-    if (begin >= cut || begin < share * blockIdx.y) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = static_cast<int>(blockIdx.x) * kJoinColumns;
-    if (c0 >= it.cols) return;
     wait_previous();
+    if (begin >= cut || begin < share * blockIdx.y || c0 >= it.cols) return;
     const uint64_t last = (end - 1) / share;
     constexpr int kEach = D / (kJoinThreads / 32);
     float m = kNegInf, l = 0.0f, o[kEach];

@@ -330,7 +330,10 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache c
     __shared__ uint32_t sums[2][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, place = threadIdx.x % (32 * kWarps);
     const uint64_t item = static_cast<uint64_t>(blockIdx.x) * kRows + warp / kWarps;
-    if (item >= static_cast<uint64_t>(batch.n_rows) * cache.n_kv_heads) return;  // whole warps (kWarps 8: whole blocks)
+    if (item >= static_cast<uint64_t>(batch.n_rows) * cache.n_kv_heads) {  // whole warps (kWarps 8: whole blocks)
+        wait_previous();
+        return;
+    }
     const uint32_t row = static_cast<uint32_t>(item / cache.n_kv_heads);
     uint32_t seq = 0, at = 0;
     const auto rows = [&](uint32_t s) {
