@@ -59,7 +59,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // Programmatic launches: the next kernel of the stream may start, and wait
 // for the work of the one before.  Every thread of a kernel launched that way
 // waits before it returns, one with nothing to do too: what follows in the
-// stream is ordered behind that kernel only, so it must not end first.
+// stream is ordered behind that kernel only, so it must not end first.  What
+// the kernel before wrote is read with __ldcg: neither the read-only path nor a
+// line that its blocks left in this SM's L1 may serve it.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

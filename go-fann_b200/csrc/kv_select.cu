@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_long_kernel(gofann_kv_ca
     float* out = p.scores ? p.scores + (static_cast<size_t>(row) * cache.n_kv_heads + head) * p.n_select : nullptr;
     const int want = static_cast<int>(p.n_select);
     const auto key_of = [&](int b) {
-        const float x = sc[b];
+        const float x = __ldcg(sc + b);
         if (x == kNegInf) return 0u;
         return b < static_cast<int>(p.n_first) || b >= blocks - static_cast<int>(p.n_recent) ? 0xffffffffu : order_key(x);
     };
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_long_kernel(gofann_kv_ca
         if (above || (tie && t0 < ties)) {
             const uint32_t slot = a0 + (t0 < ties ? t0 : ties);
             ids[slot] = b;
-            if (out) out[slot] = sc[b];
+            if (out) out[slot] = __ldcg(sc + b);
         }
         __syncthreads();
     }

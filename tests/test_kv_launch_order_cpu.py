@@ -53,3 +53,19 @@ def test_every_return_is_behind_the_wait(body):
     assert outer is not None, "no wait that every thread reaches"
     for m in re.finditer(r"\breturn\s*;", body[:outer]):
         assert re.search(r"wait_previous\(\);\s*$", body[: m.start()]), body[max(0, m.start() - 200) : m.end()]
+
+
+@pytest.mark.parametrize("body", dependents())
+def test_results_of_the_kernel_before_come_from_l2(body):
+    """Its blocks may still run beside this kernel, so a plain load could be served by the read-only path or by a line
+    that they left in L1."""
+    sources = {"scores", "parts"}
+    while True:  # names of pointers into the scratch
+        names = "|".join(sources)
+        more = set(re.findall(rf"const float\* (\w+) = (?:{names})\b", body)) - sources
+        if not more:
+            break
+        sources |= more
+    for name in sources:
+        assert not re.search(rf"\b{name}\s*\[", body), f"{name} is indexed"
+        assert not re.search(rf"(?<!float)\*\s*(?:reinterpret_cast<[^>]*>)?\(?{name}\b", body), f"{name} is read through"

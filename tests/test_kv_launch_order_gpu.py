@@ -54,3 +54,11 @@ def test_the_next_node_of_a_graph_reads_the_whole_result(lens, rows, heads, kv):
     for _ in range(50):
         graph.replay()
         assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+
+
+@pytest.mark.parametrize("heads", [32, 9])
+def test_long_rows_of_many_heads_are_picked_from_whole_scores(heads):
+    """More than 8 query heads: the scoring kernel reads its scores back, whose lines neighbouring rows share; more than
+    2048 blocks: the picking kernel reads them from memory."""
+    from test_kv_cache_gpu import check_select
+    check_select(R.Case([64 * 2300 - 5, 64 * 2101], [3, 2], heads, 1, 64, torch.float16), 40)
