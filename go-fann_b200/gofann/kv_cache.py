@@ -68,7 +68,7 @@ def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, scalin
             return rotary_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))
 
         lo = max(math.floor(pair(beta_fast)), 0)
-        hi = min(math.ceil(pair(beta_slow)), max(rotary_dim // 2 - 1, 0))
+        hi = math.ceil(pair(beta_slow))  # past the last pair where all turn more often
         ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         freq = freq * (1 - ramp) + freq / factor * ramp
         if magnitude is None:
