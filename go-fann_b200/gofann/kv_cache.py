@@ -78,7 +78,13 @@ def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, scalin
     return (angle.cos() * m).float(), (angle.sin() * m).float()
 
 
-def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str) -> tuple[int, int]:
+def _here(x: torch.Tensor, index: int, name: str) -> None:
+    """Refuses a tensor that is not on the cache's device: a kernel would follow its address all the same."""
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, the cache on {f'cuda:{index}' if index >= 0 else 'cpu'}")
+
+
+def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str, index: int) -> tuple[int, int]:
     """Address and row stride of [rows][heads][dim] with contiguous heads."""
     if x.shape != (rows, heads, dim):
         raise ValueError(f"{name} must be [{rows} rows][{heads}][{dim}], got {tuple(x.shape)}")
@@ -87,14 +93,16 @@ def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str) ->
     stride = x.stride()
     if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{name}: the heads of a row must be contiguous")
+    _here(x, index, name)
     return x.data_ptr(), stride[0] if rows > 1 else heads * dim
 
 
-def _out(x: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, name: str) -> torch.Tensor:
+def _out(x: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, name: str, index: int) -> torch.Tensor:
     if x is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
-    if x.shape != shape or x.dtype is not dtype or not x.is_contiguous() or x.get_device() != like.get_device():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {like.device}")
+    if x.shape != shape or x.dtype is not dtype or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
+    _here(x, index, name)
     return x
 
 
@@ -121,7 +129,10 @@ class KVBatch:
             raise ValueError(f"n_rows {n_rows} and max_rows {max_rows}")
         self.page_table, self.seq_len, self.row_offset = page_table, seq_len, row_offset
         self.n_seqs, self.n_rows, self.max_rows = n_seqs, int(n_rows), int(max_rows)
+        if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != page_table.device):
+            raise ValueError(f"status must be an int32 tensor on {page_table.device}")
         self.status = status if status is not None else torch.zeros(1, dtype=torch.int32, device=page_table.device)
+        self._index = page_table.get_device()
         self.struct = A.KvBatch(page_table=page_table.data_ptr(), seq_len=seq_len.data_ptr(),
                                 row_offset=row_offset.data_ptr(), status=self.status.data_ptr(), n_seqs=n_seqs,
                                 max_pages=int(page_table.shape[1]), n_rows=self.n_rows, max_rows=self.max_rows)
@@ -167,6 +178,9 @@ class KVCache:
                                    not bounds.is_contiguous() or not bound_scale.is_contiguous()):
             raise ValueError(f"bounds must be contiguous int8 [n_pages][n_kv_heads][2][{head_dim}] and bound_scale "
                              "float32 [n_pages][n_kv_heads]")
+        for t in (bounds, bound_scale):
+            if t is not None and t.device != first.device:
+                raise ValueError(f"bounds and bound_scale are on {t.device}, pages on {first.device}")
         self.head_dim, self.n_kv_heads, self.n_pages = head_dim, n_kv, n_pages
         self.pages, self.bounds, self.bound_scale = pages, bounds, bound_scale
         self.device = first.device
@@ -189,6 +203,13 @@ class KVCache:
             return stream.cuda_stream
         return torch._C._cuda_getCurrentRawStream(self._index)
 
+    def _on(self, batch: KVBatch) -> None:
+        """Refuses what a kernel must not follow: a batch of another device, a cache in host memory."""
+        if batch._index != self._index:
+            raise ValueError(f"the batch is on {batch.page_table.device}, the cache on {self.device}")
+        if self._index < 0:
+            raise ValueError(f"the cache is on {self.device}: its operators run on a GPU")
+
     def _heads(self, q: torch.Tensor) -> int:
         shape = q.shape
         if len(shape) != 3 or shape[1] % self.n_kv_heads or not shape[1]:
@@ -204,23 +225,23 @@ class KVCache:
 
         Returns the rotated queries and, where k_out / v_out are given or
         `held` is set, the keys and values as the cache holds them (else None)."""
-        d, n_kv, n = self.head_dim, self.n_kv_heads, batch.n_rows
+        d, n_kv, n, index = self.head_dim, self.n_kv_heads, batch.n_rows, self._index
         dtype = k.dtype
         if dtype not in DTYPES:
             raise TypeError(f"keys are {dtype}, not bfloat16 or float16")
-        k_at, k_stride = _rows(k, n, n_kv, d, dtype, "k")
-        v_at, v_stride = _rows(v, n, n_kv, d, dtype, "v")
+        k_at, k_stride = _rows(k, n, n_kv, d, dtype, "k", index)
+        v_at, v_stride = _rows(v, n, n_kv, d, dtype, "v", index)
         heads, q_at, q_stride, q_to, k_to, v_to = n_kv, None, 0, None, None, None
         if q is not None:
             heads = self._heads(q)
-            q_at, q_stride = _rows(q, n, heads, d, dtype, "q")
-            q_out = _out(q_out, (n, heads, d), dtype, k, "q_out")
+            q_at, q_stride = _rows(q, n, heads, d, dtype, "q", index)
+            q_out = _out(q_out, (n, heads, d), dtype, k, "q_out", index)
             q_to = q_out.data_ptr()
         if held or k_out is not None:
-            k_out = _out(k_out, (n, n_kv, d), dtype, k, "k_out")
+            k_out = _out(k_out, (n, n_kv, d), dtype, k, "k_out", index)
             k_to = k_out.data_ptr()
         if held or v_out is not None:
-            v_out = _out(v_out, (n, n_kv, d), dtype, k, "v_out")
+            v_out = _out(v_out, (n, n_kv, d), dtype, k, "v_out", index)
             v_to = v_out.data_ptr()
         cos_at, sin_at, n_positions, positions_at = None, None, 0, None
         if rotary_dim:
@@ -228,11 +249,15 @@ class KVCache:
                     cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or \
                     not cos.is_contiguous() or not sin.is_contiguous():
                 raise ValueError(f"cos and sin must be contiguous float32 [positions][{rotary_dim // 2}]")
+            _here(cos, index, "cos")
+            _here(sin, index, "sin")
             cos_at, sin_at, n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
         if positions is not None:
             if positions.dtype is not torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
                 raise ValueError("positions must be contiguous int32 [n_rows]")
+            _here(positions, index, "positions")
             positions_at = positions.data_ptr()
+        self._on(batch)
         p = A.KvAppendParams(q_at, k_at, v_at, q_stride, k_stride, v_stride, cos_at, sin_at, positions_at, q_to, k_to,
                              v_to, DTYPES[dtype], heads, n_positions, rotary_dim, 1 if interleaved else 0)
         status = self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), self._stream(stream))
@@ -244,11 +269,12 @@ class KVCache:
                scores=None, stream=None):
         """Blocks that each row and key/value head reads: ids int32 and scores
         f32 [n_rows][n_kv_heads][n_select], ascending blocks, -1 / -inf fill."""
-        heads, n = self._heads(q), batch.n_rows
-        at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q")
+        heads, n, index = self._heads(q), batch.n_rows, self._index
+        at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q", index)
         shape = (n, self.n_kv_heads, n_select)
-        ids = _out(ids, shape, torch.int32, q, "ids")
-        scores = _out(scores, shape, torch.float32, q, "scores")
+        ids = _out(ids, shape, torch.int32, q, "ids", index)
+        scores = _out(scores, shape, torch.float32, q, "scores", index)
+        self._on(batch)
         ref = C.byref(A.KvSelectParams(at, stride, ids.data_ptr(), scores.data_ptr(), DTYPES[q.dtype], heads, n_select,
                                        first, recent))
         scratch, size = batch.scratch((0, heads, self.n_kv_heads, self.head_dim, n_select),
@@ -266,21 +292,24 @@ class KVCache:
         reads (select's ids); key_bits int32 [n_seqs][words]: a bit per token,
         0 hides it (filtered out or evicted).  scale defaults to
         head_dim^-0.5."""
-        heads, n, d = self._heads(q), batch.n_rows, self.head_dim
-        at, stride = _rows(q, n, heads, d, q.dtype, "q")
-        out = _out(out, (n, heads, d), q.dtype, q, "out")
-        lse = _out(lse, (n, heads), torch.float32, q, "lse")
+        heads, n, d, index = self._heads(q), batch.n_rows, self.head_dim, self._index
+        at, stride = _rows(q, n, heads, d, q.dtype, "q", index)
+        out = _out(out, (n, heads, d), q.dtype, q, "out", index)
+        lse = _out(lse, (n, heads), torch.float32, q, "lse", index)
         selected_at, n_select, bits_at, words = None, 0, None, 0
         if selected is not None:
             if selected.dtype is not torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
                     selected.shape[:2] != (n, self.n_kv_heads):
                 raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width]")
+            _here(selected, index, "selected")
             selected_at, n_select = selected.data_ptr(), selected.shape[2]
         if key_bits is not None:
             if key_bits.dtype is not torch.int32 or key_bits.dim() != 2 or not key_bits.is_contiguous() or \
                     key_bits.shape[0] != batch.n_seqs:
                 raise ValueError("key_bits must be contiguous int32 [n_seqs][words]")
+            _here(key_bits, index, "key_bits")
             bits_at, words = key_bits.data_ptr(), key_bits.shape[1]
+        self._on(batch)
         ref = C.byref(A.KvAttentionParams(at, stride, selected_at, bits_at, out.data_ptr(), lse.data_ptr(),
                                           d ** -0.5 if scale is None else scale, DTYPES[q.dtype], heads, n_select, words,
                                           1 if causal else 0, window))
