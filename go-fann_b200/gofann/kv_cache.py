@@ -78,10 +78,9 @@ def rope_tables(n_positions: int, rotary_dim: int, base: float = 10000.0, scalin
     return (angle.cos() * m).float(), (angle.sin() * m).float()
 
 
-def _here(x: torch.Tensor, index: int, name: str) -> None:
-    """Refuses a tensor that is not on the cache's device: a kernel would follow its address all the same."""
-    if x.get_device() != index:
-        raise ValueError(f"{name} is on {x.device}, the cache on {f'cuda:{index}' if index >= 0 else 'cpu'}")
+def _elsewhere(x: torch.Tensor, index: int, name: str) -> ValueError:
+    """A tensor that is not on the cache's device: a kernel would follow its address all the same."""
+    return ValueError(f"{name} is on {x.device}, the cache on {f'cuda:{index}' if index >= 0 else 'cpu'}")
 
 
 def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str, index: int) -> tuple[int, int]:
@@ -93,7 +92,8 @@ def _rows(x: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str, in
     stride = x.stride()
     if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{name}: the heads of a row must be contiguous")
-    _here(x, index, name)
+    if x.get_device() != index:
+        raise _elsewhere(x, index, name)
     return x.data_ptr(), stride[0] if rows > 1 else heads * dim
 
 
@@ -102,7 +102,8 @@ def _out(x: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, name: 
         return torch.empty(shape, dtype=dtype, device=like.device)
     if x.shape != shape or x.dtype is not dtype or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
-    _here(x, index, name)
+    if x.get_device() != index:
+        raise _elsewhere(x, index, name)
     return x
 
 
@@ -203,6 +204,16 @@ class KVCache:
             return stream.cuda_stream
         return torch._C._cuda_getCurrentRawStream(self._index)
 
+    def _away(self):
+        """What makes the cache's device the current one, or None where it is: launches, outputs and the number of SMs
+        that a call counts on are the current device's."""
+        if self._index < 0:
+            return None
+        try:
+            return None if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
+        except RuntimeError:  # no driver: what is wrong with the arguments is said first
+            return None
+
     def _on(self, batch: KVBatch) -> None:
         """Refuses what a kernel must not follow: a batch of another device, a cache in host memory."""
         if batch._index != self._index:
@@ -225,6 +236,11 @@ class KVCache:
 
         Returns the rotated queries and, where k_out / v_out are given or
         `held` is set, the keys and values as the cache holds them (else None)."""
+        away = self._away()
+        if away is not None:
+            with away:
+                return self.append(batch, q, k, v, cos, sin, rotary_dim, interleaved, positions, q_out, k_out, v_out, held,
+                                   stream)
         d, n_kv, n, index = self.head_dim, self.n_kv_heads, batch.n_rows, self._index
         dtype = k.dtype
         if dtype not in DTYPES:
@@ -249,13 +265,16 @@ class KVCache:
                     cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or \
                     not cos.is_contiguous() or not sin.is_contiguous():
                 raise ValueError(f"cos and sin must be contiguous float32 [positions][{rotary_dim // 2}]")
-            _here(cos, index, "cos")
-            _here(sin, index, "sin")
+            if cos.get_device() != index:
+                raise _elsewhere(cos, index, "cos")
+            if sin.get_device() != index:
+                raise _elsewhere(sin, index, "sin")
             cos_at, sin_at, n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
         if positions is not None:
             if positions.dtype is not torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
                 raise ValueError("positions must be contiguous int32 [n_rows]")
-            _here(positions, index, "positions")
+            if positions.get_device() != index:
+                raise _elsewhere(positions, index, "positions")
             positions_at = positions.data_ptr()
         self._on(batch)
         p = A.KvAppendParams(q_at, k_at, v_at, q_stride, k_stride, v_stride, cos_at, sin_at, positions_at, q_to, k_to,
@@ -269,6 +288,10 @@ class KVCache:
                scores=None, stream=None):
         """Blocks that each row and key/value head reads: ids int32 and scores
         f32 [n_rows][n_kv_heads][n_select], ascending blocks, -1 / -inf fill."""
+        away = self._away()
+        if away is not None:
+            with away:
+                return self.select(batch, q, n_select, first, recent, ids, scores, stream)
         heads, n, index = self._heads(q), batch.n_rows, self._index
         at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q", index)
         shape = (n, self.n_kv_heads, n_select)
@@ -292,6 +315,10 @@ class KVCache:
         reads (select's ids); key_bits int32 [n_seqs][words]: a bit per token,
         0 hides it (filtered out or evicted).  scale defaults to
         head_dim^-0.5."""
+        away = self._away()
+        if away is not None:
+            with away:
+                return self.attend(batch, q, scale, causal, window, selected, key_bits, out, lse, stream)
         heads, n, d, index = self._heads(q), batch.n_rows, self.head_dim, self._index
         at, stride = _rows(q, n, heads, d, q.dtype, "q", index)
         out = _out(out, (n, heads, d), q.dtype, q, "out", index)
@@ -301,13 +328,15 @@ class KVCache:
             if selected.dtype is not torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
                     selected.shape[:2] != (n, self.n_kv_heads):
                 raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width]")
-            _here(selected, index, "selected")
+            if selected.get_device() != index:
+                raise _elsewhere(selected, index, "selected")
             selected_at, n_select = selected.data_ptr(), selected.shape[2]
         if key_bits is not None:
             if key_bits.dtype is not torch.int32 or key_bits.dim() != 2 or not key_bits.is_contiguous() or \
                     key_bits.shape[0] != batch.n_seqs:
                 raise ValueError("key_bits must be contiguous int32 [n_seqs][words]")
-            _here(key_bits, index, "key_bits")
+            if key_bits.get_device() != index:
+                raise _elsewhere(key_bits, index, "key_bits")
             bits_at, words = key_bits.data_ptr(), key_bits.shape[1]
         self._on(batch)
         ref = C.byref(A.KvAttentionParams(at, stride, selected_at, bits_at, out.data_ptr(), lse.data_ptr(),

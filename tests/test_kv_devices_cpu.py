@@ -76,3 +76,36 @@ def test_parts_of_a_cache_and_of_a_batch_are_on_one_device():
     for status in (torch.zeros(1, dtype=torch.int32, device="meta"), torch.zeros(1), torch.zeros(0, dtype=torch.int32)):
         with pytest.raises(ValueError, match="status must be"):
             KV.KVBatch(*args, status=status)
+
+
+@pytest.mark.parametrize("op", ["append", "select", "attend"])
+def test_a_call_runs_on_the_device_of_its_cache(op, monkeypatch):
+    """Another device is current: the library is called, and asked for its scratch, with the cache's device current, and
+    the other one is current again behind the call."""
+    cache, batch, calls = setting()
+    current, seen = [3], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*_):
+                seen.append((name, current[0]))
+                return 256 if name.endswith("bytes") else 0
+            return call
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    cache._lib = Library()
+    getattr(cache, op)(batch, **calls[op])
+    assert seen and {device for _, device in seen} == {0}
+    assert current == [3]
