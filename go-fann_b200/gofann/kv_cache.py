@@ -12,9 +12,12 @@ attention reads all blocks or the picked ones.
     ids, _ = cache.select(batch, q, n_select=64, first=1, recent=2)
     out, lse = cache.attend(batch, q, selected=ids)
 
-Calls run on the current stream of the cache's device (or on `stream`).
-Scratch belongs to the batch object, so calls of one batch object are ordered
-on one stream.  There is no CPU or torch fallback.
+Calls run on the current stream of the cache's device, or on `stream`: then
+their outputs and scratch are memory of that stream, and their arguments are
+kept for it; the caller orders it behind what makes the arguments.  Scratch
+belongs to the batch object, one for each stream, and is kept until the batch
+object goes, as a captured graph needs it.  Outputs carry no gradient.  There
+is no CPU or torch fallback.
 """
 from __future__ import annotations
 
@@ -138,18 +141,22 @@ class KVBatch:
                                 row_offset=row_offset.data_ptr(), status=self.status.data_ptr(), n_seqs=n_seqs,
                                 max_pages=int(page_table.shape[1]), n_rows=self.n_rows, max_rows=self.max_rows)
         self._ref = C.byref(self.struct)
-        self._scratch = None
+        self._scratch = {}  # by stream: (address, bytes) of its newest buffer
+        self._buffers = []  # all of them: a graph may hold an outgrown one's address
         self._needs = {}
 
-    def scratch(self, key: tuple, need) -> tuple[int, int]:
-        """Address and size of the device scratch of a call (kept, grown on
-        demand); `need` tells the bytes, once for each `key`, a call's sizes."""
+    def scratch(self, stream: int, key: tuple, need) -> tuple[int, int]:
+        """Address and size of the device scratch of a call on `stream`, the
+        current one (kept, grown on demand); `need` tells the bytes, once for
+        each `key`, a call's sizes."""
         n_bytes = self._needs.get(key)
         if n_bytes is None:
             n_bytes = self._needs[key] = max(int(need()), 256)
-        if self._scratch is None or self._scratch.numel() < n_bytes:
-            self._scratch = torch.empty(n_bytes, dtype=torch.uint8, device=self.page_table.device)
-        return self._scratch.data_ptr(), n_bytes
+        got = self._scratch.get(stream)
+        if got is None or got[1] < n_bytes:
+            self._buffers.append(torch.empty(n_bytes, dtype=torch.uint8, device=self.page_table.device))
+            got = self._scratch[stream] = (self._buffers[-1].data_ptr(), n_bytes)
+        return got
 
     def check(self) -> None:
         """Raises where a call found a page, position, length or row out of range (synchronises)."""
@@ -199,27 +206,34 @@ class KVCache:
                    bounds=torch.zeros((n_pages, n_kv_heads, 2, head_dim), dtype=torch.int8, device=device),
                    bound_scale=torch.zeros((n_pages, n_kv_heads), dtype=torch.float32, device=device))
 
-    def _stream(self, stream) -> int:
-        if stream is not None:
-            return stream.cuda_stream
-        return torch._C._cuda_getCurrentRawStream(self._index)
-
-    def _away(self):
-        """What makes the cache's device the current one, or None where it is: launches, outputs and the number of SMs
-        that a call counts on are the current device's."""
+    def _away(self, stream):
+        """What makes `stream` and the cache's device the current ones, or None where nothing has to: launches, outputs,
+        scratch and the number of SMs that a call counts on are the current ones'."""
         if self._index < 0:
             return None
+        if stream is not None:
+            if stream.device_index != self._index:
+                raise ValueError(f"the stream is of cuda:{stream.device_index}, the cache on cuda:{self._index}")
+            return torch.cuda.stream(stream)
         try:
             return None if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
         except RuntimeError:  # no driver: what is wrong with the arguments is said first
             return None
 
-    def _on(self, batch: KVBatch) -> None:
-        """Refuses what a kernel must not follow: a batch of another device, a cache in host memory."""
+    def _keep(self, stream, batch: KVBatch, *tensors) -> None:
+        """Keeps the memory of a call's arguments until `stream` has run it."""
+        for t in (self.pages, self.bounds, self.bound_scale, batch.page_table, batch.seq_len, batch.row_offset, batch.status,
+                  *tensors):
+            if t is not None:
+                t.record_stream(stream)
+
+    def _on(self, batch: KVBatch) -> int:
+        """The current stream; refuses what a kernel must not follow: a batch of another device, a cache in host memory."""
         if batch._index != self._index:
             raise ValueError(f"the batch is on {batch.page_table.device}, the cache on {self.device}")
         if self._index < 0:
             raise ValueError(f"the cache is on {self.device}: its operators run on a GPU")
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def _heads(self, q: torch.Tensor) -> int:
         shape = q.shape
@@ -236,11 +250,13 @@ class KVCache:
 
         Returns the rotated queries and, where k_out / v_out are given or
         `held` is set, the keys and values as the cache holds them (else None)."""
-        away = self._away()
+        away = self._away(stream)
         if away is not None:
             with away:
-                return self.append(batch, q, k, v, cos, sin, rotary_dim, interleaved, positions, q_out, k_out, v_out, held,
-                                   stream)
+                got = self.append(batch, q, k, v, cos, sin, rotary_dim, interleaved, positions, q_out, k_out, v_out, held)
+            if stream is not None:
+                self._keep(stream, batch, q, k, v, cos, sin, positions, q_out, k_out, v_out)
+            return got
         d, n_kv, n, index = self.head_dim, self.n_kv_heads, batch.n_rows, self._index
         dtype = k.dtype
         if dtype not in DTYPES:
@@ -276,10 +292,10 @@ class KVCache:
             if positions.get_device() != index:
                 raise _elsewhere(positions, index, "positions")
             positions_at = positions.data_ptr()
-        self._on(batch)
+        now = self._on(batch)
         p = A.KvAppendParams(q_at, k_at, v_at, q_stride, k_stride, v_stride, cos_at, sin_at, positions_at, q_to, k_to,
                              v_to, DTYPES[dtype], heads, n_positions, rotary_dim, 1 if interleaved else 0)
-        status = self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), self._stream(stream))
+        status = self._lib.gofann_kv_append(self._ref, batch._ref, C.byref(p), now)
         if status:
             A.check(status, "gofann_kv_append")
         return q_out if q is not None else None, k_out, v_out
@@ -288,21 +304,24 @@ class KVCache:
                scores=None, stream=None):
         """Blocks that each row and key/value head reads: ids int32 and scores
         f32 [n_rows][n_kv_heads][n_select], ascending blocks, -1 / -inf fill."""
-        away = self._away()
+        away = self._away(stream)
         if away is not None:
             with away:
-                return self.select(batch, q, n_select, first, recent, ids, scores, stream)
+                got = self.select(batch, q, n_select, first, recent, ids, scores)
+            if stream is not None:
+                self._keep(stream, batch, q, ids, scores)
+            return got
         heads, n, index = self._heads(q), batch.n_rows, self._index
         at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q", index)
         shape = (n, self.n_kv_heads, n_select)
         ids = _out(ids, shape, torch.int32, q, "ids", index)
         scores = _out(scores, shape, torch.float32, q, "scores", index)
-        self._on(batch)
+        now = self._on(batch)
         ref = C.byref(A.KvSelectParams(at, stride, ids.data_ptr(), scores.data_ptr(), DTYPES[q.dtype], heads, n_select,
                                        first, recent))
-        scratch, size = batch.scratch((0, heads, self.n_kv_heads, self.head_dim, n_select),
+        scratch, size = batch.scratch(now, (0, heads, self.n_kv_heads, self.head_dim, n_select),
                                       lambda: self._lib.gofann_kv_select_scratch_bytes(self._ref, batch._ref, ref))
-        status = self._lib.gofann_kv_select(self._ref, batch._ref, ref, scratch, size, self._stream(stream))
+        status = self._lib.gofann_kv_select(self._ref, batch._ref, ref, scratch, size, now)
         if status:
             A.check(status, "gofann_kv_select")
         return ids, scores
@@ -315,10 +334,13 @@ class KVCache:
         reads (select's ids); key_bits int32 [n_seqs][words]: a bit per token,
         0 hides it (filtered out or evicted).  scale defaults to
         head_dim^-0.5."""
-        away = self._away()
+        away = self._away(stream)
         if away is not None:
             with away:
-                return self.attend(batch, q, scale, causal, window, selected, key_bits, out, lse, stream)
+                got = self.attend(batch, q, scale, causal, window, selected, key_bits, out, lse)
+            if stream is not None:
+                self._keep(stream, batch, q, selected, key_bits, out, lse)
+            return got
         heads, n, d, index = self._heads(q), batch.n_rows, self.head_dim, self._index
         at, stride = _rows(q, n, heads, d, q.dtype, "q", index)
         out = _out(out, (n, heads, d), q.dtype, q, "out", index)
@@ -338,13 +360,13 @@ class KVCache:
             if key_bits.get_device() != index:
                 raise _elsewhere(key_bits, index, "key_bits")
             bits_at, words = key_bits.data_ptr(), key_bits.shape[1]
-        self._on(batch)
+        now = self._on(batch)
         ref = C.byref(A.KvAttentionParams(at, stride, selected_at, bits_at, out.data_ptr(), lse.data_ptr(),
                                           d ** -0.5 if scale is None else scale, DTYPES[q.dtype], heads, n_select, words,
                                           1 if causal else 0, window))
-        scratch, size = batch.scratch((1, heads, self.n_kv_heads, d, n_select),
+        scratch, size = batch.scratch(now, (1, heads, self.n_kv_heads, d, n_select),
                                       lambda: self._lib.gofann_kv_attention_scratch_bytes(self._ref, batch._ref, ref))
-        status = self._lib.gofann_kv_attention(self._ref, batch._ref, ref, scratch, size, self._stream(stream))
+        status = self._lib.gofann_kv_attention(self._ref, batch._ref, ref, scratch, size, now)
         if status:
             A.check(status, "gofann_kv_attention")
         return out, lse
