@@ -348,8 +348,8 @@ class KVCache:
         selected_at, n_select, bits_at, words = None, 0, None, 0
         if selected is not None:
             if selected.dtype is not torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
-                    selected.shape[:2] != (n, self.n_kv_heads):
-                raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width]")
+                    selected.shape[:2] != (n, self.n_kv_heads) or not selected.shape[2]:
+                raise ValueError(f"selected must be contiguous int32 [{n}][{self.n_kv_heads}][width from 1]")
             if selected.get_device() != index:
                 raise _elsewhere(selected, index, "selected")
             selected_at, n_select = selected.data_ptr(), selected.shape[2]
@@ -359,7 +359,8 @@ class KVCache:
                 raise ValueError("key_bits must be contiguous int32 [n_seqs][words]")
             if key_bits.get_device() != index:
                 raise _elsewhere(key_bits, index, "key_bits")
-            bits_at, words = key_bits.data_ptr(), key_bits.shape[1]
+            # (no words hide every token; their tensor has no address, which would stand for no mask)
+            bits_at, words = key_bits.data_ptr() or batch.page_table.data_ptr(), key_bits.shape[1]
         now = self._on(batch)
         ref = C.byref(A.KvAttentionParams(at, stride, selected_at, bits_at, out.data_ptr(), lse.data_ptr(),
                                           d ** -0.5 if scale is None else scale, DTYPES[q.dtype], heads, n_select, words,
