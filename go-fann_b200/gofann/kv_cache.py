@@ -313,6 +313,8 @@ class KVCache:
             return got
         heads, n, index = self._heads(q), batch.n_rows, self._index
         at, stride = _rows(q, n, heads, self.head_dim, q.dtype, "q", index)
+        if not (0 <= first <= A.U32MAX and 0 <= recent <= A.U32MAX):
+            raise ValueError(f"first {first} and recent {recent} (blocks of n_select {n_select})")
         shape = (n, self.n_kv_heads, n_select)
         ids = _out(ids, shape, torch.int32, q, "ids", index)
         scores = _out(scores, shape, torch.float32, q, "scores", index)
@@ -345,6 +347,8 @@ class KVCache:
         at, stride = _rows(q, n, heads, d, q.dtype, "q", index)
         out = _out(out, (n, heads, d), q.dtype, q, "out", index)
         lse = _out(lse, (n, heads), torch.float32, q, "lse", index)
+        if not 0 <= window <= A.U32MAX:
+            raise ValueError(f"window {window} (0 for none, at most {A.U32MAX})")
         selected_at, n_select, bits_at, words = None, 0, None, 0
         if selected is not None:
             if selected.dtype is not torch.int32 or selected.dim() != 3 or not selected.is_contiguous() or \
