@@ -187,6 +187,35 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], float (&code)[8])
     return static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(hm)) << 16);
 }
 
+// Eight codes of a token that the page holds, from dimension d0 on, the values
+// of a key's and the params of their group.
+template <int D>
+__device__ __forceinline__ uint32_t held_key(const uint8_t* chunk, int token, int d0, float (&x)[8], float (&code)[8])
+{
+    const int g = 2 * (token >> 4) + (token & 1), kt = (token >> 2) & 3, r = (token >> 1) & 1, grp = d0 / kKvGroup;
+    const uint32_t sm = reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kKeyParams)[kv_param_word<D>(token) + grp];
+    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffff)));
+    const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int d = d0 + k, tj = (d >> 2) & 15, n = (d >> 1) & 1, e = d & 1;
+        code[k] = static_cast<float>((chunk[(((kt * KvChunk<D>::kGroups + grp) * 8 + g) * 16 + tj) * 4 + 2 * e + r] >> (4 * n)) & 15);
+        x[k] = __fadd_rn(__fmul_rn(code[k], s), m);
+    }
+    return sm;
+}
+template <int D>
+__device__ __forceinline__ uint32_t held_value(const uint8_t* chunk, int token, int d0, float (&code)[8])
+{
+    const int t = token >> 4, kt = (token >> 2) & 3, n = (token >> 1) & 1, e = token & 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int d = d0 + k, dt = d >> 4, r = (d >> 3) & 1, g = d & 7;
+        code[k] = static_cast<float>((chunk[KvChunk<D>::kValueCodes + (((dt * 8 + g) * 4 + t) * 4 + kt) * 4 + 2 * e + r] >> (4 * n)) & 15);
+    }
+    return reinterpret_cast<const uint32_t*>(chunk + KvChunk<D>::kValueParams)[kv_param_word<D>(token) + d0 / kKvGroup];
+}
+
 // The page words [i] of this thread, and the nibbles of them that the rows
 // [lo, hi) of the page write.
 __device__ __forceinline__ uint32_t key_mask(int i, int G, int lo, int hi)
@@ -230,15 +259,21 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
     __shared__ uint32_t params[2][kKvPage][G];
     __shared__ __align__(16) float high_of[kVectors + kParts][D], low_of[kVectors + kParts][D];
     __shared__ float top[kAppendThreads / 32];
+    __shared__ int missing;  // whether a row has no position in the tables
 
     const uint32_t head = blockIdx.y;
     const int lane = threadIdx.x & 31;
     if (blockIdx.x == 0 && head == 0 && batch.status) {
+        kv_check_sequences(batch, threadIdx.x, kAppendThreads);
         for (uint32_t s = threadIdx.x; s < batch.n_seqs; s += kAppendThreads) {
             int first, n;
             kv_rows(batch, s, first, n);
-            if (__ldg(batch.seq_len + s) > batch.max_pages * GOFANN_KV_PAGE || n > kv_len(batch, s)) kv_invalid(batch);
+            if (n > kv_len(batch, s)) kv_invalid(batch);  // rows before the sequence's first token
         }
+    }
+    if (kMode != kRotateNone) {
+        if (threadIdx.x == 0) missing = 0;  // (a flag in registers: chunks of 2043 rows 47 us instead of 45)
+        __syncthreads();
     }
     uint32_t seq, at;
     if (!kv_find(batch.n_seqs, blockIdx.x, [&](uint32_t s) { return touched_pages(batch, s); }, seq, at)) return;
@@ -332,10 +367,12 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) next[a] = fetch(part + a * share);
         float c[8], s[8];
+        bool write = on;  // not where the tables have no such position
         if (kMode != kRotateNone) {
             int pos = p.positions ? __ldg(p.positions + row) : base + (on ? token : lo);
             if (pos < 0 || static_cast<uint32_t>(pos) >= p.n_positions) {
-                if (d0 == 0) kv_invalid(batch);
+                if (d0 == 0) missing = 1;
+                write = false;
                 pos = 0;
             }
             load_angles<kMode>(p, pos, d0, c, s);
@@ -350,7 +387,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
             float x[8];
             unpack8<kBf16>(raw, x);
             if (kMode != kRotateNone) rotate8<kMode, kBf16>(p, raw, d0, c, s, low_of[vec], x);
-            if (on && kind < n_q) *reinterpret_cast<uint4*>(q_out + kind * D) = pack8<kBf16>(x);
+            if (write && kind < n_q) *reinterpret_cast<uint4*>(q_out + kind * D) = pack8<kBf16>(x);
         }
         float x[8], code[8];
         unpack8<kBf16>(raw_k, x);
@@ -358,7 +395,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
         if (kMode != kRotateNone) rotate8<kMode, kBf16>(p, raw_k, d0, c, s, low_of[vec], x);
         const uint32_t kp_word = quantise8(x, code);
         const uint64_t kv_out = (static_cast<uint64_t>(row) * cache.n_kv_heads + head) * D + d0;
-        const bool mine = on && part == 0;
+        const bool mine = write && part == 0;
         if (mine) {
             uint32_t c8[2] = {0, 0};
 #pragma unroll
@@ -389,6 +426,26 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 128 ? 4 : 3)
         *reinterpret_cast<float4*>(&low_of[vec][d0 + 4]) = make_float4(low[4], low[5], low[6], low[7]);
     }
     __syncthreads();
+    if (kMode != kRotateNone && missing) {
+        if (threadIdx.x == 0) kv_invalid(batch);
+        // rows that are not written: their places keep the tokens that they hold
+        for (int token = lo + vec; token < hi; token += kVectors) {
+            const int pos = p.positions ? __ldg(p.positions + first_row + base + token - start) : base + token;
+            if (pos >= 0 && static_cast<uint32_t>(pos) < p.n_positions) continue;
+            float x[8], code[8];
+            params[0][token][d0 / kKvGroup] = held_key<D>(chunk, token, d0, x, code);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                key_codes[token * kKeyRow + d0 + k] = static_cast<uint8_t>(code[k]);
+                high_of[vec][d0 + k] = fmaxf(high_of[vec][d0 + k], x[k]);
+                low_of[vec][d0 + k] = fminf(low_of[vec][d0 + k], x[k]);
+            }
+            params[1][token][d0 / kKvGroup] = held_value<D>(chunk, token, d0, code);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) value_codes[(d0 + k) * kValueRow + token] = static_cast<uint8_t>(code[k]);
+        }
+        __syncthreads();
+    }
 
     // ---- merge the codes into the page's words
 #pragma unroll

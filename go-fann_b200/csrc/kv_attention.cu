@@ -780,6 +780,7 @@ __global__ void __launch_bounds__(Attend<D, NT>::kThreads, 1) kv_attend_kernel(g
             return static_cast<unsigned long long>(w0 < w1 ? w0 : ~0ull);
         },
         from);
+    if (blockIdx.x == 0) kv_check_sequences(batch, threadIdx.x, Cfg::kThreads);
     if (u0 >= u1) return;
 
     bool alive = true;  // false once a wait has run out

@@ -558,6 +558,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
         }
         if (lane == 0) start = it;
     }
+    if (warp == 2 && blockIdx.x == 0) kv_check_sequences(batch, lane, 32);
     if (warp == 1 && lane == 0) {
         for (int i = 0; i < kRaw; ++i) {
             barrier_init(raw_full + 8 * i, 1);

@@ -35,26 +35,33 @@ __device__ __forceinline__ int kv_param_word(int token)
 }
 
 // ------------------------------------------------------------- the sequences
-// Lengths and rows of a sequence, clamped to what the tables hold so that no
-// wrong entry is followed.
+// Lengths and rows of a sequence.  A length that the table does not hold
+// counts as 0 and offsets that are out of range as no rows: cut to what is in
+// range they would move the rows to other positions, where append would write
+// over cached tokens.
 __device__ __forceinline__ int kv_len(const gofann_kv_batch& b, uint32_t s)
 {
-    const uint32_t cap = b.max_pages * GOFANN_KV_PAGE;
     const uint32_t n = __ldg(b.seq_len + s);
-    return static_cast<int>(n < cap ? n : cap);
+    return n <= b.max_pages * GOFANN_KV_PAGE ? static_cast<int>(n) : 0;
 }
 __device__ __forceinline__ void kv_rows(const gofann_kv_batch& b, uint32_t s, int& first, int& count)
 {
-    uint32_t lo = __ldg(b.row_offset + s), hi = __ldg(b.row_offset + s + 1);
-    lo = lo < b.n_rows ? lo : b.n_rows;
-    hi = hi < b.n_rows ? hi : b.n_rows;
+    const uint32_t lo = __ldg(b.row_offset + s), hi = __ldg(b.row_offset + s + 1);
     first = static_cast<int>(lo);
-    count = hi > lo ? static_cast<int>(hi - lo) : 0;
+    count = lo <= hi && hi <= b.n_rows ? static_cast<int>(hi - lo) : 0;
 }
 
 __device__ __forceinline__ void kv_invalid(const gofann_kv_batch& b)
 {
     if (b.status) atomicExch(b.status, GOFANN_ERR_INVALID);
+}
+// Reports such lengths and offsets, the sequences from `s` on in steps.
+__device__ __forceinline__ void kv_check_sequences(const gofann_kv_batch& b, uint32_t s, uint32_t step)
+{
+    for (; s < b.n_seqs; s += step) {
+        const uint32_t lo = __ldg(b.row_offset + s), hi = __ldg(b.row_offset + s + 1);
+        if (lo > hi || hi > b.n_rows || __ldg(b.seq_len + s) > b.max_pages * GOFANN_KV_PAGE) kv_invalid(b);
+    }
 }
 
 // The sequence that holds item `flat` when sequence s has count(s) items, and

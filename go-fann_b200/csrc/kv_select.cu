@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache c
 {
     constexpr int kRows = kPickThreads / 32 / kWarps;  // rows of a thread block
     __shared__ uint32_t sums[2][8];
+    if (blockIdx.x == 0) kv_check_sequences(batch, threadIdx.x, kPickThreads);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, place = threadIdx.x % (32 * kWarps);
     const uint64_t item = static_cast<uint64_t>(blockIdx.x) * kRows + warp / kWarps;
     if (item >= static_cast<uint64_t>(batch.n_rows) * cache.n_kv_heads) {  // whole warps (kWarps 8: whole blocks)
@@ -471,6 +472,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_long_kernel(gofann_kv_ca
     __shared__ uint32_t warp_sum[kPickThreads / 32][2];
     __shared__ uint32_t found_digit, found_rank;
     const uint32_t row = blockIdx.x, head = blockIdx.y;
+    if (row == 0 && head == 0) kv_check_sequences(batch, threadIdx.x, kPickThreads);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t seq = 0, at = 0;
     const auto rows = [&](uint32_t s) {

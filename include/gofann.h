@@ -702,8 +702,14 @@ typedef struct gofann_kv_batch {
     const int32_t* page_table;   /* device [n_seqs][max_pages]: pages of a sequence in token order */
     const uint32_t* seq_len;     /* device [n_seqs], at most max_pages * GOFANN_KV_PAGE */
     const uint32_t* row_offset;  /* device [n_seqs + 1], ascending from 0 to n_rows */
-    int32_t* status;             /* device [1] error word or NULL: set to GOFANN_ERR_INVALID where a page,
-                                    position, length or row is out of range; that item is skipped */
+    int32_t* status;             /* device [1] error word or NULL: set to GOFANN_ERR_INVALID where something is
+                                    out of range, and that is skipped.  A page: nothing is written there, its
+                                    tokens are hidden.  A length above the table's: the sequence counts as
+                                    empty (its rows see and write nothing).  Row offsets that do not ascend or
+                                    pass n_rows: the sequence has no rows.  gofann_kv_append also sets it for
+                                    rows before the sequence's first token, which the others give no keys, and
+                                    for rotary positions that the tables do not have: such a row is not
+                                    written, its place in the page keeps the token that it holds */
     uint32_t n_seqs;
     uint32_t max_pages;
     uint32_t n_rows;
