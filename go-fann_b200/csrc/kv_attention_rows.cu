@@ -38,7 +38,10 @@
 // of 16 bits anyway); logits, sums and the output are f32.  A column's weights are relative to a
 // reference, its first maximum, times 2^7; the reference moves up to the
 // maximum only where 32 weights sum to more than 2^15 (f16 ends at 2^16), so
-// the maximum is rarely looked for and the output rarely rescaled.
+// the maximum is rarely looked for and the output rarely rescaled.  The output
+// leaves tensor memory for an f32 sum every 8192 tokens (kFold), as the tensor
+// cores' own sum of values of one sign drifts (chunks of two prompts 1306 ->
+// 1315 us).
 #include "kv_attention.cuh"
 
 namespace gofann {
@@ -56,6 +59,13 @@ constexpr int kRowThreads = 32 * (kLoadWarp + 3);  // whole warpgroups
 constexpr int kSoftmaxRegs = 104, kDecodeRegs = 72, kOtherRegs = 56;
 constexpr float kHead = 7.0f;      // log2 of a weight at the reference
 constexpr float kMost = 32768.0f;  // sum of 32 weights from which the reference moves up
+// Steps after which the output so far leaves tensor memory.  The tensor cores
+// truncate their sums, so a long one falls short: by 5e-8 of itself for every
+// product of 16 tokens, 4e-4 over 131072 tokens (an f16's half unit is 2.4e-4
+// to 4.9e-4).  512 products of 8192 tokens lose 2^-15 at the most; the parts
+// are added in f32, rounded to nearest.
+constexpr int kFold = 64;
+static_assert((kFold & (kFold - 1)) == 0, "steps are counted modulo it");
 
 template <int D>
 struct Rows {
@@ -503,9 +513,55 @@ __device__ __forceinline__ uint64_t steps_per_block(uint64_t total, uint32_t blo
 
 // A block's partial result in scratch: [256] base, [256] sum, [D][256]
 // values, so that the threads of a warp, a column each, write side by side;
-// two per block (its first item, and its last if that is another).
+// two per block (its first item, and its last if that is another).  One more
+// per block, behind those, is where its output is folded to: the reference of
+// the weights in place of the base.
 template <int D>
 constexpr size_t kRowPartFloats = kWidth * (D + 2);
+
+// Where this thread's column of a block's output is folded to.
+template <int D>
+__device__ __forceinline__ float* fold_column(float* parts)
+{
+    return parts + (2ull * gridDim.x + blockIdx.x) * kRowPartFloats<D> + threadIdx.x;
+}
+// The output so far, by the reference `ref`, joins what was folded before
+// (unless it is the first); the next product starts it anew.  These are rare
+// and kept out of the step's code, whose registers they would take.
+template <int D>
+__device__ __noinline__ void fold_output(uint32_t addr, float* parts, float ref, float unit, bool first)
+{
+    float* acc = fold_column<D>(parts);
+    const float then = first ? kNegInf : *acc, f = then == kNegInf ? 0.0f : exp2_fast((then - ref) * unit);
+    *acc = ref;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        uint32_t r[16];
+        tensor_load16(addr + c, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float* at = acc + (2 + c + i) * kWidth;
+            *at = f > 0.0f ? fmaf(*at, f, __uint_as_float(r[i])) : __uint_as_float(r[i]);
+        }
+    }
+}
+// What was folded joins the rest of the output in tensor memory.
+template <int D>
+__device__ __noinline__ void unfold_output(uint32_t addr, float* parts, float ref, float unit)
+{
+    const float* acc = fold_column<D>(parts);
+    const float f = *acc == kNegInf ? 0.0f : exp2_fast((*acc - ref) * unit);
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        uint32_t r[16];
+        tensor_load16(addr + c, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            r[i] = __float_as_uint(f > 0.0f ? fmaf(acc[(2 + c + i) * kWidth], f, __uint_as_float(r[i])) : __uint_as_float(r[i]));
+        tensor_store16(addr + c, r);
+    }
+    tensor_wait_store();
+}
 
 // Place of a column's row in out and lse.
 __device__ __forceinline__ uint64_t output_row(const gofann_kv_attention_params& p, int group, int first_row, uint32_t head,
@@ -720,7 +776,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
 #pragma unroll
                 for (int i = 0; i < 2 * kTiles; ++i) {
                     const int tile = i % kTiles, h = i / kTiles;
-                    ok = ok && all_wait(p_full + 16 * tile + 8 * h, g) && output(tile, h, g, j > 0 || h > 0);
+                    ok = ok && all_wait(p_full + 16 * tile + 8 * h, g) && output(tile, h, g, j % kFold > 0 || h > 0);
                     if (!ok) break;
                     if (h == 0) continue;
                     if (more) {
@@ -851,13 +907,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
 
             float ref = kNegInf;
             uint64_t l2 = 0;  // two parts of the sum of weights
-            const int from = it.from, to = it.to;
-            int key0 = (it.lo + 2 * from) * kKvPage;
-            for (int j = from; j < to && ok; ++j, ++g, ++sg) {
+            const int steps = it.to - it.from;
+            int key0 = (it.lo + 2 * it.from) * kKvPage;
+            for (int j = 0; j < steps && ok; ++j, ++g, ++sg) {
                 for (int h = 0; h < 2; ++h, key0 += kKvPage) {
                     ok = wait(s_full + 16 * tile + 8 * h, sg);
                     if (!ok) break;
                     fence_after();
+                    if (h == 0 && j > 0 && j % kFold == 0) fold_output<D>(o_at, parts, ref, unit, j == kFold);
                     const uint32_t sh = s_at + h * kKvPage;
                     const uint64_t shown = step_shown[(g & 7) * 2 + h];
                     if (shown != ~0ull || key0 + kKvPage - 1 > warp_limit || key0 <= warp_low) {
@@ -911,7 +968,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                                 tensor_wait_store();
                                 scale_weights(sh, f);
                             }
-                            if (j > from || h > 0) {
+                            if (h > 0 || j % kFold > 0) {
                                 // behind the product of the page before
                                 ok = h == 0 || wait(o_half + 8 * tile, g);
                                 fence_after();
@@ -935,6 +992,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             if (!ok) break;
             ++sg;
             fence_after();
+            if (steps > kFold) unfold_output<D>(o_at, parts, ref, unit);
             const float l = first_of(l2) + second_of(l2), inv = l > 0.0f ? 1.0f / l : 0.0f;
             const float at = l > 0.0f ? fmaf(ref, unit, -kHead) : kNegInf;
             const uint64_t out_row = output_row(p, group, it.first_row, it.head, at_col);
@@ -1079,7 +1137,7 @@ int launch_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, cons
 
 size_t attend_rows_scratch(uint32_t head_dim, int sms)
 {
-    return 2 * sizeof(float) * (head_dim == 64 ? kRowPartFloats<64> : kRowPartFloats<128>) * static_cast<size_t>(sms);
+    return 3 * sizeof(float) * (head_dim == 64 ? kRowPartFloats<64> : kRowPartFloats<128>) * static_cast<size_t>(sms);
 }
 
 int attend_rows(const gofann_kv_cache& cache, const gofann_kv_batch& batch, const gofann_kv_attention_params& p,
