@@ -12,6 +12,9 @@ namespace gofann {
 namespace {
 
 constexpr int kScoreThreads = 256;
+// The score of a block without a page: no number, as a product that overflows
+// is -inf and its block may be one that is always kept.
+constexpr float kNoPage = __builtin_nanf("");
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(kScoreThreads, (D == 64 ? 3 : 2) + (kGroups ==
                         float* o = out[e] + at + 8 * u + w;
                         float x = v[e][w];
                         if (kCols == 16 && chunk > 0) x = fmaxf(x, *o);
-                        if (chunk == chunks - 1) x = scale < 0.0f ? kNegInf : __fmul_rn(x, scale);
+                        if (chunk == chunks - 1) x = scale < 0.0f ? kNoPage : __fmul_rn(x, scale);
                         *o = x;
                     }
                 }
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(gofann_kv_cache c
         key[i] = 0;
         if (b < blocks) {
             const float x = __ldcg(sc + b);
-            if (x != kNegInf) {
+            if (x == x) {
                 key[i] = b < static_cast<int>(p.n_first) || b >= blocks - static_cast<int>(p.n_recent) ? 0xffffffffu
                                                                                                         : order_key(x);
                 ++valid;
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_long_kernel(gofann_kv_ca
     const int want = static_cast<int>(p.n_select);
     const auto key_of = [&](int b) {
         const float x = __ldcg(sc + b);
-        if (x == kNegInf) return 0u;
+        if (x != x) return 0u;
         return b < static_cast<int>(p.n_first) || b >= blocks - static_cast<int>(p.n_recent) ? 0xffffffffu : order_key(x);
     };
     // the smallest key taken, and how many of its blocks (lowest first)

@@ -793,7 +793,8 @@ GOFANN_API int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_ba
  * rint(q / qs), qs = max |q| / 127 (both 0 where q is zero or not finite), u =
  * sum over d of q8 * (q8 > 0 ? largest : smallest) as an integer, score = max
  * over the query heads of the key/value head of (u * qs), times bound_scale.
- * Integers and rounded products only: the same ids on every run.  Ties go to
+ * Integers and rounded products only: the same ids on every run.  Products that
+ * overflow count as the infinities that they give.  Ties go to
  * the lowest block.  scratch: gofann_kv_select_scratch_bytes, 256-byte
  * aligned. */
 GOFANN_API size_t gofann_kv_select_scratch_bytes(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
