@@ -625,18 +625,20 @@ __device__ __forceinline__ uint64_t units_per_block(uint64_t total, uint32_t blo
 template <int D, int NT>
 constexpr size_t kPartFloats = 8 * NT * (D + 2);
 
+// A row's sum of weights is 0 where it sees no key, and no number where its
+// query holds one that is none, which its output then shows.
 template <int D>
 __device__ __forceinline__ void store_row(const Call& p, const Tile& tile, uint32_t head, int group,
                                           bool selected, int c, int d, float m, float l, const float (&o)[4])
 {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     const int col = tile.col0 + c;
     const uint64_t row = tile.first_row + (selected ? tile.row : col / group);
     const uint64_t at = row * p.n_heads + head * group + (selected ? col : col % group);
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * D + d) =
-        l > 0.0f ? make_uint2(kv_pack2(o[0] * inv, o[1] * inv, p.dtype), kv_pack2(o[2] * inv, o[3] * inv, p.dtype))
-                 : make_uint2(0u, 0u);
-    if (d == 0 && p.lse) p.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
+        l != 0.0f ? make_uint2(kv_pack2(o[0] * inv, o[1] * inv, p.dtype), kv_pack2(o[2] * inv, o[3] * inv, p.dtype))
+                  : make_uint2(0u, 0u);
+    if (d == 0 && p.lse) p.lse[at] = l != 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
 }
 
 // The rows of a whole item from the lanes that hold them: pairs of columns
@@ -657,9 +659,9 @@ __device__ __forceinline__ void store_item(const Call& p, const Tile& tile, uint
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const float l = st.l[n][c];
-            inv[c] = l > 0.0f ? 1.0f / l : 0.0f;
+            inv[c] = l != 0.0f ? 1.0f / l : 0.0f;
             if (g == 0 && p.lse && n * 8 + 2 * t + c < tile.cols)
-                p.lse[place(n * 8 + 2 * t + c)] = l > 0.0f ? (st.m[n][c] + log2f(l)) * kLn2 : kNegInf;
+                p.lse[place(n * 8 + 2 * t + c)] = l != 0.0f ? (st.m[n][c] + log2f(l)) * kLn2 : kNegInf;
         }
         const bool on = n * 8 + g < tile.cols;
         uint16_t* out = static_cast<uint16_t*>(p.out) + (on ? place(n * 8 + g) : 0) * D;
@@ -667,8 +669,8 @@ __device__ __forceinline__ void store_item(const Call& p, const Tile& tile, uint
         for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float a = inv[0] > 0.0f ? st.o[dt][n][2 * r] * inv[0] : 0.0f;
-                const float b = inv[1] > 0.0f ? st.o[dt][n][2 * r + 1] * inv[1] : 0.0f;
+                const float a = inv[0] != 0.0f ? st.o[dt][n][2 * r] * inv[0] : 0.0f;
+                const float b = inv[1] != 0.0f ? st.o[dt][n][2 * r + 1] * inv[1] : 0.0f;
                 const uint32_t w = transpose8x8(kv_pack2(a, b, p.dtype));
                 if (on) *reinterpret_cast<uint32_t*>(out + dt * 16 + 8 * r + 2 * t) = w;
             }

@@ -993,8 +993,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
             ++sg;
             fence_after();
             if (steps > kFold) unfold_output<D>(o_at, parts, ref, unit);
-            const float l = first_of(l2) + second_of(l2), inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const float at = l > 0.0f ? fmaf(ref, unit, -kHead) : kNegInf;
+            const float l = first_of(l2) + second_of(l2), inv = l != 0.0f ? 1.0f / l : 0.0f;
+            const float at = l != 0.0f ? fmaf(ref, unit, -kHead) : kNegInf;
             const uint64_t out_row = output_row(p, group, it.first_row, it.head, at_col);
             const bool whole = it.from == 0 && it.to == it.steps;
             float* part = parts + (2ull * blockIdx.x + (it.flat == u0 ? 0 : 1)) * kRowPartFloats<D>;
@@ -1010,7 +1010,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         uint2 w = make_uint2(0u, 0u);
-                        if (l > 0.0f)
+                        if (l != 0.0f)
                             w = make_uint2(kv_pack2(o[i] * inv, o[i + 1] * inv, p.dtype),
                                            kv_pack2(o[i + 2] * inv, o[i + 3] * inv, p.dtype));
                         *reinterpret_cast<uint2*>(out + i) = w;
@@ -1020,7 +1020,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv_attend_rows_kernel(gofann_k
                     for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * kWidth + col] = o[i];
                 }
             }
-            if (on && whole && p.lse) p.lse[out_row] = l > 0.0f ? (at + log2f(l)) * kLn2 : kNegInf;
+            if (on && whole && p.lse) p.lse[out_row] = l != 0.0f ? (at + log2f(l)) * kLn2 : kNegInf;
             if (on && !whole) {
                 part[col] = at;
                 part[kWidth + col] = l;
@@ -1082,11 +1082,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_rows_kernel(gofann_kv_ca
             m = top;
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) turn[lane][warp * kEach + k] = l > 0.0f ? o[k] * inv : 0.0f;
+    for (int k = 0; k < kEach; ++k) turn[lane][warp * kEach + k] = l != 0.0f ? o[k] * inv : 0.0f;
     if (warp == 0 && p.lse && c0 + lane < it.cols)
-        p.lse[output_row(p, group, it.first_row, it.head, it.col0 + c0 + lane)] = l > 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
+        p.lse[output_row(p, group, it.first_row, it.head, it.col0 + c0 + lane)] = l != 0.0f ? (m + log2f(l)) * kLn2 : kNegInf;
     __syncthreads();
     for (int i = threadIdx.x; i < kJoinColumns * (D / 2); i += kJoinThreads) {
         const int c = i / (D / 2), d = i % (D / 2) * 2;

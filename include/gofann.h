@@ -760,7 +760,8 @@ typedef struct gofann_kv_attention_params {
     const uint32_t* key_bits;    /* device [n_seqs][key_words]: bit i % 32 of word i / 32 shows token i
                                     (the layout of gofann_predicate_pass_masks; tokens beyond the words are
                                     hidden), or NULL = every token */
-    void* out;                   /* device [n_rows][n_heads][head_dim]; a row that sees no key gives 0 */
+    void* out;                   /* device [n_rows][n_heads][head_dim]; a row that sees no key gives 0, one whose
+                                    query is not finite no number */
     float* lse;                  /* device [n_rows][n_heads] natural log of the sum of exponentials (-inf for
                                     a row that sees no key), or NULL */
     float scale;                 /* of q.k, finite */
