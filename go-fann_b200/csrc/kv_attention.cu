@@ -547,7 +547,7 @@ __device__ __forceinline__ void load_query(const Call& p, const Tile& tile, uint
             sum[grp] *= 0x1p-24f;  // the unit of the codes' products
         }
         // undoes `down` and the codes' subnormals
-        const float undo = p.scale == 0.0f ? 1.0f : fmaxf(fabsf(p.scale) * kLog2e * power_of_two(24 - ex), FLT_MIN);
+        const float undo = p.scale == 0.0f ? 1.0f : fmaxf(fabsf(p.scale) * kLog2e * power_of_two(-ex) * 0x1p24f, FLT_MIN);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             q.unit[n][e] = __shfl_sync(kFull, undo, 4 * (2 * t + e));

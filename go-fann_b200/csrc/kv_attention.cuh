@@ -31,13 +31,14 @@ __device__ __forceinline__ void dense_blocks(const gofann_kv_attention_params& p
 }
 
 // The power of two that brings a query column with largest magnitude `top`
-// to [2^13, 2^14), as its exponent: every bf16 or f16 within 2^27 of the
-// largest is then an exact f16.
+// to [2^13, 2^14), as its exponent (from 2^-99 on; smaller ones stay below):
+// every f16 within 2^27 of the largest, every bf16 within 2^30, is then an
+// exact f16.  The few-column kernel scales half of the elements by another
+// 2^-4, which leaves 2^23 and 2^26.
 __device__ __forceinline__ int query_exponent(float top)
 {
-    int ex = static_cast<int>(__float_as_uint(top) >> 23);
-    ex = ex < 28 ? 28 : ex > 240 ? 240 : ex;
-    return 140 - ex;
+    const int ex = static_cast<int>(__float_as_uint(top) >> 23);
+    return 140 - (ex < 28 ? 28 : ex);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
