@@ -126,8 +126,8 @@ class KVBatch:
                 raise ValueError(f"{name} must be a contiguous int32 tensor")
             if t.device != page_table.device:
                 raise ValueError(f"{name} is on {t.device}, page_table on {page_table.device}")
-        n_seqs = int(seq_len.shape[0])
-        if page_table.dim() != 2 or page_table.shape[0] != n_seqs or tuple(row_offset.shape) != (n_seqs + 1,):
+        n_seqs = seq_len.numel()
+        if seq_len.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != n_seqs or tuple(row_offset.shape) != (n_seqs + 1,):
             raise ValueError("page_table [n_seqs][max_pages], seq_len [n_seqs] and row_offset [n_seqs + 1] disagree")
         if n_rows < 0 or not 0 <= max_rows <= n_rows:
             raise ValueError(f"n_rows {n_rows} and max_rows {max_rows}")
