@@ -737,8 +737,9 @@ __device__ __forceinline__ void look_up(const gofann_kv_cache& cache, const gofa
 // What bounds it: the instructions that turn codes into operands and join a
 // page's sums (a warp issues 94 M of them for 0.81 GB), whose fixed latencies
 // 12 to 16 warps hide in part; 54 % of the issue slots are taken.  32 rows over
-// 32768 tokens (64 query, 8 key/value heads of 128) take 170 us, 4.8 TB/s, 0.73
-// of the measured copy; one row over 131072 tokens 51 us, of which the
+// 32768 tokens (64 query, 8 key/value heads of 128) take 186 us, 4.4 TB/s, 0.67
+// of the measured copy (170 to 186 from one device to the next); one row over
+// 131072 tokens 53 us, of which the
 // partial results' join is 8; 48 rows of 64 selected blocks 70 us, 3.2 TB/s:
 // each (row, head) has its own list of pages to look up and its own join.
 template <int D, int NT, bool kSelected>

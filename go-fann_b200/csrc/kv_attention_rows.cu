@@ -20,7 +20,7 @@
 // parts are a third of them), whose operands share shared memory's port with the
 // decoded pages and tensor memory's with S and P.  Chunks of 2043 rows of two
 // prompts (32 query, 8 key/value heads of 128, up to 12289 tokens): 686
-// GFLOP of visible products in 1285 us, 534 TFLOP/s, 0.32 of a plain product's
+// GFLOP of visible products in 1315 us, 522 TFLOP/s, 0.31 of a plain product's
 // measured rate; the tensor pipe is active 40 % of the time, and the thread
 // that issues waits 0.4 of a step: for P 1850 of 7500 cycles, for values 510,
 // for keys 430.  Keys of one f16 number took 900 us.  Eight warps for values,

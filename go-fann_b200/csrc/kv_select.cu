@@ -1,5 +1,5 @@
-// kv_select.cu — the blocks of the 4-bit cache that a query reads, by an int8
-// upper bound of q.k over each block.
+// kv_select.cu — the blocks of the 4-bit cache that a query reads, by an upper
+// bound of the int8 query's product with each block's keys.
 //
 // Two launches, the second programmatic: scores of every (row, key/value head,
 // block) by int8 matrix instructions (m16n8k32: 16 query columns x 8 blocks x

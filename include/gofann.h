@@ -790,7 +790,9 @@ GOFANN_API int gofann_kv_append(const gofann_kv_cache* cache, const gofann_kv_ba
 
 /* The n_select blocks of each row and key/value head with the largest score,
  * among the blocks from the sequence's first to the row's own.  The score is
- * an upper bound of q.k over the block's keys in 8 bits: per query head q8 =
+ * an upper bound of the 8-bit query's product with the block's held keys (not
+ * of q.k: rounding q to 8 bits may lose more than the bound has room for): per
+ * query head q8 =
  * rint(q / qs), qs = max |q| / 127 (both 0 where q is zero or not finite), u =
  * sum over d of q8 * (q8 > 0 ? largest : smallest) as an integer, score = max
  * over the query heads of the key/value head of (u * qs), times bound_scale.
@@ -809,8 +811,11 @@ GOFANN_API int gofann_kv_select(const gofann_kv_cache* cache, const gofann_kv_ba
  * (causal), inside the window and shown by key_bits.  Query head h reads
  * key/value head h / (n_heads / n_kv_heads).  Logits, sums and the output are
  * accumulated in f32; weights are rounded to f16, and so are values where the
- * query rows of all sequences are many.  Every sum has a fixed order.  scratch: gofann_kv_attention_scratch_bytes,
- * 256-byte aligned. */
+ * call has many query columns: no selected blocks, and max_rows * n_heads /
+ * n_kv_heads * head_dim from 16384 on.  That is decided once for all sequences
+ * of a call, so rows of single tokens beside a prompt's chunk are faster in a
+ * call of their own.  Every sum has a fixed order.  scratch:
+ * gofann_kv_attention_scratch_bytes, 256-byte aligned. */
 GOFANN_API size_t gofann_kv_attention_scratch_bytes(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                                                     const gofann_kv_attention_params* params);
 GOFANN_API int gofann_kv_attention(const gofann_kv_cache* cache, const gofann_kv_batch* batch,
