@@ -16,8 +16,9 @@ Calls run on the current stream of the cache's device, or on `stream`: then
 their outputs and scratch are memory of that stream, and their arguments are
 kept for it; the caller orders it behind what makes the arguments.  Scratch
 belongs to the batch object, one for each stream, and is kept until the batch
-object goes, as a captured graph needs it.  Outputs carry no gradient.  There
-is no CPU or torch fallback.
+object goes, as a captured graph needs it; graphs captured from one batch
+object share it and are replayed one after the other.  Outputs carry no
+gradient.  There is no CPU or torch fallback.
 """
 from __future__ import annotations
 
